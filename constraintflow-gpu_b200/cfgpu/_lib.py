@@ -18,7 +18,7 @@ CF_RELAX_DEEPPOLY, CF_RELAX_CROWN, CF_RELAX_ZONO, CF_RELAX_IBP, CF_RELAX_CROWNIB
 CF_RELAX_DEEPPOLY_STRICT, CF_RELAX_CROWNIBP_STRICT = 5, 6
 CF_MAX_DIMS = 6
 CF_STATIC_SCRATCH_BYTES = 32 << 20
-CF_F32, CF_BOOL = 0, 1
+CF_F32, CF_BOOL, CF_BF16, CF_F16 = 0, 1, 2, 3
 OPS = dict(add=0, sub=1, mul=2, truediv=3, ge=4, gt=5, le=6, lt=7, eq=8, ne=9, and_=10, or_=11, max=12, min=13)
 UOPS = dict(neg=0, not_=1, sigmoid=2, relu=3, to_f32=4)
 
@@ -49,6 +49,21 @@ class CfProfileStats(ctypes.Structure):
 
 class CfConvGeom(ctypes.Structure):
     _fields_ = [(n, _i32) for n in ("K", "C", "ox", "oy", "ix", "iy", "kx", "ky", "sx", "sy", "px", "py")]
+
+
+class CfAdapterLayer(ctypes.Structure):
+    _fields_ = [("dtype", _i32), ("n_adapters", _i32), ("rank", _i32), ("reserved", _i32), ("n_out", _i64),
+                ("n_in", _i64), ("W_dev", _vp), ("w_rs", _i64), ("bias_dev", _vp), ("A_dev", _vp), ("a_es", _i64),
+                ("a_rs", _i64), ("B_dev", _vp), ("b_es", _i64), ("b_rs", _i64), ("scale_dev", _vp),
+                ("ranks_dev", _vp)]
+
+
+class CfAnswerRules(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("n", _i64), ("n_tokens", _i64), ("n_biases", _i64), ("allowed_words", _i64),
+                ("n_masks", _i32), ("reserved", _i32)] + \
+               [(name + "_dev", _vp) for name in ("tokens", "token_offsets", "prompt_len", "repetition", "frequency",
+                                                  "presence", "bias_ids", "bias_values", "bias_offsets", "allowed",
+                                                  "allowed_row")]
 
 
 class CfNetwork(ctypes.Structure):
@@ -94,6 +109,11 @@ def _load():
         "cf_conv_scale": (_i32, [P(CfConvGeom), _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp]),
         "cf_conv_transpose": (_i32, [P(CfConvGeom), _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i64,
                                      _i64, _i64, _vp]),
+        "cf_adapter_workspace_bytes": (_sz, [P(CfAdapterLayer), _i32, _i64, _i64]),
+        "cf_adapter_matmul": (_i32, [P(CfAdapterLayer), _i32, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _sz,
+                                     _vp]),
+        "cf_edit_logits": (_i32, [P(CfAnswerRules), _i32, _vp, _i64, _vp, _i64, _vp]),
+        "cf_answer_margin": (_i32, [P(CfAnswerRules), _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
         "cf_profile_enable": (_i32, [_i32]),
         "cf_profile_collect": (_i32, [P(CfProfileStats)]),
         "cf_last_error": (ctypes.c_char_p, []),
@@ -115,6 +135,7 @@ EXPORTED = ("cf_network_neurons", "cf_deeppoly_workspace_bytes", "cf_deeppoly_ru
             "cf_relu_relax",
             "cf_backsub_step", "cf_concretize", "cf_ew_binary", "cf_ew_unary", "cf_ew_where", "cf_ew_clamp",
             "cf_ew_any", "cf_bmm", "cf_conv_densify", "cf_conv_apply", "cf_conv_scale", "cf_conv_transpose",
+            "cf_adapter_workspace_bytes", "cf_adapter_matmul", "cf_edit_logits", "cf_answer_margin",
             "cf_input_box", "cf_spec_matrix", "cf_profile_enable", "cf_profile_collect",
             "cf_last_error", "cf_version")
 

@@ -1,6 +1,8 @@
 """Tensor-level wrappers over libcfgpu's block kernels (cf_ew_binary, cf_ew_unary,
 cf_ew_where, cf_ew_clamp, cf_ew_any, cf_bmm, cf_conv_*), used by the gbcsr mirror
-(constraintflow.gbcsr) and by the general traversal (cfgpu.general).
+(constraintflow.gbcsr) and by the general traversal (cfgpu.general), and over the
+operators for many variants of one network in a batch (cf_adapter_matmul,
+cf_edit_logits, cf_answer_margin).
 
 Operands are CUDA tensors, possibly broadcast views (zero strides); results are new
 contiguous tensors.  PyTorch only allocates the memory and supplies the stream.
@@ -191,3 +193,214 @@ def conv_transpose(g, nb, per_b, Y, ystr, W, OH, OW, out, ostr):
     _lib.check(_lib.lib.cf_conv_transpose(ctypes.byref(g), nb, per_b, Y.data_ptr(), *ystr, W.data_ptr(), OH, OW,
                                           out.data_ptr(), *ostr, _stream()), "cf_conv_transpose")
     return out
+
+
+# ------------------------------------------------- many variants of one network in a batch
+_DTYPES = {torch.float32: _lib.CF_F32, torch.bfloat16: _lib.CF_BF16, torch.float16: _lib.CF_F16}
+
+
+def _expect(name, t, dtype, shape, dev, strided=False):
+    """Refuse a tensor that is not `dtype` on `dev` of `shape` (None: any size), its last
+    dimension contiguous (strided) or all of them."""
+    ok = t.dtype == dtype and t.device == dev and t.dim() == len(shape) and \
+        all(w is None or s == w for s, w in zip(t.shape, shape))
+    if ok and strided:
+        ok = t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1
+    elif ok:
+        ok = t.is_contiguous()
+    if not ok:
+        raise Exception(f"SHAPE MISMATCH: {name} must be {dtype} {tuple('any' if w is None else w for w in shape)} on "
+                        f"{dev}{', its rows contiguous' if strided else ', contiguous'}; got {t.dtype} "
+                        f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _cuda(name, t):
+    if t.device.type != "cuda":
+        raise RuntimeError(f"{name} is on {t.device}: libcfgpu runs on CUDA tensors only (no CPU fallback)")
+    return t.device
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _row_stride(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _on(dev):
+    """Make dev the current device, for the launch, where it is not."""
+    return torch.cuda.device(dev)
+
+
+class AdapterLayer:
+    """An affine layer with low-rank adapters, one of them for each request of a batch.
+
+    W [n_out, n_in] (and bias [n_out]) are shared; adapter e adds scale[e] * B[e] @ A[e] to W,
+    with A [n_adapters, rank, n_in], B [n_adapters, n_out, rank], scale [n_adapters] float32 and,
+    optionally, ranks [n_adapters] int32, each adapter's own rank (what A and B hold beyond it
+    is not used).  W, bias, A and B are of one dtype (float32, bfloat16, float16), on one GPU.
+    The tensors are kept and read at every call: an adapter is exchanged by writing into them."""
+
+    def __init__(self, W, A, B, scale, ranks=None, bias=None):
+        dev = _cuda("W", W)
+        dt = W.dtype
+        if dt not in _DTYPES:
+            raise NotImplementedError(f"adapters over {dt} weights (float32, bfloat16 and float16 are supported)")
+        if W.dim() != 2 or A.dim() != 3:
+            raise Exception(f"SHAPE MISMATCH: W {tuple(W.shape)} and A {tuple(A.shape)} are not [n_out, n_in] and "
+                            "[n_adapters, rank, n_in]")
+        self.n_out, self.n_in = int(W.shape[0]), int(W.shape[1])
+        self.n_adapters, self.rank = int(A.shape[0]), int(A.shape[1])
+        _expect("W", W, dt, (None, None), dev, strided=True)
+        _expect("A", A, dt, (None, None, self.n_in), dev, strided=True)
+        _expect("B", B, dt, (self.n_adapters, self.n_out, self.rank), dev, strided=True)
+        _expect("scale", scale, torch.float32, (self.n_adapters,), dev)
+        if ranks is not None:
+            _expect("ranks", ranks, torch.int32, (self.n_adapters,), dev)
+        if bias is not None:
+            _expect("bias", bias, dt, (self.n_out,), dev)
+        self.device, self.dtype = dev, dt
+        self._keep = (W, A, B, scale, ranks, bias)
+
+        def strides(t):
+            rs = t.stride(1) if t.shape[1] > 1 else t.shape[2]
+            return (t.stride(0) if t.shape[0] > 1 else 0), max(rs, 0)
+        a_es, a_rs = strides(A)
+        b_es, b_rs = strides(B)
+        self.c = _lib.CfAdapterLayer(_DTYPES[dt], self.n_adapters, self.rank, 0, self.n_out, self.n_in, W.data_ptr(),
+                                     _row_stride(W), _ptr(bias), A.data_ptr(), a_es, a_rs, B.data_ptr(), b_es, b_rs,
+                                     scale.data_ptr(), _ptr(ranks))
+        self._ref = ctypes.byref(self.c)
+
+
+def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
+    """Rows of many requests through `layer` (an AdapterLayer), each with its request's adapter.
+
+    x [T, n_in] -> x @ W.T + bias + scale_e * (x @ A_e.T) @ B_e.T  [T, n_out]; or, with
+    substitute, coefficient rows over the layer's outputs taken to its inputs (also the
+    gradient with respect to the layer's input): x [T, n_out] -> x @ W + scale_e * (x @ B_e) @ A_e.
+    offsets [n_requests + 1] int64: the rows of request q are offsets[q] .. offsets[q+1]-1;
+    ids [n_requests] int32: its adapter, any value outside 0 .. n_adapters-1 none.  Both are
+    read on the device, without a synchronisation.  Rows of no request are left as they were in
+    `out`, and are 0 in a new result.  `out` must not overlap x."""
+    dev = layer.device
+    K, N = (layer.n_out, layer.n_in) if substitute else (layer.n_in, layer.n_out)
+    if x.stride(-1) != 1:
+        x = x.contiguous()
+    _expect("x", x, layer.dtype, (None, K), dev, strided=True)
+    T, Q = int(x.shape[0]), int(ids.shape[0])
+    _expect("offsets", offsets, torch.int64, (Q + 1,), dev)
+    _expect("ids", ids, torch.int32, (None,), dev)
+    if out is not None:
+        _expect("out", out, layer.dtype, (T, N), dev, strided=True)
+    with _on(dev):
+        if out is None:
+            out = torch.zeros(T, N, dtype=layer.dtype, device=dev)
+        need = _lib.lib.cf_adapter_workspace_bytes(layer._ref, int(substitute), T, Q)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        LAUNCHES[0] += 2
+        st = _lib.lib.cf_adapter_matmul(layer._ref, int(substitute), T, x.data_ptr(), _row_stride(x), Q,
+                                        offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
+                                        ws.data_ptr(), need, _stream())
+    _lib.check(st, "cf_adapter_matmul")
+    return out
+
+
+class AnswerRules:
+    """The rule by which each of `rows` rows' answer is taken from its n logits.
+
+    tokens [n_tokens] int32 with token_offsets [rows + 1] int64: the rows' histories, the first
+    prompt_len [rows] int32 (default 0) tokens of each given, the rest answered; repetition,
+    frequency, presence [rows] float32: the penalties (a repetition factor > 0);
+    bias_ids [n_biases] int32, bias_values float32, bias_offsets [rows + 1] int64: biases, of an
+    id given more than once the last; allowed [n_masks, words >= ceil(n / 32)] int32: sets of
+    allowed answers, bit j % 32 of word j / 32 for answer j; allowed_row [rows] int32: the rows'
+    sets, any value outside 0 .. n_masks-1 none (default: row r has set r).  The tensors are
+    kept and read at every call.
+
+        v = x;  j in the history: v = v / repetition if v > 0 else v * repetition
+        answered c > 0 times:     v = v - frequency * c;  v = v - presence
+        j has a bias:             v = v + bias;      j is not allowed: v = -inf
+    """
+
+    def __init__(self, rows, n, tokens=None, token_offsets=None, prompt_len=None, repetition=None, frequency=None,
+                 presence=None, bias_ids=None, bias_values=None, bias_offsets=None, allowed=None, allowed_row=None):
+        self.rows, self.n = int(rows), int(n)
+        given = dict(tokens=tokens, token_offsets=token_offsets, prompt_len=prompt_len, repetition=repetition,
+                     frequency=frequency, presence=presence, bias_ids=bias_ids, bias_values=bias_values,
+                     bias_offsets=bias_offsets, allowed=allowed, allowed_row=allowed_row)
+        first = next(((k, t) for k, t in given.items() if t is not None), None)
+        self.device = _cuda(*first) if first else None
+        i32, i64, f32 = torch.int32, torch.int64, torch.float32
+        shapes = dict(tokens=(i32, (None,)), token_offsets=(i64, (self.rows + 1,)), prompt_len=(i32, (self.rows,)),
+                      repetition=(f32, (self.rows,)), frequency=(f32, (self.rows,)), presence=(f32, (self.rows,)),
+                      bias_ids=(i32, (None,)), bias_values=(f32, (None,)), bias_offsets=(i64, (self.rows + 1,)),
+                      allowed=(i32, (None, None)), allowed_row=(i32, (self.rows,)))
+        for k, t in given.items():
+            if t is not None:
+                _expect(k, t, shapes[k][0], shapes[k][1], self.device)
+        if bias_ids is not None and bias_values is not None and bias_ids.shape != bias_values.shape:
+            raise Exception(f"SHAPE MISMATCH: {tuple(bias_ids.shape)} bias ids, {tuple(bias_values.shape)} values")
+        self._keep = given
+        # an empty list has no storage of its own: nothing is in it, offsets and all
+        if tokens is not None and tokens.numel() == 0:
+            given = {k: None if k in ("tokens", "token_offsets", "prompt_len", "repetition", "frequency", "presence")
+                     else t for k, t in given.items()}
+        if allowed is not None and allowed.shape[0] == 0:
+            given = {k: None if k.startswith("allowed") else t for k, t in given.items()}
+        if bias_ids is not None and bias_ids.numel() == 0:
+            given = {k: None if k.startswith("bias_") else t for k, t in given.items()}
+        count = {k: 0 if given[k] is None else int(given[k].shape[0]) for k in ("tokens", "bias_ids", "allowed")}
+        self.c = _lib.CfAnswerRules(self.rows, self.n, count["tokens"], count["bias_ids"],
+                                    0 if allowed is None else int(allowed.shape[1]), count["allowed"], 0,
+                                    *[_ptr(t) for t in given.values()])
+        self._ref = ctypes.byref(self.c)
+
+
+def _rules_rows(name, t, rules, dtype):
+    dev = _cuda(name, t)
+    if rules.device is not None and dev != rules.device:
+        raise Exception(f"SHAPE MISMATCH: {name} is on {dev}, the rules are on {rules.device}")
+    if t.dim() == 2 and t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    _expect(name, t, dtype, (rules.rows, rules.n), dev, strided=True)
+    return t, dev
+
+
+def edit_logits(logits, rules, out=None):
+    """The rules applied to logits [rows, n] (float32, bfloat16, float16), in float32, rounded
+    once to the logits' dtype; `out` may be the logits themselves."""
+    if logits.dtype not in _DTYPES:
+        raise NotImplementedError(f"logits of {logits.dtype} (float32, bfloat16 and float16 are supported)")
+    x, dev = _rules_rows("logits", logits, rules, logits.dtype)
+    if out is None:
+        out = torch.empty(rules.rows, rules.n, dtype=x.dtype, device=dev)
+    else:
+        _expect("out", out, x.dtype, (rules.rows, rules.n), dev, strided=True)
+    with _on(dev):
+        LAUNCHES[0] += 1
+        st = _lib.lib.cf_edit_logits(rules._ref, _DTYPES[x.dtype], x.data_ptr(), _row_stride(x), out.data_ptr(),
+                                     _row_stride(out), _stream())
+    _lib.check(st, "cf_edit_logits")
+    return out
+
+
+def answer_margin(l, u, labels, rules):
+    """How far labels [rows] (int64) are certified under the rules: l, u [rows, n] float32
+    bounds of the logits.  Returns margin [rows] float32, the label's edited lower bound less
+    the best edited upper bound among the other answers (> 0: the answer is the label), and
+    rival [rows] int32, that other answer (the lowest on equal bounds, -1: none is left).
+    A label that is not allowed has margin -inf; a bound that is NaN bounds nothing."""
+    l, dev = _rules_rows("l", l, rules, torch.float32)
+    u, _ = _rules_rows("u", u, rules, torch.float32)
+    _expect("u", u, torch.float32, (rules.rows, rules.n), dev, strided=True)
+    _expect("labels", labels, torch.int64, (rules.rows,), dev)
+    margin = torch.empty(rules.rows, dtype=torch.float32, device=dev)
+    rival = torch.empty(rules.rows, dtype=torch.int32, device=dev)
+    with _on(dev):
+        LAUNCHES[0] += 1
+        st = _lib.lib.cf_answer_margin(rules._ref, l.data_ptr(), _row_stride(l), u.data_ptr(), _row_stride(u),
+                                       labels.data_ptr(), margin.data_ptr(), rival.data_ptr(), _stream())
+    _lib.check(st, "cf_answer_margin")
+    return margin, rival

@@ -298,8 +298,9 @@ enum {
   CF_OP_AND = 10, CF_OP_OR = 11, CF_OP_MAX = 12, CF_OP_MIN = 13
 };
 enum { CF_UOP_NEG = 0, CF_UOP_NOT = 1, CF_UOP_SIGMOID = 2, CF_UOP_RELU = 3, CF_UOP_TO_F32 = 4 };
-/* dtype codes of a block: 0 float32, 1 bool (one byte, 0/1) */
-enum { CF_F32 = 0, CF_BOOL = 1 };
+/* dtype codes of a block: 0 float32, 1 bool (one byte, 0/1).  CF_BF16 and CF_F16 are data types
+ * of the per-request operators below only. */
+enum { CF_F32 = 0, CF_BOOL = 1, CF_BF16 = 2, CF_F16 = 3 };
 
 /* out = x op y.  Arithmetic in float32 (bool reads as 0/1); comparisons, and, or give
  * bool; the result is converted to out_dtype (bool: value != 0). */
@@ -389,6 +390,101 @@ cf_status cf_conv_scale(const cf_conv_geom* g, int64_t nb, const float* P, int64
 cf_status cf_conv_transpose(const cf_conv_geom* g, int64_t nb, int64_t per_b, const float* Y, int64_t x_bs,
                             int64_t x_ss, int64_t x_es, const float* W, int32_t OH, int32_t OW, float* out,
                             int64_t o_bs, int64_t o_ss, int64_t o_es, void* stream);
+
+/* ---- many variants of one network in a batch ----------------------------------------
+ * No counterpart in the reference, whose regions share one network and one decision rule.
+ * Requests (regions under certification, sequences being answered) may each carry a
+ * low-rank adapter beside a layer's shared weights, and a rule by which their answer is
+ * taken from the logits.
+ *
+ * An affine layer with adapters: W [n_out, n_in], bias [n_out] or NULL, and for adapter e
+ * A_e [rank, n_in], B_e [n_out, rank] and scale_e, standing for W + scale_e B_e A_e.  Rows of
+ * W, A_e and B_e are contiguous, at w_rs / a_rs / b_rs elements; adapter e starts at e*a_es /
+ * e*b_es.  ranks_dev (or NULL) gives each adapter's own rank <= rank: what A_e and B_e hold
+ * beyond it is not used, whatever it is.  Data is of one dtype (CF_F32, CF_BF16, CF_F16),
+ * scales are float32. */
+typedef struct cf_adapter_layer {
+  int32_t dtype;
+  int32_t n_adapters;
+  int32_t rank;
+  int32_t reserved;
+  int64_t n_out, n_in;
+  const void* W_dev;
+  int64_t w_rs;
+  const void* bias_dev;
+  const void* A_dev;
+  int64_t a_es, a_rs;
+  const void* B_dev;
+  int64_t b_es, b_rs;
+  const float* scale_dev;   /* [n_adapters] */
+  const int32_t* ranks_dev; /* [n_adapters] or NULL */
+} cf_adapter_layer;
+
+/* Rows of n_requests requests through the layer.  offsets_dev [n_requests + 1] (int64, not
+ * decreasing): request q has the rows offsets[q] .. offsets[q+1]-1; ids_dev [n_requests]
+ * (int32): its adapter, any value outside 0 .. n_adapters-1 none.
+ *   substitute == 0: y = x W^T + bias + scale_e (x A_e^T) B_e^T      x [T, n_in], y [T, n_out]
+ *   substitute != 0: y = x W + scale_e (x B_e) A_e                   x [T, n_out], y [T, n_in]
+ * (coefficient rows over the layer's outputs taken to its inputs, as cf_backsub_step's product;
+ * the bias does not take part).  Rows of x and y are contiguous, at x_rs / y_rs elements.  Rows
+ * of no request (before offsets[0], from offsets[n_requests] on) are left as they were.  x and y
+ * do not overlap.  A request's rows depend on its own adapter only: infinities or NaN in another
+ * adapter or in rows of other requests do not reach them.  Products are accumulated in float32;
+ * float32 data is multiplied as 3xTF32, as in the chained substitution. */
+size_t cf_adapter_workspace_bytes(const cf_adapter_layer* layer, int32_t substitute, int64_t T,
+                                  int64_t n_requests);
+cf_status cf_adapter_matmul(const cf_adapter_layer* layer, int32_t substitute, int64_t T, const void* x_dev,
+                            int64_t x_rs, int64_t n_requests, const int64_t* offsets_dev, const int32_t* ids_dev,
+                            void* y_dev, int64_t y_rs, void* workspace_dev, size_t workspace_bytes, void* stream);
+
+/* The rule by which each of `rows` rows' answer is taken from its n logits:
+ *   tokens_dev [n_tokens] int32, row r's history at token_offsets[r] .. token_offsets[r+1]-1;
+ *     its first prompt_len[r] tokens (NULL: 0) were given, the rest answered
+ *   repetition / frequency / presence [rows] float32 (NULL: 1 / 0 / 0)
+ *   bias_ids / bias_values [n_biases], row r's at bias_offsets[r] .. bias_offsets[r+1]-1; of an
+ *     id given more than once the last entry counts
+ *   allowed_dev [n_masks, allowed_words] int32: bit j % 32 of word j / 32 set: j is allowed;
+ *     row r has mask allowed_row[r] (NULL: r), any value outside 0 .. n_masks-1 none
+ * applied to a logit x of answer j, in float32, each step rounded:
+ *   v = x; j in the history: v = v > 0 ? v / repetition : v * repetition; answered c > 0 times:
+ *   v = v - frequency * c, v = v - presence; j has a bias: v = v + bias; not allowed: -inf.
+ * Tokens and ids outside 0 .. n-1 are ignored, and offsets are held within their lists.  With
+ * repetition > 0 every step is monotone: the edited bounds of a logit bound the edited logit. */
+typedef struct cf_answer_rules {
+  int64_t rows, n;
+  int64_t n_tokens, n_biases;
+  int64_t allowed_words;
+  int32_t n_masks;
+  int32_t reserved;
+  const int32_t* tokens_dev;
+  const int64_t* token_offsets_dev;
+  const int32_t* prompt_len_dev;
+  const float* repetition_dev;
+  const float* frequency_dev;
+  const float* presence_dev;
+  const int32_t* bias_ids_dev;
+  const float* bias_values_dev;
+  const int64_t* bias_offsets_dev;
+  const int32_t* allowed_dev;
+  const int32_t* allowed_row_dev;
+} cf_answer_rules;
+
+/* out = the rules applied to logits [rows, n] (rows at in_rs elements, 0 = one row for all) of
+ * dtype CF_F32, CF_BF16 or CF_F16; out of the same dtype, rows at out_rs, may be the input
+ * itself. */
+cf_status cf_edit_logits(const cf_answer_rules* rules, int32_t dtype, const void* logits_dev, int64_t in_rs,
+                         void* out_dev, int64_t out_rs, void* stream);
+
+/* The certified margin of label[r] (int64) under the rules, from lower bounds l and upper bounds
+ * u [rows, n] of the logits (rows at l_rs / u_rs floats, 0 = one row for all):
+ *   margin[r] = edit(l)[label] - max over j != label of edit(u)[j],  rival[r] = that j
+ * (the lowest on equal values): margin > 0 proves that the answer is label.  A label that is not
+ * allowed or no answer, and a difference that has no value, give -inf; no other answer left:
+ * rival -1 (margin +inf for a label above -inf).  A bound that is NaN bounds nothing: l counts as
+ * -inf, u as +inf. */
+cf_status cf_answer_margin(const cf_answer_rules* rules, const float* l_dev, int64_t l_rs, const float* u_dev,
+                           int64_t u_rs, const int64_t* labels_dev, float* margin_dev, int32_t* rival_dev,
+                           void* stream);
 
 /* Message for the last non-OK status on this host thread ("" if none). */
 const char* cf_last_error(void);

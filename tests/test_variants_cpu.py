@@ -1,0 +1,147 @@
+"""Per-request adapters and answer rules without a GPU: refusals before any launch, and the
+64-bit forms that the GPU tests compare with, against independent statements of them."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import variants_oracle as V
+from cfgpu import _lib, ops
+
+
+def c_layer(**kw):
+    d = dict(dtype=_lib.CF_BF16, n_adapters=2, rank=4, reserved=0, n_out=32, n_in=16, W_dev=256, w_rs=16, bias_dev=None,
+             A_dev=256, a_es=64, a_rs=16, B_dev=256, b_es=128, b_rs=4, scale_dev=256, ranks_dev=None)
+    d.update(kw)
+    return _lib.CfAdapterLayer(**d)
+
+
+def call(L, substitute=0, T=8, x=256, x_rs=16, q=2, off=256, ids=256, y=4096, y_rs=32, ws=1 << 16, wsb=None):
+    if wsb is None:
+        wsb = _lib.lib.cf_adapter_workspace_bytes(ctypes.byref(L), substitute, T, q)
+    return _lib.lib.cf_adapter_matmul(ctypes.byref(L), substitute, T, x, x_rs, q, off, ids, y, y_rs, ws, wsb, None)
+
+
+@pytest.mark.parametrize("layer,args,status", [
+    (dict(dtype=_lib.CF_BOOL), {}, "UNSUPPORTED"), (dict(dtype=9), {}, "UNSUPPORTED"),
+    (dict(n_out=-1), {}, "SHAPE"), (dict(rank=-1), {}, "SHAPE"), (dict(w_rs=15), {}, "SHAPE"),
+    (dict(a_rs=15), {}, "SHAPE"), (dict(b_rs=3), {}, "SHAPE"), (dict(W_dev=257), {}, "SHAPE"),
+    (dict(W_dev=None), {}, "NULL"), (dict(A_dev=None), {}, "NULL"), (dict(B_dev=None), {}, "NULL"),
+    (dict(scale_dev=None), {}, "NULL"),
+    ({}, dict(T=-1), "SHAPE"), ({}, dict(q=-1), "SHAPE"), ({}, dict(y_rs=31), "SHAPE"), ({}, dict(x_rs=-1), "SHAPE"),
+    ({}, dict(x=None), "NULL"), ({}, dict(y=None), "NULL"), ({}, dict(off=None), "NULL"), ({}, dict(ids=None), "NULL"),
+    ({}, dict(wsb=0), "WORKSPACE"), ({}, dict(ws=None), "WORKSPACE"), ({}, dict(ws=(1 << 16) + 8), "WORKSPACE"),
+])
+def test_adapter_refusals(layer, args, status):
+    st = call(c_layer(**layer), **args)
+    assert st == getattr(_lib, f"CF_ERR_{status}"), _lib.lib.cf_last_error()
+    assert _lib.lib.cf_last_error()
+
+
+def test_nothing_to_do_is_no_error():
+    assert call(c_layer(), T=0) == _lib.CF_OK
+    assert call(c_layer(), q=0) == _lib.CF_OK
+    assert call(c_layer(n_out=0)) == _lib.CF_OK
+
+
+def test_adapter_fault_injection(monkeypatch):
+    monkeypatch.setenv("CF_FAULT", "adapter_matmul")
+    assert call(c_layer()) == _lib.CF_ERR_INJECTED
+
+
+def c_rules(**kw):
+    d = dict(rows=2, n=10)
+    d.update(kw)
+    return _lib.CfAnswerRules(**d)
+
+
+@pytest.mark.parametrize("rules,status", [
+    (dict(rows=-1), "SHAPE"), (dict(n=1 << 31), "SHAPE"), (dict(n_tokens=1 << 31), "SHAPE"),
+    (dict(tokens_dev=256), "NULL"), (dict(token_offsets_dev=256), "NULL"), (dict(repetition_dev=256), "NULL"),
+    (dict(bias_ids_dev=256, bias_offsets_dev=256), "NULL"), (dict(allowed_row_dev=256), "NULL"),
+    (dict(allowed_dev=256, n_masks=1, allowed_words=1), "SHAPE"),
+    (dict(allowed_dev=256, n_masks=2, allowed_words=0), "SHAPE"),
+])
+def test_rules_refusals(rules, status):
+    R = c_rules(**rules)
+    want = getattr(_lib, f"CF_ERR_{status}")
+    assert _lib.lib.cf_edit_logits(ctypes.byref(R), _lib.CF_F32, 256, 10, 4096, 10, None) == want
+    assert _lib.lib.cf_answer_margin(ctypes.byref(R), 256, 10, 256, 10, 256, 256, 256, None) == want
+
+
+def test_edit_and_margin_refusals():
+    R = c_rules()
+    ref = ctypes.byref(R)
+    e, m = _lib.lib.cf_edit_logits, _lib.lib.cf_answer_margin
+    assert e(None, _lib.CF_F32, 256, 10, 4096, 10, None) == _lib.CF_ERR_NULL
+    assert e(ref, _lib.CF_BOOL, 256, 10, 4096, 10, None) == _lib.CF_ERR_UNSUPPORTED
+    assert e(ref, _lib.CF_F32, None, 10, 4096, 10, None) == _lib.CF_ERR_NULL
+    assert e(ref, _lib.CF_F32, 256, 10, 4096, 9, None) == _lib.CF_ERR_SHAPE
+    assert e(ref, _lib.CF_F32, 258, 10, 4096, 10, None) == _lib.CF_ERR_SHAPE
+    assert m(ref, 256, 10, 256, 10, None, 256, 256, None) == _lib.CF_ERR_NULL
+    assert m(ref, 256, -1, 256, 10, 256, 256, 256, None) == _lib.CF_ERR_SHAPE
+    assert m(ctypes.byref(c_rules(n=0)), 256, 0, 256, 0, 256, 256, 256, None) == _lib.CF_ERR_SHAPE
+    assert e(ctypes.byref(c_rules(n=0)), _lib.CF_F32, None, 0, None, 0, None) == _lib.CF_OK
+
+
+def test_cpu_tensors_are_refused():
+    W, A, B = torch.zeros(4, 4), torch.zeros(1, 2, 4), torch.zeros(1, 4, 2)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.AdapterLayer(W, A, B, torch.ones(1))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.AnswerRules(1, 4, allowed=torch.zeros(1, 1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.edit_logits(torch.zeros(1, 4), ops.AnswerRules(1, 4))
+    with pytest.raises(NotImplementedError):
+        ops.edit_logits(torch.zeros(1, 4, dtype=torch.float64), ops.AnswerRules(1, 4))
+
+
+# ------------------------------------------------------------------------- the 64-bit forms
+def test_oracle_adapter_is_the_merged_weight():
+    g = torch.Generator()
+    g.manual_seed(0)
+    W, A, B = (torch.randn(*s, generator=g) for s in ((6, 5), (2, 3, 5), (2, 6, 3)))
+    scale = torch.tensor([0.5, 2.0])
+    for sub in (False, True):
+        x = torch.randn(4, 6 if sub else 5, generator=g)
+        y, tol = V.adapter(x, W, A, B, scale, [0, 1, 3, 4], [1, -1, 0], substitute=sub)
+        for row, e in ((0, 1), (1, None), (2, None), (3, 0)):
+            M = W.double() if e is None else W.double() + scale[e].double() * B[e].double() @ A[e].double()
+            want = x[row].double() @ (M if sub else M.t())
+            assert torch.allclose(y[row], want, rtol=1e-12, atol=1e-12)
+        assert (tol > 0).all()
+        with pytest.raises(AssertionError):
+            V.check((y * 1.001).to(torch.float32), y, tol)
+
+
+def test_oracle_substitute_is_the_input_gradient():
+    """x W + s (x B) A is the gradient of <x, layer(z)> with respect to z: by differences, which
+    are exact up to rounding for a linear layer."""
+    g = torch.Generator()
+    g.manual_seed(1)
+    W, A, B = (torch.randn(*s, generator=g) for s in ((6, 5), (1, 3, 5), (1, 6, 3)))
+    x, z = torch.randn(1, 6, generator=g), torch.randn(1, 5, generator=g)
+    scale = torch.tensor([0.7])
+    grad, _ = V.adapter(x, W, A, B, scale, [0, 1], [0], substitute=True)
+
+    def value(z):
+        return (x.double() * V.adapter(z, W, A, B, scale, [0, 1], [0])[0]).sum()
+    for k in range(5):
+        d = torch.zeros(1, 5, dtype=torch.float64)
+        d[0, k] = 0.25
+        diff = (value(z.double() + d) - value(z.double() - d)) / 0.5
+        assert abs(float(diff - grad[0, k])) < 1e-12
+
+
+def test_oracle_rules_by_hand():
+    n = 4
+    x = torch.tensor([[2.0, -2.0, 1.0, 5.0]])
+    kw = dict(tokens=torch.tensor([0, 1, 1, 2], dtype=torch.int32), token_offsets=torch.tensor([0, 4]),
+              prompt_len=torch.tensor([1], dtype=torch.int32), repetition=torch.tensor([2.0]),
+              frequency=torch.tensor([0.5]), presence=torch.tensor([0.25]),
+              bias_ids=torch.tensor([3, 3], dtype=torch.int32), bias_values=torch.tensor([9.0, 1.0]),
+              bias_offsets=torch.tensor([0, 2]), allowed=V.pack(torch.tensor([[True, True, False, True]])))
+    assert V.rules(x, n, **kw).tolist() == [[1.0, -4.0 - 1.0 - 0.25, -math.inf, 6.0]]
+    m, j = V.margin(x, x, torch.tensor([3]), n, **kw)
+    assert m.tolist() == [5.0] and j.tolist() == [0]
