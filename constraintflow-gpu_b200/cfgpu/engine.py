@@ -38,10 +38,14 @@ class DeepPolyEngine:
     None: every traversal reaches the input).  relu_strict: the lower ReLU slope is 1 where
     l + u > 0 (the relu_n of those programs and of zid.cf) instead of l + u >= 0; deeppoly
     and crownibp.
+    adapters: {index of a linear layer: (A [E, rank, n_in], B [E, n_out, rank], scale [E][,
+    ranks [E]])}: variants of the network that share its weights, W + scale[e] * B[e] @ A[e] in
+    those layers (the same E everywhere).  run(..., adapter_ids=[B] int32) certifies every
+    region for its own variant, in one batch; DeepPoly, through the general traversal.
     """
 
     def __init__(self, layers, input_size, device="cuda", n_spec=N_CLASSES - 1, certifier="deeppoly",
-                 stop_depth=None, relu_strict=False):
+                 stop_depth=None, relu_strict=False, adapters=None):
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise ValueError("DeepPolyEngine runs on a CUDA device only (no CPU fallback)")
@@ -130,10 +134,28 @@ class DeepPolyEngine:
                                           "layers")
             self.net = None
             self.N = self.input_size + sum(widths) + self.n_spec
+        self._adapters = self._adapter_layers(adapters, certifier, stop_depth, relu_strict) if adapters else {}
         self._ws = None
         self.graphs = True           # CUDA-graph replay of the general traversal (DeepPoly)
         self._graph_cache = {}
         self.replayed_launches = 0   # libcfgpu kernels replayed by those graphs
+
+    def _adapter_layers(self, adapters, certifier, stop_depth, relu_strict):
+        from . import ops
+        if certifier != "deeppoly" or stop_depth is not None or relu_strict:
+            raise NotImplementedError("adapters apply to the plain DeepPoly traversal")
+        made = {}
+        for idx, given in adapters.items():
+            if not 0 <= idx < len(self._general) or self._general[idx][0] != "linear":
+                raise NotImplementedError(f"adapters of layer {idx}: only linear layers carry them")
+            A, B, scale, ranks = tuple(given) + (None,) * (4 - len(given))
+            A, B, scale = (torch.as_tensor(t, dtype=torch.float32).to(self.device).contiguous() for t in (A, B, scale))
+            if ranks is not None:
+                ranks = torch.as_tensor(ranks, dtype=torch.int32).to(self.device).contiguous()
+            made[idx] = ops.AdapterLayer(self._general[idx][1], A, B, scale, ranks)
+        if len({layer.n_adapters for layer in made.values()}) > 1:
+            raise ValueError("every adapted layer needs the same number of adapters")
+        return made
 
     def workspace_bytes(self, chunk):
         if self.net is None:
@@ -153,7 +175,7 @@ class DeepPolyEngine:
     workspace_budget = 8 << 30
 
     def run(self, l0, u0, spec_W, want_state=False, workspace_budget=None, out=None, check_device=False,
-            replay=None):
+            replay=None, adapter_ids=None):
         """Bounds for B regions.
 
         l0, u0: [B, n_input] float32 device tensors (normalised input box);
@@ -179,8 +201,16 @@ class DeepPolyEngine:
         if want_state:
             sl = torch.empty(B, self.N, dtype=torch.float32, device=self.device)
             su = torch.empty_like(sl)
-        if self.net is None:
-            lb, ub, sl_g, su_g = self._general_run(l0, u0, spec_W, lb, ub)
+        if adapter_ids is not None:
+            if not self._adapters:
+                raise ValueError("adapter_ids on an engine without adapters")
+            if replay is not None:
+                raise NotImplementedError("decision replay of adapted networks")
+            if tuple(adapter_ids.shape) != (B,) or adapter_ids.dtype != torch.int32 or \
+                    adapter_ids.device != self.device or not adapter_ids.is_contiguous():
+                raise Exception(f"SHAPE MISMATCH: adapter_ids must be contiguous int32 {(B,)} on {self.device}")
+        if self.net is None or adapter_ids is not None:
+            lb, ub, sl_g, su_g = self._general_run(l0, u0, spec_W, lb, ub, adapter_ids)
             if want_state:
                 sl.copy_(sl_g)
                 su.copy_(su_g)
@@ -222,7 +252,7 @@ class DeepPolyEngine:
             return lb, ub, sl, su
         return lb, ub
 
-    def _general_run(self, l0, u0, spec_W, lb, ub):
+    def _general_run(self, l0, u0, spec_W, lb, ub, adapter_ids=None):
         """Bounds through the general lowest-layer-first traversal (cfgpu.general).
 
         DeepPoly's traversal takes no data-dependent decision on the host, so for a given
@@ -231,45 +261,51 @@ class DeepPolyEngine:
         runs eagerly."""
         from . import general
         if self.certifier == "deeppoly" and self.graphs:
-            g = self._graph_cache.get(int(l0.shape[0]))
+            key = (int(l0.shape[0]), adapter_ids is not None)
+            g = self._graph_cache.get(key)
             if g is None:
-                g = self._capture(l0, u0, spec_W)
+                g = self._capture(l0, u0, spec_W, adapter_ids, key)
             if g is not None:
                 g["l0"].copy_(l0)
                 g["u0"].copy_(u0)
                 g["W"].copy_(spec_W)
+                if adapter_ids is not None:
+                    g["ids"].copy_(adapter_ids)
                 g["graph"].replay()
                 self.replayed_launches += g["launches"]
                 lb.copy_(g["sl"][:, -self.n_spec:])
                 ub.copy_(g["su"][:, -self.n_spec:])
                 return lb, ub, g["sl"], g["su"]
-        bounds, _ = general.run(self._general, l0, u0, spec_W, self.certifier)
+        adapters = self._adapters if adapter_ids is not None else None
+        bounds, _ = general.run(self._general, l0, u0, spec_W, self.certifier, adapters, adapter_ids)
         sl, su = general.state(l0, u0, bounds)
         lb.copy_(bounds[-1][0])
         ub.copy_(bounds[-1][1])
         return lb, ub, sl, su
 
-    def _capture(self, l0, u0, spec_W):
+    def _capture(self, l0, u0, spec_W, adapter_ids, key):
         from . import general
-        static = {"l0": l0.clone(), "u0": u0.clone(), "W": spec_W.clone()}
+        static = {"l0": l0.clone(), "u0": u0.clone(), "W": spec_W.clone(),
+                  "ids": None if adapter_ids is None else adapter_ids.clone()}
+        variant = (self._adapters if adapter_ids is not None else None, static["ids"])
         try:
             side = torch.cuda.Stream(self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
             with torch.cuda.stream(side):      # warm-up outside the capture
-                general.run(self._general, static["l0"], static["u0"], static["W"], "deeppoly")
+                general.run(self._general, static["l0"], static["u0"], static["W"], "deeppoly", *variant)
             torch.cuda.current_stream(self.device).wait_stream(side)
             graph = torch.cuda.CUDAGraph()
             from . import ops
             n0 = ops.LAUNCHES[0]
             with torch.cuda.graph(graph):
-                bounds, _ = general.run(self._general, static["l0"], static["u0"], static["W"], "deeppoly")
+                bounds, _ = general.run(self._general, static["l0"], static["u0"], static["W"], "deeppoly", *variant)
                 static["sl"], static["su"] = general.state(static["l0"], static["u0"], bounds)
         except RuntimeError:
             self.graphs = False                  # capture refused: run eagerly from now on
             return None
         static["graph"] = graph
         static["launches"] = ops.LAUNCHES[0] - n0
-        self._graph_cache[int(l0.shape[0])] = static
+        self._graph_cache[key] = static
         return static
 
     def input_spec(self, X, y, eps, dataset):
@@ -298,6 +334,36 @@ class DeepPolyEngine:
         l0, u0, W = self.input_spec(X, y, eps, dataset)
         lb, ub = self.run(l0, u0, W, out=out)
         return lb, ub
+
+    def answer(self, l0, u0, labels, rules, adapter_ids=None):
+        """Whether each region's answer under `rules` (ops.AnswerRules over the network's last
+        layer) is its label: (margin [B] float32, rival [B] int32), margin > 0 certifies it
+        (ops.answer_margin).  Without a repetition factor the rules add a constant to each
+        logit, and the margin is taken from the property rows' bounds of y[label] - y[j]; with
+        one, from the bounds of the logits themselves.  labels [B] int64 device tensor of
+        answers in 0 .. n_last-1."""
+        from . import ops
+        B, n = int(l0.shape[0]), self.n_last
+        if (rules.rows, rules.n) != (B, n) or self.n_spec != n - 1:
+            raise Exception(f"SHAPE MISMATCH: rules for {rules.rows} rows of {rules.n} answers and {self.n_spec} "
+                            f"property rows; {B} regions of {n} answers")
+        if tuple(labels.shape) != (B,) or labels.dtype != torch.int64 or labels.device != self.device or \
+                not labels.is_contiguous():
+            raise Exception(f"SHAPE MISMATCH: labels must be contiguous int64 {(B,)} on {self.device}")
+        W = torch.empty(B, n - 1, n, dtype=torch.float32, device=self.device)
+        stream = torch.cuda.current_stream(self.device).cuda_stream
+        check(lib.cf_spec_matrix(B, n, labels.data_ptr(), W.data_ptr(), stream), "cf_spec_matrix")
+        if rules.c.repetition_dev:
+            _, _, sl, su = self.run(l0, u0, W, want_state=True, adapter_ids=adapter_ids)
+            at = self.N - self.n_spec - n
+            return ops.answer_margin(sl[:, at:at + n], su[:, at:at + n], labels, rules)
+        lb, _ = self.run(l0, u0, W, adapter_ids=adapter_ids)
+        # y[j] - y[label] <= -lb: upper bounds of the other answers relative to the label's 0
+        row = torch.arange(n - 1, device=self.device)
+        col = row + (row >= labels[:, None])
+        lo = torch.zeros(B, n, dtype=torch.float32, device=self.device)
+        up = torch.zeros_like(lo).scatter_(1, col, ops.unary("neg", lb.float(), torch.float32))
+        return ops.answer_margin(lo, up, labels, rules)
 
 
 def profile_enable(on=True):

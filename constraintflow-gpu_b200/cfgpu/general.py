@@ -27,10 +27,12 @@ substitution is a column scaling instead of a product with an n x n matrix, or a
 layer's weights (_Conv, the KernelBlock of constraintflow/gbcsr/sparse_block.py:1158),
 substituted by the transposed convolution of every coefficient row (cf_conv_transpose,
 as DenseBlock @ KernelBlock, :839-911) and densified (cf_conv_densify) only where it
-starts a traversal or meets another block over the same layer.  Every
-arithmetic operation is a libcfgpu kernel (cfgpu.ops: cf_bmm, cf_signscale, cf_ew_binary,
-cf_ew_clamp, cf_ew_any; cf_relu_relax for DeepPoly's relaxation); torch provides memory,
-views and copies.
+starts a traversal or meets another block over the same layer; or a linear layer whose regions
+carry low-rank adapters (_Adapted), substituted by the shared weights and each region's own
+adapter in one product (cf_adapter_matmul).  Every
+arithmetic operation is a libcfgpu kernel (cfgpu.ops: cf_bmm, cf_adapter_matmul, cf_signscale,
+cf_ew_binary, cf_ew_clamp, cf_ew_any; cf_relu_relax for DeepPoly's relaxation); torch provides
+memory, views and copies.
 """
 import operator
 
@@ -62,9 +64,34 @@ class _Conv:
         return ops.conv_densify(self.g, 1, self.W, 0, self.ckk, 0)
 
 
+class _Adapted:
+    """A linear layer's weights W + scale_e B_e A_e, e the adapter of the region: the shared
+    matrix and the adapters (ops.AdapterLayer) with the regions' adapter ids [B] int32."""
+
+    def __init__(self, layer, ids):
+        self.layer, self.ids = layer, ids
+        self.shape = (int(ids.shape[0]), layer.n_out, layer.n_in)
+
+    def dim(self):
+        return 3
+
+    def apply(self, A):
+        """A [B, r, n_out] through the layer: [B, r, n_in]."""
+        B, r, n_out = A.shape
+        offsets = torch.arange(0, B * r + 1, r, dtype=torch.int64, device=A.device)
+        out = torch.empty(B * r, self.layer.n_in, dtype=F32, device=A.device)
+        ops.adapter_matmul(A.reshape(B * r, n_out), self.layer, offsets, self.ids, substitute=True, out=out)
+        return out.view(B, r, self.layer.n_in)
+
+    def dense(self):
+        n = self.layer.n_out
+        eye = torch.eye(n, dtype=F32, device=self.ids.device)
+        return self.apply(eye.expand(self.shape[0], n, n))
+
+
 def _full(B, t):
     """[1 or B, r, n] -> a [B, r, n] view (batch stride 0 when shared)."""
-    if isinstance(t, _Conv):
+    if isinstance(t, (_Conv, _Adapted)):
         t = t.dense()
     return t.expand(B, t.shape[1], t.shape[2]) if t.shape[0] == 1 else t
 
@@ -93,7 +120,10 @@ def _add_block(B, blocks, t, M):
 
 def _apply(B, A, M):
     """A [B, r, n_t] times block M over layer s: bmm for dense, column scaling for diagonal,
-    the transposed convolution of every row for conv weights."""
+    the transposed convolution of every row for conv weights, the shared weights and the
+    region's adapter for an adapted layer."""
+    if isinstance(M, _Adapted):
+        return M.apply(A)
     if isinstance(M, _Conv):
         r, cols = A.shape[1], M.shape[2]
         out = torch.empty(B, r, cols, dtype=F32, device=A.device)
@@ -245,7 +275,7 @@ def _stack_poly(B, P, Q):
     return blocks, torch.cat([P[1], Q[1]], dim=1)
 
 
-def run(layers, l0, u0, spec_W, relaxation="deeppoly"):
+def run(layers, l0, u0, spec_W, relaxation="deeppoly", adapters=None, adapter_ids=None):
     """DeepPoly or CROWN bounds of a network of linear / conv / relu / add / concat layers.
 
     layers: list of (kind, W [n_out, n_in] (conv: [cout, cin, kh, kw]) device float32 or
@@ -253,7 +283,8 @@ def run(layers, l0, u0, spec_W, relaxation="deeppoly"):
     network input[, conv geometry (cin, ih, iw, cout, oh, ow, stride, pad)]), in the order of the
     reference's ONNX reader (breadth first from the input; every parent listed before
     its children).  l0, u0 [B, n0], spec_W [B, n_spec, n_last] device float32; the
-    property layer reads the last layer of the list.
+    property layer reads the last layer of the list.  adapters: {index of a linear layer:
+    ops.AdapterLayer over its W}, adapter_ids [B] int32 the regions' adapters.
     Returns (bounds, branches): bounds per layer (excluding input, including the property
     layer) of (l [B, n], u [B, n]) device float32; branches: BRANCH_* per ReLU layer (CROWN).
     """
@@ -299,7 +330,7 @@ def run(layers, l0, u0, spec_W, relaxation="deeppoly"):
             A0 = W
             c0 = torch.zeros(B, W.shape[1], dtype=F32, device=l0.device)
         elif kind == "linear":
-            A0 = W.unsqueeze(0)
+            A0 = W.unsqueeze(0) if idx not in (adapters or {}) else _Adapted(adapters[idx], adapter_ids)
             c0 = bias.unsqueeze(0).expand(B, -1).contiguous()
         elif kind == "conv":
             A0 = _Conv(W, layer[4])

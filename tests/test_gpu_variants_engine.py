@@ -1,0 +1,209 @@
+"""Certifying adapted variants of one network in one batch, and answers under rules."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import variants_oracle as V
+
+pytestmark = pytest.mark.gpu
+E, RANK = 3, 4
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+def make(wid=0, B=6, seed=0, adapted=(0, 2, 4)):
+    """The 784-50x3-10 network (or the residual one) with adapters in some linear layers."""
+    from cfgpu import nets
+    wl = nets.workload(wid)
+    X = nets.centres(wl, B)
+    y = nets.labels(wl, X)
+    l0, u0 = nets.input_box(X, wl.eps, wl.dataset)
+    g = torch.Generator()
+    g.manual_seed(seed)
+    linear = [i for i, L in enumerate(wl.layers) if L.kind == "linear"]
+    adapters = {}
+    for i in linear:
+        if adapted is None or i in adapted:
+            n_out, n_in = wl.layers[i].W.shape
+            adapters[i] = (torch.randn(E, RANK, n_in, generator=g) * n_in**-0.5,
+                           torch.randn(E, n_out, RANK, generator=g) * 0.3, torch.rand(E, generator=g) + 0.5)
+    ids = (torch.arange(B) % (E + 1) - 1).to(torch.int32)
+    return wl, y, l0, u0, adapters, ids
+
+
+def merged(wl, adapters, e):
+    """The layers of variant e, its adapters added to the weights (in float64, rounded once)."""
+    import copy
+    layers = []
+    for i, L in enumerate(wl.layers):
+        L = copy.copy(L)
+        if e >= 0 and i in adapters:
+            A, B, s = adapters[i]
+            L.W = (torch.as_tensor(L.W).double() + float(s[e]) * B[e].double() @ A[e].double()).float().numpy()
+        layers.append(L)
+    return layers
+
+
+def points(layers, z):
+    """The network's values at points z [n, n0], float64, layer by layer."""
+    vals = []
+    for i, L in enumerate(layers):
+        parents = getattr(L, "parents", None) or (i - 1,)
+        ins = [z if p < 0 else vals[p] for p in parents]
+        if L.kind == "linear":
+            vals.append(ins[0] @ torch.as_tensor(L.W).double().t() + torch.as_tensor(L.b).double())
+        elif L.kind == "relu":
+            vals.append(ins[0].clamp(min=0))
+        elif L.kind == "add":
+            vals.append(ins[0] + ins[1])
+        else:
+            vals.append(torch.cat(ins, dim=1))
+    return vals
+
+
+def engine(wl, adapters, layers=None):
+    from cfgpu.engine import DeepPolyEngine
+    return DeepPolyEngine(layers or wl.layers, wl.input_size, dev(), adapters=adapters)
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_each_region_is_bounded_for_its_variant(graphs):
+    """The bounds equal those of a network with the adapter merged into its weights, which
+    replays the same ReLU decisions: 8e-5 of the layer's largest bound (the measured float32
+    disagreement of two implementations with equal decisions) plus 1e-5 of the value."""
+    from cfgpu import nets
+    wl, y, l0, u0, adapters, ids = make()
+    B = l0.shape[0]
+    spec = nets.spec_weight(y).to(dev())
+    eng = engine(wl, adapters)
+    eng.graphs = graphs
+    for turn in range(2):                     # a second batch through the same captured pass
+        lb, ub, sl, su = eng.run(l0.to(dev()), u0.to(dev()), spec, want_state=True, adapter_ids=ids.to(dev()))
+        sl, su = sl.clone(), su.clone()
+        for e in range(-1, E):
+            m = engine(wl, None, merged(wl, adapters, e))
+            _, _, ml, mu = m.run(l0.to(dev()), u0.to(dev()), spec, want_state=True, replay=(sl, su))
+            rows = [b for b in range(B) if int(ids[b]) == e]
+            at = wl.input_size
+            for L in list(wl.layers) + [None]:
+                n = 9 if L is None else L.n_out
+                for got, want in ((sl, ml), (su, mu)):
+                    g, w = got[rows, at:at + n].double(), want[rows, at:at + n].double()
+                    S = torch.maximum(ml[rows, at:at + n].abs(), mu[rows, at:at + n].abs()).double().amax()
+                    assert ((g - w).abs() <= 1e-5 * w.abs() + 8e-5 * S).all(), (e, at, float((g - w).abs().max() / S))
+                at += n
+        assert torch.equal(lb.float(), sl[:, -9:]) and torch.equal(ub.float(), su[:, -9:])
+        ids = ids.roll(1)
+
+
+@pytest.mark.parametrize("wid", [0, 5, 6])
+def test_bounds_hold_at_points(wid):
+    """Chain, residual and concat networks: the variant's own values lie within its bounds."""
+    from cfgpu import nets
+    wl, y, l0, u0, adapters, ids = make(wid, adapted=None)
+    spec = nets.spec_weight(y)
+    _, _, sl, su = engine(wl, adapters).run(l0.to(dev()), u0.to(dev()), spec.to(dev()), want_state=True,
+                                            adapter_ids=ids.to(dev()))
+    sl, su = sl.cpu().double(), su.cpu().double()
+    g = torch.Generator()
+    g.manual_seed(1)
+    for b in range(l0.shape[0]):
+        layers = merged(wl, adapters, int(ids[b]))
+        z = l0[b].double() + (u0[b] - l0[b]).double() * torch.rand(40, l0.shape[1], generator=g).round().double()
+        vals = points(layers, z)
+        v = torch.cat(vals + [vals[-1] @ spec[b].double().t()], dim=1)
+        lo, up = sl[b, wl.input_size:], su[b, wl.input_size:]
+        slack = 1e-4 * torch.maximum(lo.abs(), up.abs()).max()
+        assert (v >= lo - slack).all() and (v <= up + slack).all()
+
+
+def test_without_ids_the_network_itself_runs():
+    from cfgpu import nets
+    wl, y, l0, u0, adapters, ids = make()
+    spec = nets.spec_weight(y).to(dev())
+    a = engine(wl, adapters).run(l0.to(dev()), u0.to(dev()), spec)
+    b = engine(wl, None).run(l0.to(dev()), u0.to(dev()), spec)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def rules_for(B, n, seed, repetition):
+    import test_gpu_variants as T
+    from cfgpu import ops
+    kw = T.make_rules(B, n, seed=seed, hist=4, biases=3, masks=2)
+    if not repetition:
+        kw.pop("repetition")
+    return kw, ops.AnswerRules(B, n, **T.on_gpu(kw))
+
+
+@pytest.mark.parametrize("repetition", [False, True])
+@pytest.mark.parametrize("adapted", [False, True])
+def test_answer_under_rules(repetition, adapted):
+    """At points of a region the edited logits leave the label ahead of every other answer by
+    the margin at least (up to the float32 error of the bounds)."""
+    wl, y, l0, u0, adapters, ids = make()
+    B, n = l0.shape[0], 10
+    eng = engine(wl, adapters)
+    kw, rules = rules_for(B, n, 3, repetition)
+    where = ids.to(dev()) if adapted else None
+    margin, rival = eng.answer(l0.to(dev()), u0.to(dev()), y.to(dev()), rules, adapter_ids=where)
+    margin, rival = margin.cpu().double(), rival.cpu()
+    g = torch.Generator()
+    g.manual_seed(2)
+    for b in range(B):
+        layers = merged(wl, adapters, int(ids[b]) if adapted else -1)
+        z = l0[b].double() + (u0[b] - l0[b]).double() * torch.rand(60, l0.shape[1], generator=g).round().double()
+        logits = points(layers, z)[-1]
+        one = {k: (v[b:b + 1] if k in ("prompt_len", "repetition", "frequency", "presence", "allowed_row") else
+                   v[b:b + 2] if k.endswith("offsets") else v) for k, v in kw.items()}
+        v = torch.cat([V.rules(p[None], n, **one) for p in logits])
+        mine = v[:, int(y[b])]
+        others = v.clone()
+        others[:, int(y[b])] = -math.inf
+        gap = (mine - others.max(dim=1).values)
+        gap[gap.isnan()] = -math.inf
+        assert (gap >= margin[b] - 1e-4 * logits.abs().max()).all(), b
+        if margin[b] > -math.inf and int(rival[b]) >= 0:
+            assert others[0, int(rival[b])] > -math.inf
+
+
+def test_answer_without_edits_is_the_property():
+    """No rules at all: the margin is the least of the property's lower bounds."""
+    from cfgpu import nets, ops
+    wl, y, l0, u0, adapters, ids = make()
+    eng = engine(wl, adapters)
+    lb, _ = eng.run(l0.to(dev()), u0.to(dev()), nets.spec_weight(y).to(dev()), adapter_ids=ids.to(dev()))
+    margin, _ = eng.answer(l0.to(dev()), u0.to(dev()), y.to(dev()), ops.AnswerRules(l0.shape[0], 10),
+                           adapter_ids=ids.to(dev()))
+    assert torch.equal(margin.double(), lb.min(dim=1).values)
+
+
+def test_refusals():
+    from cfgpu import nets, ops
+    from cfgpu.engine import DeepPolyEngine
+    wl, y, l0, u0, adapters, ids = make()
+    spec = nets.spec_weight(y).to(dev())
+    for kw in (dict(certifier="ibp"), dict(stop_depth=1), dict(relu_strict=True)):
+        with pytest.raises(NotImplementedError):
+            DeepPolyEngine(wl.layers, wl.input_size, dev(), adapters=adapters, **kw)
+    with pytest.raises(NotImplementedError, match="only linear"):
+        engine(wl, {1: adapters[0]})
+    with pytest.raises(ValueError, match="same number"):
+        engine(wl, {0: adapters[0], 2: tuple(t[:1] for t in adapters[2])})
+    with pytest.raises(Exception, match="SHAPE MISMATCH"):
+        engine(wl, {0: adapters[2]})
+    eng = engine(wl, adapters)
+    box = (l0.to(dev()), u0.to(dev()))
+    with pytest.raises(Exception, match="SHAPE MISMATCH"):
+        eng.run(*box, spec, adapter_ids=ids.long().to(dev()))
+    with pytest.raises(Exception, match="SHAPE MISMATCH"):
+        eng.run(*box, spec, adapter_ids=ids[:2].to(dev()))
+    with pytest.raises(ValueError, match="without adapters"):
+        engine(wl, None).run(*box, spec, adapter_ids=ids.to(dev()))
+    with pytest.raises(Exception, match="SHAPE MISMATCH"):
+        eng.answer(*box, y.to(dev()), ops.AnswerRules(2, 10))
+    with pytest.raises(Exception, match="SHAPE MISMATCH"):
+        eng.answer(*box, y.int().to(dev()), ops.AnswerRules(6, 10))
