@@ -112,6 +112,7 @@ def _load():
         "cf_adapter_workspace_bytes": (_sz, [P(CfAdapterLayer), _i32, _i64, _i64]),
         "cf_adapter_matmul": (_i32, [P(CfAdapterLayer), _i32, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _sz,
                                      _vp]),
+        "cf_adapter_check": (_i32, [_vp]),
         "cf_edit_logits": (_i32, [P(CfAnswerRules), _i32, _vp, _i64, _vp, _i64, _vp]),
         "cf_answer_margin": (_i32, [P(CfAnswerRules), _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
         "cf_profile_enable": (_i32, [_i32]),
@@ -135,8 +136,8 @@ EXPORTED = ("cf_network_neurons", "cf_deeppoly_workspace_bytes", "cf_deeppoly_ru
             "cf_relu_relax",
             "cf_backsub_step", "cf_concretize", "cf_ew_binary", "cf_ew_unary", "cf_ew_where", "cf_ew_clamp",
             "cf_ew_any", "cf_bmm", "cf_conv_densify", "cf_conv_apply", "cf_conv_scale", "cf_conv_transpose",
-            "cf_adapter_workspace_bytes", "cf_adapter_matmul", "cf_edit_logits", "cf_answer_margin",
-            "cf_input_box", "cf_spec_matrix", "cf_profile_enable", "cf_profile_collect",
+            "cf_adapter_workspace_bytes", "cf_adapter_matmul", "cf_adapter_check", "cf_edit_logits",
+            "cf_answer_margin", "cf_input_box", "cf_spec_matrix", "cf_profile_enable", "cf_profile_collect",
             "cf_last_error", "cf_version")
 
 

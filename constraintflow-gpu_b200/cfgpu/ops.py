@@ -299,12 +299,19 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
             out = torch.zeros(T, N, dtype=layer.dtype, device=dev)
         need = _lib.lib.cf_adapter_workspace_bytes(layer._ref, int(substitute), T, Q)
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        LAUNCHES[0] += 2
+        LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
         st = _lib.lib.cf_adapter_matmul(layer._ref, int(substitute), T, x.data_ptr(), _row_stride(x), Q,
                                         offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
                                         ws.data_ptr(), need, _stream())
     _lib.check(st, "cf_adapter_matmul")
     return out
+
+
+def adapter_check(device=None):
+    """Wait for the current stream and raise if a bounded device-side wait of an adapter_matmul
+    on `device` gave up since the last check (its rows are not valid then)."""
+    with _on(torch.device("cuda") if device is None else device):
+        _lib.check(_lib.lib.cf_adapter_check(_stream()), "cf_adapter_check")
 
 
 class AnswerRules:

@@ -1,0 +1,762 @@
+// Tensor-core tiles of the adapter product (cf_adapter.cuh): 128 rows x kBN columns of
+// x [M | Q_e], float32 accumulators in TMEM.
+//
+//   k_adapter_tile<.., kShrink = true>   v = s_e x P_e for the rows of one request in one row tile
+//   k_adapter_tile<.., kShrink = false>  y = x M + b + v Q_e
+//
+// The contraction is dealt out to the CTAs of a cluster (few tiles: one token's product is as
+// wide as the weights, so the cluster makes enough CTAs to read them at full bandwidth); the
+// parts meet in shared memory, each CTA summing every rank's part of its own rows in rank order.
+// A row tile whose rows all carry one adapter takes v Q_e as further steps of the contraction;
+// other tiles add it row by row on the CUDA cores, where a row reads its own adapter only.
+//
+// Operands in shared memory are 128-byte-swizzled images, 128 bytes of the contraction a row:
+//   TMA:    16-bit data by tensor maps; M and Q_e with n contiguous (substitution) stay as they
+//           lie, as MN-major images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
+//   loads:  any stride and alignment, and float32, by the epilogue's warps; float32 is split into
+//           tf32 hi + lo planes (3xTF32: hi*hi + hi*lo + lo*hi).
+#include <cooperative_groups.h>
+#include <cuda.h>
+
+#include "cf_adapter.cuh"
+#include "cf_tc.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace cf {
+namespace adapter {
+namespace {
+
+using namespace tc;
+
+constexpr int kWorkers = 256;  // warps 0-7: loads, epilogue
+constexpr int kProducerWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 320;
+
+// A bounded wait that gave up leaves its site here (cf_adapter_check).
+__device__ int g_err;
+
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: float32 accumulator, A and B of type ab (0 f16, 1 bf16, 2 tf32), A
+// K-major, B K-major or (bit 16) MN-major, 128 x n.
+__device__ __forceinline__ uint32_t idesc(uint32_t ab, uint32_t n, bool mn_major) {
+  return (1u << 4) | (ab << 7) | (ab << 10) | ((uint32_t)mn_major << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
+}
+
+// MN-major, 128-byte swizzle: 64 columns (128 B) x 8 contraction steps an atom; groups of 8 steps
+// 1024 B apart, blocks of 64 columns 64 steps x 128 B = 8192 B apart.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <typename T>
+struct Kind;  // of a type: elements in 128 bytes, planes of an operand, descriptor type
+template <>
+struct Kind<float> {
+  static constexpr int kStep = 32, kPlanes = 2, kAb = 2;
+};
+template <>
+struct Kind<__nv_bfloat16> {
+  static constexpr int kStep = 64, kPlanes = 1, kAb = 1;
+};
+template <>
+struct Kind<__half> {
+  static constexpr int kStep = 64, kPlanes = 1, kAb = 0;
+};
+
+struct Maps {
+  CUtensorMap x, b, v_hi, v_lo, q;
+};
+
+struct Tiling {
+  int64_t m_tiles, units;  // units: clusters that work on tiles; behind them, clusters that plan tiles
+  int32_t split;           // CTAs of a cluster
+  int32_t x_rows;          // rows of a TMA box of x
+  int32_t whole;           // plan_tile
+  int32_t q_tma;           // v Q_e can be a further step of the contraction
+  int32_t dependent;       // launched while the shrink kernel may still run
+};
+
+template <int kStages>
+struct Bars {
+  uint64_t full[kStages], empty[kStages], done;
+  uint32_t tmem;
+};
+
+// 16 bytes of row `row` (elements k .. of n_k), zero beyond
+template <typename T>
+__device__ __forceinline__ uint4 load16(const T* row, int64_t k, int64_t n_k, bool vec) {
+  constexpr int E = 16 / sizeof(T);
+  if (vec && k + E <= n_k) return *(const uint4*)(row + k);
+  alignas(16) T t[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) t[i] = k + i < n_k ? row[k + i] : from_f32<T>(0.0f);
+  return *(const uint4*)t;
+}
+
+// a 16-byte chunk of one operand row into its plane(s)
+template <typename T>
+__device__ __forceinline__ void put(uint32_t plane, uint32_t plane_bytes, uint32_t row, uint32_t chunk, uint4 d) {
+  const uint32_t at = plane + row * 128u + ((chunk ^ (row & 7u)) << 4);
+  if constexpr (Kind<T>::kPlanes == 2) {
+    float hi[4], lo[4];
+    split_tf32(__uint_as_float(d.x), hi[0], lo[0]);
+    split_tf32(__uint_as_float(d.y), hi[1], lo[1]);
+    split_tf32(__uint_as_float(d.z), hi[2], lo[2]);
+    split_tf32(__uint_as_float(d.w), hi[3], lo[3]);
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(hi[0]), "f"(hi[1]), "f"(hi[2]), "f"(hi[3])
+                 : "memory");
+    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + plane_bytes), "f"(lo[0]), "f"(lo[1]),
+                 "f"(lo[2]), "f"(lo[3])
+                 : "memory");
+  } else {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(d.x), "r"(d.y), "r"(d.z), "r"(d.w)
+                 : "memory");
+  }
+}
+
+// y columns n .. n+3 of row t
+template <typename T>
+__device__ __forceinline__ void store4(const Problem& p, int64_t t, int64_t n, const float (&a)[4]) {
+  T* y = (T*)p.y + t * p.y_rs + n;
+  if (p.y_vec && n + 4 <= p.N) {
+    alignas(16) T o[4] = {from_f32<T>(a[0]), from_f32<T>(a[1]), from_f32<T>(a[2]), from_f32<T>(a[3])};
+    if constexpr (sizeof(T) == 4)
+      *(uint4*)y = *(const uint4*)o;
+    else
+      *(uint2*)y = *(const uint2*)o;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < p.N) y[i] = from_f32<T>(a[i]);
+  }
+}
+
+// a += v[t] Q_e at columns n .. n+3 (columns beyond N are not read)
+template <typename T, bool kSub>
+__device__ __forceinline__ void add_lowrank(const Problem& p, int64_t t, int e, int rank, int64_t n, float (&a)[4]) {
+  const float* v = p.v + t * p.v_rs;
+  const T* Q = (const T*)p.Qm + e * p.q_es;
+  if constexpr (kSub) {  // rows of n
+    const bool full = n + 4 <= p.N;
+#pragma unroll 4
+    for (int r = 0; r < rank; ++r) {
+      const T* q = Q + r * p.q_rs + n;
+      const float w = v[r];
+      if (full && p.q_vec) {
+        alignas(16) T d[4];
+        if constexpr (sizeof(T) == 4)
+          *(uint4*)d = *(const uint4*)q;
+        else
+          *(uint2*)d = *(const uint2*)q;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = fmaf(w, to_f32(d[i]), a[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.N) a[i] = fmaf(w, to_f32(q[i]), a[i]);
+      }
+    }
+  } else {  // rows of r
+    constexpr int E = 16 / sizeof(T);
+    int r = 0;
+    if (p.q_vec) {
+      for (; r + E <= rank; r += E) {
+        float w[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i] = v[r + i];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (n + c >= p.N) break;
+          alignas(16) T d[E];
+          *(uint4*)d = *(const uint4*)(Q + (n + c) * p.q_ns + r);
+#pragma unroll
+          for (int i = 0; i < E; ++i) a[c] = fmaf(w[i], to_f32(d[i]), a[c]);
+        }
+      }
+    }
+    for (; r < rank; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        if (n + c < p.N) a[c] = fmaf(v[r], to_f32(Q[(n + c) * p.q_ns + r]), a[c]);
+  }
+}
+
+template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
+__global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_adapter_tile(const Problem p, const __grid_constant__ Maps maps,
+                                                           const Tiling g) {
+  constexpr int kStep = Kind<T>::kStep, kPlanes = Kind<T>::kPlanes;
+  constexpr bool kMn = kTma && kSub;  // B images lie n-contiguous
+  constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128;
+  constexpr uint32_t kStageBytes = (kABytes + kBBytes) * kPlanes;
+  static_assert((kBM * (kBN + 4)) * 4 <= kStageBytes * kStages, "the tile is staged where the operands were");
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Bars<kStages> bars;
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem);
+  cg::cluster_group cl = cg::this_cluster();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = g.split;
+  const int rank = split > 1 ? (int)cl.block_rank() : 0;
+  const int64_t unit = blockIdx.x / split;
+
+  // ---- which tile
+  int64_t m, n0 = 0, row0 = 0, row1 = 0;  // rows [row0, row1) of the tile are this unit's (shrink)
+  int e = kNone, e_rank = 0, r0 = 0;
+  if constexpr (kShrink) {
+    launch_dependents();
+    const int64_t blocks_r = (p.R + kBN - 1) / kBN;
+    if (unit >= g.units) {
+      const int64_t tile = ((unit - g.units) * split + rank) * (kThreads / 32) + warp;
+      if (tile < g.m_tiles) plan_tile(p, tile, g.whole);
+      return;
+    }
+    const int64_t u = unit / blocks_r;
+    r0 = (int)(unit - u * blocks_r) * kBN;
+    // Units are the steps of the staircase of (tile, request) pairs: tile + request is different
+    // for each pair that overlaps.  Request q of unit u: the first that ends behind tile u - q's start.
+    int64_t lo = 0, hi = p.Q;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (p.offsets[mid + 1] + kBM * mid > kBM * u)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    if (lo >= p.Q) return;
+    m = u - lo;
+    if (m < 0 || m >= g.m_tiles) return;
+    row0 = max(p.offsets[lo], m * kBM);
+    row1 = min(min(p.offsets[lo + 1], (m + 1) * kBM), p.T);
+    e = adapter_of(p, lo);
+    e_rank = rank_of(p, e);
+    if (row0 >= row1 || e < 0 || r0 >= e_rank) return;  // the whole cluster returns
+  } else {
+    m = unit % g.m_tiles;
+    n0 = unit / g.m_tiles * kBN;
+  }
+  const int64_t t0 = m * kBM;
+  const int rows = (int)min((int64_t)kBM, p.T - t0);
+  // columns that the MMAs take, a multiple of 16
+  const int cols = kShrink ? min(kBN, (min(p.R - r0, kBN) + 15) / 16 * 16) : kBN;
+
+  const int n_k = (int)((p.K + kStep - 1) / kStep);
+  const int kb = (int)((int64_t)n_k * rank / split), ke = (int)((int64_t)n_k * (rank + 1) / split);
+
+  // ---- set-up
+  if (warp == kMmaWarp) tmem_alloc(&bars.tmem, kBN < 32 ? 32 : kBN);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars.full[i], kTma ? 1 : kWorkers);
+      mbar_init(&bars.empty[i], 1);
+    }
+    mbar_init(&bars.done, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  int* err = &g_err;
+
+  // The low-rank steps behind the contraction: only known once the shrink kernel is done.
+  auto lowrank_steps = [&](int& te, int& tr) {
+    te = kNone, tr = 0;
+    if (kShrink || rank != 0 || p.R == 0 || !g.q_tma) return 0;
+    dependency_wait();
+    te = *(volatile int*)(p.tile_e + m);
+    if (te < 0) return 0;
+    tr = rank_of(p, te);
+    const int steps = (tr + kStep - 1) / kStep;
+    return kTma ? 2 * steps : steps;
+  };
+
+  bool ok = true;
+  if (kTma && warp == kProducerWarp && lane == 0) {
+    int it = 0, te, tr;
+    auto stage_for = [&](uint32_t bytes) -> int {
+      const int s = it % kStages, round = it / kStages;
+      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 11)) return -1;
+      mbar_arrive_expect_tx(&bars.full[s], bytes);
+      ++it;
+      return s;
+    };
+    const uint32_t a_bytes = (uint32_t)g.x_rows * 128;
+    // B image: `bcols` columns from column c on, contraction from k on, of map entry z
+    auto load_b = [&](uint32_t dst, const CUtensorMap* map, int c, int k, int z, int bcols, uint64_t* bar) {
+      if constexpr (kMn) {
+        for (int j = 0; j < bcols; j += 64) tma_3d(dst + j * 128, map, c + j, k, z, bar);
+      } else {
+        tma_3d(dst, map, k, c, z, bar);
+      }
+    };
+    const int bcols = kMn ? (cols + 63) / 64 * 64 : kBN;
+    for (int k = kb; k < ke && ok; ++k) {
+      const int s = stage_for(a_bytes + bcols * 128);
+      if (s < 0) {
+        ok = false;
+        break;
+      }
+      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
+      tma_3d(a, &maps.x, k * kStep, (int)t0, 0, &bars.full[s]);
+      load_b(b, &maps.b, (int)(kShrink ? r0 : n0), k * kStep, kShrink ? e : 0, bcols, &bars.full[s]);
+    }
+    if constexpr (!kShrink) {
+      const int extra = ok ? lowrank_steps(te, tr) : 0;
+      for (int i = 0; i < extra && ok; ++i) {
+        const int s = stage_for(a_bytes + kBN * 128);
+        if (s < 0) {
+          ok = false;
+          break;
+        }
+        const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
+        const int r = i / 2 * kStep;
+        tma_3d(a, i & 1 ? &maps.v_lo : &maps.v_hi, r, (int)t0, 0, &bars.full[s]);
+        load_b(b, &maps.q, (int)n0, r, te, kBN, &bars.full[s]);
+      }
+    }
+    if (!ok)  // copies in flight land before shared memory is given up
+      for (int i = max(0, it - kStages); i < it; ++i)
+        mbar_wait_drain(&bars.full[i % kStages], (i / kStages) & 1, err, 12);
+  } else if (warp == kMmaWarp && lane == 0) {
+    int it = 0, te = kNone, tr = 0;
+    const uint32_t id = idesc(Kind<T>::kAb, cols, kMn);
+    auto step = [&](int k16) -> bool {  // k16: MMAs of this step
+      const int s = it % kStages, round = it / kStages;
+      if (!mbar_wait(&bars.full[s], round & 1, err, 21)) return false;
+      tc_fence_after();
+      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes * kPlanes;
+      const uint64_t ad = sw128_desc(a), bd = kMn ? mn_desc(b) : sw128_desc(b);
+      constexpr uint64_t kAStep = 32 >> 4, kBStep = kMn ? (16 * 128) >> 4 : 32 >> 4;
+      for (int j = 0; j < k16; ++j) {
+        const uint32_t acc = it > 0 || j > 0;
+        if constexpr (kPlanes == 2) {
+          constexpr uint64_t kALo = kABytes >> 4, kBLo = kBBytes >> 4;
+          mma_tf32(tmem, ad + j * kAStep, bd + j * kBStep, id, acc);
+          mma_tf32(tmem, ad + j * kAStep, bd + kBLo + j * kBStep, id, 1);
+          mma_tf32(tmem, ad + kALo + j * kAStep, bd + j * kBStep, id, 1);
+        } else {
+          mma_f16(tmem, ad + j * kAStep, bd + j * kBStep, id, acc);
+        }
+      }
+      mma_commit(&bars.empty[s]);
+      ++it;
+      return true;
+    };
+    for (int k = kb; k < ke && ok; ++k) ok = step(4);
+    if constexpr (!kShrink) {
+      const int extra = ok ? lowrank_steps(te, tr) : 0;
+      constexpr int kMma = kStep / 4;  // contraction of one MMA
+      for (int i = 0; i < extra && ok; ++i) {
+        const int r = (kTma ? i / 2 : i) * kStep;
+        ok = step((min(tr - r, kStep) + kMma - 1) / kMma);
+      }
+    }
+    mma_commit(&bars.done);
+    if (!ok) mbar_wait_drain(&bars.done, 0, err, 22);
+  } else if (!kTma && warp < kProducerWarp) {
+    // ---- loads: the chunks of the next step are in registers while the MMAs run
+    constexpr int kXTasks = kBM * 8 / kWorkers, kBTasks = kBN * 8 / kWorkers;
+    constexpr int E = 16 / sizeof(T);
+    uint4 xr[kXTasks], br[kBTasks];
+    const int chunk = threadIdx.x & 7, prow = threadIdx.x >> 3;  // K-contiguous rows
+    // one operand row's chunk with k scattered (n contiguous in memory)
+    auto gather = [&](const T* base, int64_t ks, int64_t k, int64_t n_kk) -> uint4 {
+      alignas(16) T t[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i) t[i] = k + i < n_kk ? base[(k + i) * ks] : from_f32<T>(0.0f);
+      return *(const uint4*)t;
+    };
+    auto fetch_b = [&](const T* B, int64_t ks, int64_t ns, int64_t c0, int64_t n_c, int64_t k0, int64_t n_kk,
+                       bool vec) {
+#pragma unroll
+      for (int j = 0; j < kBTasks; ++j) {
+        if constexpr (kSub) {  // consecutive threads: consecutive columns
+          const int task = j * kWorkers + threadIdx.x;
+          const int64_t c = c0 + task % kBN, k = k0 + (task / kBN) * E;
+          br[j] = c < n_c ? gather(B + c * ns, ks, k, n_kk) : make_uint4(0, 0, 0, 0);
+        } else {
+          const int64_t c = c0 + prow + j * (kWorkers / 8), k = k0 + chunk * E;
+          br[j] = c < n_c ? load16<T>(B + c * ns, k, n_kk, vec) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+    int it = 0, te = kNone, tr = 0;
+    auto put_step = [&]() -> bool {
+      const int s = it % kStages, round = it / kStages;
+      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 31)) return false;
+      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes * kPlanes;
+#pragma unroll
+      for (int j = 0; j < kXTasks; ++j) put<T>(a, kABytes, prow + j * (kWorkers / 8), chunk, xr[j]);
+#pragma unroll
+      for (int j = 0; j < kBTasks; ++j) {
+        if constexpr (kSub) {
+          const int task = j * kWorkers + threadIdx.x;
+          put<T>(b, kBBytes, task % kBN, task / kBN, br[j]);
+        } else {
+          put<T>(b, kBBytes, prow + j * (kWorkers / 8), chunk, br[j]);
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bars.full[s]);
+      ++it;
+      return true;
+    };
+    auto fetch = [&](int k) {
+#pragma unroll
+      for (int j = 0; j < kXTasks; ++j) {
+        const int64_t t = t0 + prow + j * (kWorkers / 8);
+        xr[j] = t < p.T ? load16<T>((const T*)p.x + t * p.x_rs, (int64_t)k * kStep + chunk * E, p.K, p.x_vec)
+                        : make_uint4(0, 0, 0, 0);
+      }
+      if constexpr (kShrink)
+        fetch_b((const T*)p.P + e * p.p_es, p.p_ks, p.p_rs, r0, min(e_rank, r0 + kBN), (int64_t)k * kStep, p.K,
+                p.p_vec);
+      else
+        fetch_b((const T*)p.M, p.m_ks, p.m_ns, n0, p.N, (int64_t)k * kStep, p.K, p.m_vec);
+    };
+    if (kb < ke) fetch(kb);
+    for (int k = kb; k < ke && ok; ++k) {
+      ok = put_step();
+      if (k + 1 < ke) fetch(k + 1);
+    }
+    if constexpr (!kShrink && kPlanes == 2) {
+      const int extra = ok ? lowrank_steps(te, tr) : 0;
+      for (int i = 0; i < extra && ok; ++i) {
+        const int64_t r = (int64_t)i * kStep;
+#pragma unroll
+        for (int j = 0; j < kXTasks; ++j) {
+          const int64_t t = t0 + prow + j * (kWorkers / 8);
+          // rows of v are 16-byte aligned, v_rs a multiple of 8; beyond the rank: zeros
+          xr[j] = t < p.T ? load16<T>((const T*)(p.v + t * p.v_rs), r + chunk * E, tr, true)
+                          : make_uint4(0, 0, 0, 0);
+        }
+        fetch_b((const T*)p.Qm + te * p.q_es, p.q_rs, p.q_ns, n0, p.N, r, tr, p.q_vec);
+        ok = put_step();
+      }
+    }
+  }
+
+  // ---- the accumulators, staged in shared memory
+  __syncwarp();
+  float* part = (float*)smem;
+  constexpr int kLd = kBN + 4;
+  int te = kNone;
+  if (warp < kProducerWarp) {
+    ok = mbar_wait(&bars.done, 0, err, 41);
+    tc_fence_after();
+    const int row = (warp & 3) * 32 + lane;
+    const bool any = kb < ke;  // else the accumulators were never written (or by low-rank steps only)
+    bool low = false;
+    if (!kShrink && p.R > 0) {
+      if (g.dependent) dependency_wait();
+      te = p.tile_e[m];
+      low = te >= 0 && g.q_tma && rank == 0;
+    }
+    const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    for (int c = (warp >> 2) * 16; c < cols; c += 32) {
+      float v[16];
+      tmem_ld16(src + c, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *(float4*)(part + row * kLd + c + i) = any || low ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3])
+                                                          : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_relinquish();
+    tmem_dealloc(tmem, kBN < 32 ? 32 : kBN);
+  }
+  if (split > 1) cl.sync();
+  if (warp < kProducerWarp) {
+    auto sum4 = [&](int row, int c) -> float4 {
+      float4 s = *(const float4*)((split > 1 ? cl.map_shared_rank(part, 0) : part) + row * kLd + c);
+      for (int i = 1; i < split; ++i) {
+        const float4 q = *(const float4*)(cl.map_shared_rank(part, i) + row * kLd + c);
+        s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+      }
+      return s;
+    };
+    if constexpr (kShrink) {
+      const int a = (int)(row0 - t0), b = (int)(row1 - t0), quads = cols / 4;
+      const float scale = p.scale[e];
+      for (int i = rank * kWorkers + threadIdx.x; i < (b - a) * quads; i += split * kWorkers) {
+        const int row = a + i / quads, c = i % quads * 4;
+        const float4 s = sum4(row, c);
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (r0 + c + j < e_rank) store_v(p, t0 + row, r0 + c + j, scale * v[j]);
+      }
+    } else {
+      const int64_t n = n0 + lane * 4;
+      float bias[4] = {};
+      if (p.bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.N) bias[i] = to_f32(((const T*)p.bias)[n + i]);
+      for (int row = rank + warp * split; row < rows; row += 8 * split) {
+        const int64_t t = t0 + row;
+        const int64_t q = request_of(p, t);
+        if (q < 0 || n >= p.N || lane * 4 >= kBN) continue;
+        const float4 s = sum4(row, lane * 4);
+        float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
+        if (te == kMixed || (te >= 0 && !g.q_tma)) {
+          const int re = adapter_of(p, q);
+          add_lowrank<T, kSub>(p, t, re, rank_of(p, re), n, a);
+        }
+        store4<T>(p, t, n, a);
+      }
+    }
+  }
+  __syncwarp();
+  if (split > 1) cl.sync();  // nobody leaves while its part is read
+}
+
+// v for rows whose requests are short (a tile of the tensor cores would hold few rows of each):
+// one CTA per row and kRows columns of v.  Behind the rows, CTAs that plan row tiles.
+constexpr int kRowThreads = 256;
+template <bool kSub>
+constexpr int kRowCols = kSub ? 16 : kRowThreads / 32;
+
+template <typename T, bool kSub>
+__global__ void __launch_bounds__(kRowThreads) k_adapter_shrink_rows(const Problem p, int64_t m_tiles, int whole) {
+  launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t t = blockIdx.x;
+  if (t >= p.T) {
+    const int64_t tile = (t - p.T) * (kRowThreads / 32) + warp;
+    if (blockIdx.y == 0 && tile < m_tiles) plan_tile(p, tile, whole);
+    return;
+  }
+  const int e = adapter_of(p, request_of(p, t)), rank = rank_of(p, e);
+  const int r0 = blockIdx.y * kRowCols<kSub>;
+  if (r0 >= rank) return;
+  const T* x = (const T*)p.x + t * p.x_rs;
+  const T* P = (const T*)p.P + e * p.p_es;
+  if constexpr (kSub) {  // rows of r: 16 columns x 16 steps of k at a time
+    __shared__ float sums[kRowThreads / 32][16];
+    const int r = r0 + (threadIdx.x & 15);
+    float acc = 0.0f;
+    if (r < rank) {
+#pragma unroll 8
+      for (int64_t k = threadIdx.x >> 4; k < p.K; k += kRowThreads / 16)
+        acc = fmaf(to_f32(x[k]), to_f32(P[k * p.p_ks + r]), acc);
+    }
+    acc += __shfl_xor_sync(0xffffffffu, acc, 16);
+    if (lane < 16) sums[warp][lane] = acc;
+    __syncthreads();
+    if (threadIdx.x < 16 && r < rank) {
+      float v = 0.0f;
+      for (int i = 0; i < kRowThreads / 32; ++i) v += sums[i][threadIdx.x];
+      store_v(p, t, r, p.scale[e] * v);
+    }
+  } else {  // rows of k: a warp a column
+    constexpr int E = 16 / sizeof(T);
+    const int r = r0 + warp;
+    if (r >= rank) return;
+    P += r * p.p_rs;
+    float acc = 0.0f;
+#pragma unroll 4
+    for (int64_t k = lane * E; k < p.K; k += 32 * E) {
+      alignas(16) T a[E], b[E];
+      *(uint4*)a = load16<T>(x, k, p.K, p.x_vec);
+      *(uint4*)b = load16<T>(P, k, p.K, p.p_vec);
+#pragma unroll
+      for (int i = 0; i < E; ++i) acc = fmaf(to_f32(a[i]), to_f32(b[i]), acc);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (lane == 0) store_v(p, t, r, p.scale[e] * acc);
+  }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+  static EncodeFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+    return (EncodeFn)f;
+  }();
+  return fn;
+}
+
+// [z][y][x] of 16-bit elements, x contiguous, boxes of 64 x box_y, 128-byte swizzle, zeros outside
+cf_status encode(CUtensorMap* map, int dtype, const void* base, int64_t nx, int64_t ny, int64_t nz, int64_t ys,
+                 int64_t zs, int box_y) {
+  EncodeFn fn = encoder();
+  CF_REQUIRE(fn, CF_ERR_CUDA, "adapter_matmul: cuTensorMapEncodeTiled is not available");
+  const cuuint64_t dims[3] = {(cuuint64_t)nx, (cuuint64_t)ny, (cuuint64_t)nz};
+  const cuuint64_t strides[2] = {(cuuint64_t)ys * 2, (cuuint64_t)(nz > 1 ? zs : ys * ny) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)box_y, 1}, ones[3] = {1, 1, 1};
+  CUresult r = fn(map, dtype == CF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                  const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CF_REQUIRE(r == CUDA_SUCCESS, CF_ERR_CUDA, "adapter_matmul: tensor map: error %d", (int)r);
+  return CF_OK;
+}
+
+template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
+cf_status launch(const char* what, const Problem& p, const Maps& maps, const Tiling& g, int64_t clusters,
+                 cudaStream_t st) {
+  constexpr int smem = (kBM + kBN) * 128 * Kind<T>::kPlanes * kStages + 1024;
+  auto* kern = k_adapter_tile<T, kSub, kShrink, kTma, kBN, kStages>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  const int64_t blocks = clusters * g.split;
+  CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "%s: too many tiles", what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)g.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = g.dependent ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, p, maps, g);
+  if (e != cudaSuccess) {
+    set_error("%s: %s", what, cudaGetErrorString(e));
+    return CF_ERR_CUDA;
+  }
+  return check_launch(what);
+}
+
+// CTAs of a cluster: as many as keep the grid within two waves of single CTAs, each with at
+// least four steps of the contraction.
+int split_for(int64_t tiles, int64_t steps) {
+  int s = 1;
+  while (s < 8 && tiles * s * 2 <= 2 * 148 && steps >= s * 2 * 4) s *= 2;
+  return s;
+}
+
+template <typename T, bool kSub, bool kTma>
+cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cudaStream_t st) {
+  constexpr int kStep = Kind<T>::kStep, kStages = 3;
+  const int64_t steps = ceil_div(p.K, kStep), m_tiles = ceil_div(p.T, kBM);
+  Maps maps = {};
+  Tiling g = {};
+  g.m_tiles = m_tiles;
+  g.x_rows = (int)(p.T < kBM ? ceil_div(p.T, 8) * 8 : kBM);
+  constexpr bool f32 = Kind<T>::kPlanes == 2;
+  // float16's range does not hold every intermediate that float32 does: row by row instead
+  const bool pair = kTma && dtype == CF_BF16 && lowrank_tma;
+  g.q_tma = pair || (f32 && !kTma);
+  g.whole = pair ? 16 : f32 ? 1 : 0;
+  if (kTma) CF_TRY(encode(&maps.x, dtype, p.x, p.K, p.T, 1, p.x_rs, p.x_rs * p.T, g.x_rows));
+  if (p.R > 0 && row_shrink) {
+    const int64_t blocks = p.T + ceil_div(m_tiles, kRowThreads / 32);
+    CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "adapter_matmul: too many rows");
+    const dim3 grid((unsigned)blocks, (unsigned)ceil_div(p.R, kRowCols<kSub>));
+    k_adapter_shrink_rows<T, kSub><<<grid, kRowThreads, 0, st>>>(p, m_tiles, g.whole);
+    CF_TRY(check_launch("k_adapter_shrink_rows"));
+  } else if (p.R > 0) {
+    const int bn = p.R <= 64 ? 64 : 128;
+    const bool by_tma = kTma && lowrank_tma;
+    if (by_tma) {
+      if (kSub)
+        CF_TRY(encode(&maps.b, dtype, p.P, p.R, p.K, p.E, p.p_ks, p.p_es, 64));
+      else
+        CF_TRY(encode(&maps.b, dtype, p.P, p.K, p.R, p.E, p.p_rs, p.p_es, bn));
+    }
+    g.units = (m_tiles + p.Q - 1) * ceil_div(p.R, bn);
+    g.split = split_for(m_tiles, steps);
+    const int64_t plans = ceil_div(m_tiles, (int64_t)g.split * (kThreads / 32));
+    const int64_t clusters = g.units + plans;
+    const char* what = "k_adapter_tile (shrink)";
+    if (by_tma)
+      CF_TRY(bn == 64 ? (launch<T, kSub, true, kTma, 64, kStages>(what, p, maps, g, clusters, st))
+                      : (launch<T, kSub, true, kTma, 128, kStages>(what, p, maps, g, clusters, st)));
+    else
+      CF_TRY(bn == 64 ? (launch<T, kSub, true, false, 64, kStages>(what, p, maps, g, clusters, st))
+                      : (launch<T, kSub, true, false, 128, kStages>(what, p, maps, g, clusters, st)));
+  }
+  constexpr int bn = 128;
+  if (kTma) {
+    if (kSub)
+      CF_TRY(encode(&maps.b, dtype, p.M, p.N, p.K, 1, p.m_ks, p.m_ks * p.K, 64));
+    else
+      CF_TRY(encode(&maps.b, dtype, p.M, p.K, p.N, 1, p.m_ns, p.m_ns * p.N, bn));
+    if (pair && p.R > 0) {
+      CF_TRY(encode(&maps.v_hi, dtype, p.v_hi, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
+      CF_TRY(encode(&maps.v_lo, dtype, p.v_lo, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
+      if (kSub)
+        CF_TRY(encode(&maps.q, dtype, p.Qm, p.N, p.R, p.E, p.q_rs, p.q_es, 64));
+      else
+        CF_TRY(encode(&maps.q, dtype, p.Qm, p.R, p.N, p.E, p.q_ns, p.q_es, bn));
+    }
+  }
+  g.dependent = p.R > 0;
+  g.units = m_tiles * ceil_div(p.N, bn);
+  g.split = split_for(g.units, steps);
+  return launch<T, kSub, false, kTma, bn, kStages>("k_adapter_tile", p, maps, g, g.units, st);
+}
+
+}  // namespace
+
+cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool tma, bool row_shrink, bool lowrank_tma,
+                       cudaStream_t st) {
+  if (dtype == CF_F32)
+    return substitute ? run<float, true, false>(p, dtype, row_shrink, lowrank_tma, st)
+                      : run<float, false, false>(p, dtype, row_shrink, lowrank_tma, st);
+  if (dtype == CF_BF16) {
+    if (tma)
+      return substitute ? run<__nv_bfloat16, true, true>(p, dtype, row_shrink, lowrank_tma, st)
+                        : run<__nv_bfloat16, false, true>(p, dtype, row_shrink, lowrank_tma, st);
+    return substitute ? run<__nv_bfloat16, true, false>(p, dtype, row_shrink, lowrank_tma, st)
+                      : run<__nv_bfloat16, false, false>(p, dtype, row_shrink, lowrank_tma, st);
+  }
+  if (tma)
+    return substitute ? run<__half, true, true>(p, dtype, row_shrink, lowrank_tma, st)
+                      : run<__half, false, true>(p, dtype, row_shrink, lowrank_tma, st);
+  return substitute ? run<__half, true, false>(p, dtype, row_shrink, lowrank_tma, st)
+                    : run<__half, false, false>(p, dtype, row_shrink, lowrank_tma, st);
+}
+
+cf_status check_waits(cudaStream_t st) {
+  int site = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&site, g_err, sizeof(site), 0, cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && site != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbolAsync(g_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "adapter_check: %s", cudaGetErrorString(e));
+  CF_REQUIRE(site == 0, CF_ERR_TIMEOUT, "adapter_matmul: a bounded wait gave up (site %d)", site);
+  return CF_OK;
+}
+
+}  // namespace adapter
+}  // namespace cf

@@ -430,12 +430,16 @@ typedef struct cf_adapter_layer {
  * of no request (before offsets[0], from offsets[n_requests] on) are left as they were.  x and y
  * do not overlap.  A request's rows depend on its own adapter only: infinities or NaN in another
  * adapter or in rows of other requests do not reach them.  Products are accumulated in float32;
- * float32 data is multiplied as 3xTF32, as in the chained substitution. */
+ * float32 data is multiplied as 3xTF32, as in the chained substitution.  The workspace
+ * (256-byte aligned, >= cf_adapter_workspace_bytes) belongs to the call until it has run. */
 size_t cf_adapter_workspace_bytes(const cf_adapter_layer* layer, int32_t substitute, int64_t T,
                                   int64_t n_requests);
 cf_status cf_adapter_matmul(const cf_adapter_layer* layer, int32_t substitute, int64_t T, const void* x_dev,
                             int64_t x_rs, int64_t n_requests, const int64_t* offsets_dev, const int32_t* ids_dev,
                             void* y_dev, int64_t y_rs, void* workspace_dev, size_t workspace_bytes, void* stream);
+/* Synchronise `stream` and report whether a bounded device-side wait of a cf_adapter_matmul on
+ * the current device gave up (CF_ERR_TIMEOUT) since the last check; its rows are not valid. */
+cf_status cf_adapter_check(void* stream);
 
 /* The rule by which each of `rows` rows' answer is taken from its n logits:
  *   tokens_dev [n_tokens] int32, row r's history at token_offsets[r] .. token_offsets[r+1]-1;
