@@ -52,11 +52,12 @@ size_t workspace(const cf_adapter_layer& L, int64_t T, char* base, Problem* p) {
     hi = take((size_t)T * ld * 2);
     lo = take((size_t)T * ld * 2);
   }
-  char* tiles = take((size_t)ceil_div(T, kBM) * 4);
+  char* tile_e = take((size_t)ceil_div(T, kBM) * 4);
+  char* tile_q = take((size_t)ceil_div(T, kBM) * 4);
   if (p) {
     p->v = (float*)v, p->v_rs = ld;
     p->v_hi = (__nv_bfloat16*)hi, p->v_lo = (__nv_bfloat16*)lo;
-    p->tile_e = (int32_t*)tiles;
+    p->tile_e = (int32_t*)tile_e, p->tile_q = (int32_t*)tile_q;
   }
   return at;
 }
@@ -121,10 +122,16 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   // With few rows a request, a tile of the tensor cores would be multiplied once for each of
   // its requests: v row by row on the CUDA cores instead.
   const bool rows = T < 16 * n_requests;
+  if (L->dtype == CF_F32) return launch_f32(p, substitute != 0, rows, as_stream(stream));
   return launch_tiles(p, L->dtype, substitute != 0, tma, rows, lowrank, as_stream(stream));
 }
 
 extern "C" cf_status cf_adapter_check(void* stream) {
   clear_error();
-  return check_waits(as_stream(stream));
+  int site = 0, site_f32 = 0;
+  CF_TRY(take_site_tiles(&site, as_stream(stream)));
+  CF_TRY(take_site_f32(&site_f32, as_stream(stream)));
+  CF_REQUIRE(site == 0 && site_f32 == 0, CF_ERR_TIMEOUT, "adapter_matmul: a bounded wait gave up (site %d)",
+             site ? site : site_f32);
+  return CF_OK;
 }

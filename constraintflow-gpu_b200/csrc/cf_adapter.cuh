@@ -1,5 +1,5 @@
-// The adapter product as its kernels see it (cf_adapter.cu: entry point and plan;
-// cf_adapter_tile.cu: tensor-core tiles).
+// The adapter product as its kernels see it (cf_adapter.cu: entry point, checks and
+// workspace; the kernels: cf_adapter_tile.cu, cf_adapter_f32.cu, cf_adapter_rows.cu).
 #pragma once
 #include "cf_common.cuh"
 #include "cf_elem.cuh"
@@ -28,11 +28,12 @@ struct Problem {
   int64_t y_rs;
   // 16-byte loads of x, M, P and Q_e rows are aligned; vector stores of y are
   int32_t x_vec, m_vec, p_vec, q_vec, y_vec;
-  // workspace: v [T, v_rs] float32; its halves [T, v_rs] bfloat16 (TMA path); tile_e [tiles of rows]
+  // workspace: v [T, v_rs] float32; its halves [T, v_rs] bfloat16 (TMA path); tile_e, tile_q [row tiles]: what
+  // the tile's rows carry, and the first request that reaches into it
   float* v;
   __nv_bfloat16 *v_hi, *v_lo;
   int64_t v_rs;
-  int32_t* tile_e;
+  int32_t *tile_e, *tile_q;
 };
 
 // The request of row t: -1 for a row of no request.
@@ -60,7 +61,7 @@ __device__ __forceinline__ int rank_of(const Problem& p, int e) {
   return p.ranks ? min(max(p.ranks[e], 0), p.R) : p.R;
 }
 
-// tile_e of row tile m, by one warp.  One adapter for all of the tile's rows can be added by the
+// tile_e and tile_q of row tile m, by one warp.  One adapter for all of the tile's rows can be added by the
 // tensor cores: a tile of several would multiply each row with every one of them, and an
 // infinity or NaN of one would reach the others' rows.  `whole`: the ranks that the tensor
 // cores take are R and the multiples of `whole` (0: none), so that nothing beyond an adapter's
@@ -84,7 +85,18 @@ __device__ __forceinline__ void plan_tile(const Problem& p, int64_t m, int whole
     const int r = rank_of(p, e);
     if (!(whole > 0 && (r == p.R || r % whole == 0))) e = kMixed;
   }
-  if (lane == 0) p.tile_e[m] = e;
+  int64_t a = 0, b = p.Q;  // the first request that ends behind the tile's start
+  while (a < b) {
+    const int64_t mid = (a + b) / 2;
+    if (p.offsets[mid + 1] > m * kBM)
+      b = mid;
+    else
+      a = mid + 1;
+  }
+  if (lane == 0) {
+    p.tile_e[m] = e;
+    p.tile_q[m] = (int32_t)a;
+  }
 }
 
 __device__ __forceinline__ void store_v(const Problem& p, int64_t t, int r, float v) {
@@ -99,11 +111,17 @@ __device__ __forceinline__ void store_v(const Problem& p, int64_t t, int r, floa
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// Tensor-core tiles (cf_adapter_tile.cu).  tma: 16-byte aligned 16-bit data, read by TMA.
+// 16-bit data (cf_adapter_tile.cu).  tma: 16-byte aligned operands, read by TMA; lowrank_tma: the
+// adapters too.  row_shrink: v row by row on the CUDA cores (requests of few rows).
 cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool tma, bool row_shrink, bool lowrank_tma,
                        cudaStream_t st);
-// CF_ERR_TIMEOUT if a bounded device wait gave up since the last check on this device
-cf_status check_waits(cudaStream_t st);
+// float32 data (cf_adapter_f32.cu)
+cf_status launch_f32(const Problem& p, bool substitute, bool row_shrink, cudaStream_t st);
+// v row by row, and the plan of the row tiles (cf_adapter_rows.cu)
+cf_status launch_row_shrink(const Problem& p, int dtype, bool substitute, int whole, cudaStream_t st);
+// the first site at which a bounded device wait gave up since the last call on this device (0: none)
+cf_status take_site_tiles(int* site, cudaStream_t st);
+cf_status take_site_f32(int* site, cudaStream_t st);
 
 }  // namespace adapter
 }  // namespace cf

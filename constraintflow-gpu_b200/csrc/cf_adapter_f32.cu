@@ -1,0 +1,509 @@
+// The adapter product for float32 data: 128 x kBN tiles on tcgen05 as 3xTF32.
+//
+//   k_adapter_f32<.., kShrink = true>   v = s_e x P_e for the rows of one request in one row tile
+//   k_adapter_f32<.., kShrink = false>  y = x M + b + v Q_e
+//
+// 3xTF32: an operand is split into tf32 hi + lo, and hi*hi + hi*lo + lo*hi is summed.  The tensor
+// core adds into its accumulator with truncation, an error that grows with every addition and
+// always points towards zero, so a sum stays in the accumulator for kChunk steps of 32 only; the
+// epilogue's warps add the chunks in registers, rounded to nearest.  The error of a sum is then
+// that of 24 truncated additions of a chunk, not of 3 K / 8: against 64 bits about that of a
+// float32 FMA loop.
+//
+// The chunks also keep requests apart: the low-rank part of each request that reaches into the
+// tile is a chunk of its own, added to that request's rows only (a masked operand would not do:
+// 0 * inf of another request's adapter is NaN).  Requests of few rows would make many such chunks;
+// their low-rank part is added row by row on the CUDA cores instead.
+//
+// Warps 0-7 drain chunks and write the tile, warps 8-15 load operands of any stride and alignment
+// (the next step's loads in flight while this step's are split and stored), warp 16 issues the
+// MMAs.  One CTA an SM walks over the tiles, the epilogue of a tile under the MMAs of the next;
+// with few tiles the contraction is dealt out to the CTAs of a cluster instead, which sum their
+// parts in rank order.
+#include <cooperative_groups.h>
+
+#include "cf_adapter_dev.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace cf {
+namespace adapter {
+namespace {
+
+using namespace tc;
+
+constexpr int kDrain = 256, kLoad = 256;  // threads of the two groups
+constexpr int kMmaWarp = 16;
+constexpr int kThreads = 544;
+constexpr int kStep = 32;   // contraction of a stage: 128 bytes
+constexpr int kChunk = 2;   // steps of one accumulation
+constexpr int kStages = 2, kBufs = 2;
+
+// A bounded wait that gave up leaves its site here (cf_adapter_check).
+__device__ int g_err;
+
+struct Tiling {
+  int64_t m_tiles, units, clusters;  // clusters: on tiles; behind them, clusters that plan row tiles
+  int32_t split;                     // CTAs of a cluster
+  int32_t rowwise;                   // the low-rank part row by row
+  int32_t dependent;                 // launched while the shrink kernel may still run
+};
+
+struct Tile {
+  int64_t m, t0, n0, row0, row1;  // shrink: rows [row0, row1)
+  int e, e_rank, r0, cols;
+};
+
+// The tile of a unit; false: nothing to do.
+template <bool kShrink, int kBN>
+__device__ __forceinline__ bool tile_of(const Problem& p, const Tiling& g, int64_t unit, Tile& w) {
+  w.n0 = w.row0 = w.row1 = 0;
+  w.e = kNone, w.e_rank = w.r0 = 0;
+  if constexpr (kShrink) {
+    const int64_t blocks_r = (p.R + kBN - 1) / kBN, u = unit / blocks_r;
+    w.r0 = (int)(unit - u * blocks_r) * kBN;
+    // tile + request numbers the overlapping (tile, request) pairs; request q of unit u is the
+    // first that ends behind tile u - q's start
+    int64_t lo = 0, hi = p.Q;
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (p.offsets[mid + 1] + kBM * mid > kBM * u)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    if (lo >= p.Q) return false;
+    w.m = u - lo;
+    if (w.m < 0 || w.m >= g.m_tiles) return false;
+    w.row0 = max(p.offsets[lo], w.m * kBM);
+    w.row1 = min(min(p.offsets[lo + 1], (w.m + 1) * kBM), p.T);
+    w.e = adapter_of(p, lo);
+    w.e_rank = rank_of(p, w.e);
+    if (w.row0 >= w.row1 || w.r0 >= w.e_rank) return false;
+    w.cols = min(kBN, (w.e_rank - w.r0 + 15) / 16 * 16);
+  } else {
+    w.m = unit % g.m_tiles;
+    w.n0 = unit / g.m_tiles * kBN;
+    w.cols = kBN;
+  }
+  w.t0 = w.m * kBM;
+  return true;
+}
+
+// f(adapter, rank, first row, end row) for the requests with an adapter that reach into row tile
+// m, in order; a warp together, every lane with the same arguments.  f returns false to stop.
+template <typename F>
+__device__ __forceinline__ bool for_requests(const Problem& p, int64_t m, F&& f) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t0 = m * kBM, t1 = min(t0 + kBM, p.T);
+  for (int64_t base = p.tile_q[m]; base < p.Q; base += 32) {
+    const int64_t q = base + lane;
+    int a = 0, b = 0, e = kNone, r = 0;
+    bool past = true;
+    if (q < p.Q) {
+      const int64_t o0 = p.offsets[q], o1 = p.offsets[q + 1];
+      past = o0 >= t1;
+      a = (int)(max(o0, t0) - t0);
+      b = (int)(max(min(o1, t1), t0) - t0);
+      if (!past && a < b) {
+        e = adapter_of(p, q);
+        r = rank_of(p, e);
+      }
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, r > 0); todo; todo &= todo - 1) {
+      const int i = __ffs(todo) - 1;
+      if (!f(__shfl_sync(0xffffffffu, e, i), __shfl_sync(0xffffffffu, r, i), __shfl_sync(0xffffffffu, a, i),
+             __shfl_sync(0xffffffffu, b, i)))
+        return false;
+    }
+    if (__any_sync(0xffffffffu, past)) break;
+  }
+  return true;
+}
+
+struct Bars {
+  uint64_t full[kStages], empty[kStages], acc_full[kBufs], acc_empty[kBufs], done;
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrain) : "memory"); }
+
+template <int kBN>
+struct Chunks {  // one step's operand chunks of a loading thread
+  uint4 x[kBM * 8 / kLoad], b[kBN * 8 / kLoad];
+};
+
+template <bool kSub, bool kShrink, int kBN>
+__global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, const Tiling g) {
+  constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128, kStageBytes = 2 * (kABytes + kBBytes);
+  constexpr int kLd = kBN + 4;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ Bars bars;
+  __shared__ int row_e[kShrink ? 1 : kBM];  // each row's adapter, kMixed for a row of no request
+  __shared__ int gave_up;                   // a draining warp's wait did: all of them stop at the same tile
+  uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  const uint32_t sbase = smem_u32(smem);
+  float* part = (float*)(smem + kStages * kStageBytes);  // the tile, [kBM][kLd]
+  cg::cluster_group cl = cg::this_cluster();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = g.split, rank = split > 1 ? (int)cl.block_rank() : 0;
+  const int64_t cluster = blockIdx.x / split;
+  if constexpr (kShrink) {
+    launch_dependents();
+    if (cluster >= g.clusters) {
+      const int64_t tile = ((cluster - g.clusters) * split + rank) * (kThreads / 32) + warp;
+      if (tile < g.m_tiles) plan_tile(p, tile, 1);
+      return;
+    }
+  }
+  if (warp == kMmaWarp) tmem_alloc(&bars.tmem, kBufs * kBN);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&bars.full[i], kLoad);
+      mbar_init(&bars.empty[i], 1);
+    }
+    for (int i = 0; i < kBufs; ++i) {
+      mbar_init(&bars.acc_full[i], 1);
+      mbar_init(&bars.acc_empty[i], kDrain / 32);
+    }
+    mbar_init(&bars.done, 1);
+    fence_mbar_init();
+    gave_up = 0;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bars.tmem;
+  int* err = &g_err;
+  const int n_k = (int)((p.K + kStep - 1) / kStep);
+  const int kb = (int)((int64_t)n_k * rank / split), ke = (int)((int64_t)n_k * (rank + 1) / split);
+  // the requests' low-rank parts as chunks
+  const bool lowrank = !kShrink && p.R > 0 && !g.rowwise && rank == 0;
+  bool waited = !g.dependent;
+  bool ok = true;
+  Tile w = {};
+
+  if (warp >= 8 && warp < kMmaWarp) {
+    // ---------------------------------------------------------------- loads
+    const int tid = threadIdx.x - kDrain, chunk = tid & 7, prow = tid >> 3;
+    int it = 0;
+    auto fetch_x = [&](uint4(&d)[kBM * 8 / kLoad], const float* x, int64_t rs, int64_t t0, int64_t k, int64_t n_kk,
+                       bool vec) {
+#pragma unroll
+      for (int j = 0; j < kBM * 8 / kLoad; ++j) {
+        const int64_t t = t0 + prow + j * (kLoad / 8);
+        d[j] = t < p.T ? load16<float>(x + t * rs, k + chunk * 4, n_kk, vec) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto fetch_b = [&](uint4(&d)[kBN * 8 / kLoad], const float* B, int64_t ks, int64_t ns, int64_t c0, int64_t n_c,
+                       int64_t k0, int64_t n_kk, bool vec) {
+#pragma unroll
+      for (int j = 0; j < kBN * 8 / kLoad; ++j) {
+        if constexpr (kSub) {  // columns contiguous: consecutive threads, consecutive columns
+          const int task = j * kLoad + tid;
+          const int64_t c = c0 + task % kBN, k = k0 + task / kBN * 4;
+          float f[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = c < n_c && k + i < n_kk ? B[(k + i) * ks + c * ns] : 0.0f;
+          d[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
+                            __float_as_uint(f[3]));
+        } else {
+          const int64_t c = c0 + prow + j * (kLoad / 8);
+          d[j] = c < n_c ? load16<float>(B + c * ns, k0 + chunk * 4, n_kk, vec) : make_uint4(0, 0, 0, 0);
+        }
+      }
+    };
+    auto fetch = [&](Chunks<kBN>& d, int k) {
+      fetch_x(d.x, (const float*)p.x, p.x_rs, w.t0, (int64_t)k * kStep, p.K, p.x_vec);
+      if constexpr (kShrink)
+        fetch_b(d.b, (const float*)p.P + w.e * p.p_es, p.p_ks, p.p_rs, w.r0, w.e_rank, (int64_t)k * kStep, p.K,
+                p.p_vec);
+      else
+        fetch_b(d.b, (const float*)p.M, p.m_ks, p.m_ns, w.n0, p.N, (int64_t)k * kStep, p.K, p.m_vec);
+    };
+    auto store = [&](const Chunks<kBN>& d) -> bool {
+      const int s = it % kStages, round = it / kStages;
+      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 51)) return false;
+      const uint32_t a = sbase + s * kStageBytes, b = a + 2 * kABytes;
+#pragma unroll
+      for (int j = 0; j < kBM * 8 / kLoad; ++j) put<float>(a, kABytes, prow + j * (kLoad / 8), chunk, d.x[j]);
+#pragma unroll
+      for (int j = 0; j < kBN * 8 / kLoad; ++j) {
+        if constexpr (kSub) {
+          const int task = j * kLoad + tid;
+          put<float>(b, kBBytes, task % kBN, task / kBN, d.b[j]);
+        } else {
+          put<float>(b, kBBytes, prow + j * (kLoad / 8), chunk, d.b[j]);
+        }
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(&bars.full[s]);
+      ++it;
+      return true;
+    };
+    for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
+      if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
+      Chunks<kBN> one, two;
+      if (kb < ke) fetch(one, kb);
+      for (int k = kb; k < ke && ok; k += 2) {
+        if (k + 1 < ke) fetch(two, k + 1);
+        ok = store(one);
+        if (!ok || k + 1 >= ke) break;
+        if (k + 2 < ke) fetch(one, k + 2);
+        ok = store(two);
+      }
+      if (lowrank && ok) {
+        if (!waited) dependency_wait();
+        waited = true;
+        ok = for_requests(p, w.m, [&](int e, int r, int, int) {
+          for (int r0 = 0; r0 < r; r0 += kStep) {
+            // rows of v are 16-byte aligned, v_rs a multiple of 8; beyond the rank: zeros
+            fetch_x(one.x, p.v, p.v_rs, w.t0, r0, r, true);
+            fetch_b(one.b, (const float*)p.Qm + e * p.q_es, p.q_rs, p.q_ns, w.n0, p.N, r0, r, p.q_vec);
+            if (!store(one)) return false;
+          }
+          return true;
+        });
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    // ---------------------------------------------------------------- MMAs
+    int it = 0, ch = 0;
+    // one step into chunk ch; first / last of its chunk
+    auto step = [&](int mmas, bool first, bool last, uint32_t id) -> bool {
+      const int s = it % kStages, buf = ch % kBufs;
+      if (first && !mbar_wait(&bars.acc_empty[buf], ((ch / kBufs) & 1) ^ 1, err, 61)) return false;
+      if (!mbar_wait(&bars.full[s], (it / kStages) & 1, err, 62)) return false;
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t a = sbase + s * kStageBytes, d = tmem + buf * kBN;
+        const uint64_t ad = sw128_desc(a), bd = sw128_desc(a + 2 * kABytes);
+        constexpr uint64_t kALo = kABytes >> 4, kBLo = kBBytes >> 4;
+        for (int j = 0; j < mmas; ++j) {
+          mma_tf32(d, ad + kALo + 2 * j, bd + 2 * j, id, !first || j > 0);  // the small terms first
+          mma_tf32(d, ad + 2 * j, bd + kBLo + 2 * j, id, 1);
+          mma_tf32(d, ad + 2 * j, bd + 2 * j, id, 1);
+        }
+        mma_commit(&bars.empty[s]);
+        if (last) mma_commit(&bars.acc_full[buf]);
+      }
+      __syncwarp();
+      ++it;
+      ch += last;
+      return true;
+    };
+    for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
+      if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
+      const uint32_t id = idesc(Kind<float>::kAb, w.cols, false);
+      for (int k = kb; k < ke && ok; ++k)
+        ok = step(4, (k - kb) % kChunk == 0, (k - kb) % kChunk == kChunk - 1 || k + 1 == ke, id);
+      if (lowrank && ok) {
+        if (!waited) dependency_wait();
+        waited = true;
+        ok = for_requests(p, w.m, [&](int, int r, int, int) {
+          for (int r0 = 0; r0 < r; r0 += kStep)
+            if (!step((min(r - r0, kStep) + 7) / 8, true, true, id)) return false;
+          return true;
+        });
+      }
+    }
+    if (lane == 0) mma_commit(&bars.done);
+    mbar_wait_drain(&bars.done, 0, err, 63);  // every MMA has run before tensor memory is given up
+  } else if (warp < 8) {
+    // ---------------------------------------------------------------- chunks, tiles
+    const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (kBN / 2);
+    const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
+    int ch = 0;
+    for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
+      if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
+      const int rows = (int)min((int64_t)kBM, p.T - w.t0);
+      if constexpr (!kShrink) {
+        if (threadIdx.x < rows) {
+          const int64_t q = request_of(p, w.t0 + threadIdx.x);
+          row_e[threadIdx.x] = q < 0 ? kMixed : adapter_of(p, q);
+        }
+      }
+      float acc[kBN / 2];
+#pragma unroll
+      for (int i = 0; i < kBN / 2; ++i) acc[i] = 0.0f;
+      auto drain = [&](bool mine) -> bool {
+        const int buf = ch % kBufs;
+        if (!mbar_wait(&bars.acc_full[buf], (ch / kBufs) & 1, err, 71)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < kBN / 2; c += 16) {
+          if (kShrink && c0 + c >= w.cols) break;
+          float v[16];
+          tmem_ld16(src + buf * kBN + c, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[c + i] = mine ? acc[c + i] + v[i] : acc[c + i];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.acc_empty[buf]);
+        ++ch;
+        return true;
+      };
+      for (int k = kb; k < ke && ok; k += kChunk) ok = drain(true);
+      if (!kShrink && p.R > 0 && !waited) {
+        dependency_wait();
+        waited = true;
+      }
+      if (lowrank && ok)
+        ok = for_requests(p, w.m, [&](int, int r, int a, int b) {
+          for (int r0 = 0; r0 < r; r0 += kStep)
+            if (!drain(row >= a && row < b)) return false;
+          return true;
+        });
+#pragma unroll
+      for (int i = 0; i < kBN / 2; i += 4)
+        *(float4*)(part + row * kLd + c0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+      if (split > 1) break;  // one tile: the cluster's parts are summed below
+      if (!ok) *(volatile int*)&gave_up = 1;
+      drain_sync();
+      ok = *(volatile int*)&gave_up == 0;
+      if constexpr (kShrink) {
+        const int a = (int)(w.row0 - w.t0), b = (int)(w.row1 - w.t0), quads = w.cols / 4;
+        const float scale = p.scale[w.e];
+        for (int i = threadIdx.x; i < (b - a) * quads; i += kDrain) {
+          const int r = a + i / quads, c = i % quads * 4;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (w.r0 + c + j < w.e_rank) store_v(p, w.t0 + r, w.r0 + c + j, scale * part[r * kLd + c + j]);
+        }
+      } else {
+        const int64_t n = w.n0 + lane * 4;
+        float bias[4] = {};
+        if (p.bias)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < p.N) bias[i] = ((const float*)p.bias)[n + i];
+        if (n < p.N) {
+#pragma unroll 4
+          for (int r = warp; r < rows; r += 8) {
+            const int re = row_e[r];
+            if (re == kMixed) continue;
+            const float4 s = *(const float4*)(part + r * kLd + lane * 4);
+            float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
+            if (g.rowwise) add_lowrank<float, kSub>(p, w.t0 + r, re, rank_of(p, re), n, a);
+            store4<float>(p, w.t0 + r, n, a);
+          }
+        }
+      }
+      drain_sync();  // before the next tile is staged
+    }
+  }
+  __syncwarp();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_relinquish();
+    tmem_dealloc(tmem, kBufs * kBN);
+  }
+  if (split == 1) return;
+
+  // ---- the parts of the cluster's one tile
+  cl.sync();
+  if (warp < 8 && tile_of<kShrink, kBN>(p, g, cluster, w)) {
+    auto sum4 = [&](int row, int c) -> float4 {
+      float4 s = *(const float4*)(cl.map_shared_rank(part, 0) + row * kLd + c);
+      for (int i = 1; i < split; ++i) {
+        const float4 q = *(const float4*)(cl.map_shared_rank(part, i) + row * kLd + c);
+        s.x += q.x, s.y += q.y, s.z += q.z, s.w += q.w;
+      }
+      return s;
+    };
+    if constexpr (kShrink) {
+      const int a = (int)(w.row0 - w.t0), b = (int)(w.row1 - w.t0), quads = w.cols / 4;
+      const float scale = p.scale[w.e];
+      for (int i = rank * kDrain + threadIdx.x; i < (b - a) * quads; i += split * kDrain) {
+        const int r = a + i / quads, c = i % quads * 4;
+        const float4 s = sum4(r, c);
+        const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (w.r0 + c + j < w.e_rank) store_v(p, w.t0 + r, w.r0 + c + j, scale * v[j]);
+      }
+    } else {
+      const int rows = (int)min((int64_t)kBM, p.T - w.t0);
+      const int64_t n = w.n0 + lane * 4;
+      float bias[4] = {};
+      if (p.bias)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (n + i < p.N) bias[i] = ((const float*)p.bias)[n + i];
+      for (int r = rank + warp * split; r < rows; r += 8 * split) {
+        const int re = row_e[r];
+        if (re == kMixed || n >= p.N) continue;
+        const float4 s = sum4(r, lane * 4);
+        float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
+        if (g.rowwise) add_lowrank<float, kSub>(p, w.t0 + r, re, rank_of(p, re), n, a);
+        store4<float>(p, w.t0 + r, n, a);
+      }
+    }
+  }
+  __syncwarp();
+  cl.sync();  // nobody leaves while its part is read
+}
+
+template <bool kSub, bool kShrink, int kBN>
+cf_status launch(const Problem& p, Tiling g, cudaStream_t st) {
+  constexpr int smem = kStages * 2 * (kBM + kBN) * 128 + kBM * (kBN + 4) * 4 + 1024;
+  auto* kern = k_adapter_f32<kSub, kShrink, kBN>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "k_adapter_f32: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  g.split = split_for(kShrink ? g.m_tiles : g.units, ceil_div(p.K, kStep));
+  // one CTA an SM walks over the tiles; a cluster has one
+  g.clusters = g.split > 1 ? g.units : (g.units < 148 ? g.units : 148);
+  const int64_t plans = kShrink ? ceil_div(g.m_tiles, (int64_t)g.split * (kThreads / 32)) : 0;
+  const int64_t blocks = (g.clusters + plans) * g.split;
+  CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "k_adapter_f32: too many tiles");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)g.split;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = g.dependent ? 2 : 1;
+  e = cudaLaunchKernelEx(&cfg, kern, p, g);
+  if (e != cudaSuccess) {
+    set_error("k_adapter_f32: %s", cudaGetErrorString(e));
+    return CF_ERR_CUDA;
+  }
+  return check_launch("k_adapter_f32");
+}
+
+template <bool kSub>
+cf_status run(const Problem& p, bool row_shrink, cudaStream_t st) {
+  Tiling g = {};
+  g.m_tiles = ceil_div(p.T, kBM);
+  g.rowwise = row_shrink && p.R > 0;
+  if (p.R > 0 && row_shrink) {
+    CF_TRY(launch_row_shrink(p, CF_F32, kSub, 1, st));
+  } else if (p.R > 0) {
+    const int bn = p.R <= 64 ? 64 : 128;
+    g.units = (g.m_tiles + p.Q - 1) * ceil_div(p.R, bn);
+    CF_TRY(bn == 64 ? (launch<kSub, true, 64>(p, g, st)) : (launch<kSub, true, 128>(p, g, st)));
+  }
+  g.dependent = p.R > 0;
+  g.units = g.m_tiles * ceil_div(p.N, 128);
+  return launch<kSub, false, 128>(p, g, st);
+}
+
+}  // namespace
+
+cf_status launch_f32(const Problem& p, bool substitute, bool row_shrink, cudaStream_t st) {
+  return substitute ? run<true>(p, row_shrink, st) : run<false>(p, row_shrink, st);
+}
+
+cf_status take_site_f32(int* site, cudaStream_t st) { return take_site(&g_err, site, st); }
+
+}  // namespace adapter
+}  // namespace cf

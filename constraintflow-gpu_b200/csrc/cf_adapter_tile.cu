@@ -13,13 +13,11 @@
 // Operands in shared memory are 128-byte-swizzled images, 128 bytes of the contraction a row:
 //   TMA:    16-bit data by tensor maps; M and Q_e with n contiguous (substitution) stay as they
 //           lie, as MN-major images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
-//   loads:  any stride and alignment, and float32, by the epilogue's warps; float32 is split into
-//           tf32 hi + lo planes (3xTF32: hi*hi + hi*lo + lo*hi).
+//   loads:  any stride and alignment, by the epilogue's warps.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
-#include "cf_adapter.cuh"
-#include "cf_tc.cuh"
+#include "cf_adapter_dev.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -54,33 +52,12 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_
       : "memory");
 }
 
-// Instruction descriptor: float32 accumulator, A and B of type ab (0 f16, 1 bf16, 2 tf32), A
-// K-major, B K-major or (bit 16) MN-major, 128 x n.
-__device__ __forceinline__ uint32_t idesc(uint32_t ab, uint32_t n, bool mn_major) {
-  return (1u << 4) | (ab << 7) | (ab << 10) | ((uint32_t)mn_major << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24);
-}
-
 // MN-major, 128-byte swizzle: 64 columns (128 B) x 8 contraction steps an atom; groups of 8 steps
 // 1024 B apart, blocks of 64 columns 64 steps x 128 B = 8192 B apart.
 __device__ __forceinline__ uint64_t mn_desc(uint32_t smem_addr) {
   return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-
-template <typename T>
-struct Kind;  // of a type: elements in 128 bytes, planes of an operand, descriptor type
-template <>
-struct Kind<float> {
-  static constexpr int kStep = 32, kPlanes = 2, kAb = 2;
-};
-template <>
-struct Kind<__nv_bfloat16> {
-  static constexpr int kStep = 64, kPlanes = 1, kAb = 1;
-};
-template <>
-struct Kind<__half> {
-  static constexpr int kStep = 64, kPlanes = 1, kAb = 0;
-};
 
 struct Maps {
   CUtensorMap x, b, v_hi, v_lo, q;
@@ -101,115 +78,17 @@ struct Bars {
   uint32_t tmem;
 };
 
-// 16 bytes of row `row` (elements k .. of n_k), zero beyond
-template <typename T>
-__device__ __forceinline__ uint4 load16(const T* row, int64_t k, int64_t n_k, bool vec) {
-  constexpr int E = 16 / sizeof(T);
-  if (vec && k + E <= n_k) return *(const uint4*)(row + k);
-  alignas(16) T t[E];
-#pragma unroll
-  for (int i = 0; i < E; ++i) t[i] = k + i < n_k ? row[k + i] : from_f32<T>(0.0f);
-  return *(const uint4*)t;
-}
-
-// a 16-byte chunk of one operand row into its plane(s)
-template <typename T>
-__device__ __forceinline__ void put(uint32_t plane, uint32_t plane_bytes, uint32_t row, uint32_t chunk, uint4 d) {
-  const uint32_t at = plane + row * 128u + ((chunk ^ (row & 7u)) << 4);
-  if constexpr (Kind<T>::kPlanes == 2) {
-    float hi[4], lo[4];
-    split_tf32(__uint_as_float(d.x), hi[0], lo[0]);
-    split_tf32(__uint_as_float(d.y), hi[1], lo[1]);
-    split_tf32(__uint_as_float(d.z), hi[2], lo[2]);
-    split_tf32(__uint_as_float(d.w), hi[3], lo[3]);
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(hi[0]), "f"(hi[1]), "f"(hi[2]), "f"(hi[3])
-                 : "memory");
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + plane_bytes), "f"(lo[0]), "f"(lo[1]),
-                 "f"(lo[2]), "f"(lo[3])
-                 : "memory");
-  } else {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(d.x), "r"(d.y), "r"(d.z), "r"(d.w)
-                 : "memory");
-  }
-}
-
-// y columns n .. n+3 of row t
-template <typename T>
-__device__ __forceinline__ void store4(const Problem& p, int64_t t, int64_t n, const float (&a)[4]) {
-  T* y = (T*)p.y + t * p.y_rs + n;
-  if (p.y_vec && n + 4 <= p.N) {
-    alignas(16) T o[4] = {from_f32<T>(a[0]), from_f32<T>(a[1]), from_f32<T>(a[2]), from_f32<T>(a[3])};
-    if constexpr (sizeof(T) == 4)
-      *(uint4*)y = *(const uint4*)o;
-    else
-      *(uint2*)y = *(const uint2*)o;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < p.N) y[i] = from_f32<T>(a[i]);
-  }
-}
-
-// a += v[t] Q_e at columns n .. n+3 (columns beyond N are not read)
-template <typename T, bool kSub>
-__device__ __forceinline__ void add_lowrank(const Problem& p, int64_t t, int e, int rank, int64_t n, float (&a)[4]) {
-  const float* v = p.v + t * p.v_rs;
-  const T* Q = (const T*)p.Qm + e * p.q_es;
-  if constexpr (kSub) {  // rows of n
-    const bool full = n + 4 <= p.N;
-#pragma unroll 4
-    for (int r = 0; r < rank; ++r) {
-      const T* q = Q + r * p.q_rs + n;
-      const float w = v[r];
-      if (full && p.q_vec) {
-        alignas(16) T d[4];
-        if constexpr (sizeof(T) == 4)
-          *(uint4*)d = *(const uint4*)q;
-        else
-          *(uint2*)d = *(const uint2*)q;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = fmaf(w, to_f32(d[i]), a[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (n + i < p.N) a[i] = fmaf(w, to_f32(q[i]), a[i]);
-      }
-    }
-  } else {  // rows of r
-    constexpr int E = 16 / sizeof(T);
-    int r = 0;
-    if (p.q_vec) {
-      for (; r + E <= rank; r += E) {
-        float w[E];
-#pragma unroll
-        for (int i = 0; i < E; ++i) w[i] = v[r + i];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (n + c >= p.N) break;
-          alignas(16) T d[E];
-          *(uint4*)d = *(const uint4*)(Q + (n + c) * p.q_ns + r);
-#pragma unroll
-          for (int i = 0; i < E; ++i) a[c] = fmaf(w[i], to_f32(d[i]), a[c]);
-        }
-      }
-    }
-    for (; r < rank; ++r)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (n + c < p.N) a[c] = fmaf(v[r], to_f32(Q[(n + c) * p.q_ns + r]), a[c]);
-  }
-}
-
 template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
-__global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_adapter_tile(const Problem p, const __grid_constant__ Maps maps,
+__global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, const __grid_constant__ Maps maps,
                                                            const Tiling g) {
-  constexpr int kStep = Kind<T>::kStep, kPlanes = Kind<T>::kPlanes;
+  constexpr int kStep = Kind<T>::kStep;
   constexpr bool kMn = kTma && kSub;  // B images lie n-contiguous
   constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128;
-  constexpr uint32_t kStageBytes = (kABytes + kBBytes) * kPlanes;
+  constexpr uint32_t kStageBytes = kABytes + kBBytes;
   static_assert((kBM * (kBN + 4)) * 4 <= kStageBytes * kStages, "the tile is staged where the operands were");
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars<kStages> bars;
+  __shared__ int row_e[kShrink ? 1 : kBM];  // each row's adapter, kMixed for a row of no request
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
   cg::cluster_group cl = cg::this_cluster();
@@ -286,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_ada
     if (te < 0) return 0;
     tr = rank_of(p, te);
     const int steps = (tr + kStep - 1) / kStep;
-    return kTma ? 2 * steps : steps;
+    return 2 * steps;
   };
 
   bool ok = true;
@@ -343,19 +222,12 @@ __global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_ada
       const int s = it % kStages, round = it / kStages;
       if (!mbar_wait(&bars.full[s], round & 1, err, 21)) return false;
       tc_fence_after();
-      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes * kPlanes;
+      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
       const uint64_t ad = sw128_desc(a), bd = kMn ? mn_desc(b) : sw128_desc(b);
       constexpr uint64_t kAStep = 32 >> 4, kBStep = kMn ? (16 * 128) >> 4 : 32 >> 4;
       for (int j = 0; j < k16; ++j) {
         const uint32_t acc = it > 0 || j > 0;
-        if constexpr (kPlanes == 2) {
-          constexpr uint64_t kALo = kABytes >> 4, kBLo = kBBytes >> 4;
-          mma_tf32(tmem, ad + j * kAStep, bd + j * kBStep, id, acc);
-          mma_tf32(tmem, ad + j * kAStep, bd + kBLo + j * kBStep, id, 1);
-          mma_tf32(tmem, ad + kALo + j * kAStep, bd + j * kBStep, id, 1);
-        } else {
-          mma_f16(tmem, ad + j * kAStep, bd + j * kBStep, id, acc);
-        }
+        mma_f16(tmem, ad + j * kAStep, bd + j * kBStep, id, acc);
       }
       mma_commit(&bars.empty[s]);
       ++it;
@@ -366,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_ada
       const int extra = ok ? lowrank_steps(te, tr) : 0;
       constexpr int kMma = kStep / 4;  // contraction of one MMA
       for (int i = 0; i < extra && ok; ++i) {
-        const int r = (kTma ? i / 2 : i) * kStep;
+        const int r = i / 2 * kStep;
         ok = step((min(tr - r, kStep) + kMma - 1) / kMma);
       }
     }
@@ -399,11 +271,11 @@ __global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_ada
         }
       }
     };
-    int it = 0, te = kNone, tr = 0;
+    int it = 0;
     auto put_step = [&]() -> bool {
       const int s = it % kStages, round = it / kStages;
       if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 31)) return false;
-      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes * kPlanes;
+      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
 #pragma unroll
       for (int j = 0; j < kXTasks; ++j) put<T>(a, kABytes, prow + j * (kWorkers / 8), chunk, xr[j]);
 #pragma unroll
@@ -438,25 +310,17 @@ __global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_ada
       ok = put_step();
       if (k + 1 < ke) fetch(k + 1);
     }
-    if constexpr (!kShrink && kPlanes == 2) {
-      const int extra = ok ? lowrank_steps(te, tr) : 0;
-      for (int i = 0; i < extra && ok; ++i) {
-        const int64_t r = (int64_t)i * kStep;
-#pragma unroll
-        for (int j = 0; j < kXTasks; ++j) {
-          const int64_t t = t0 + prow + j * (kWorkers / 8);
-          // rows of v are 16-byte aligned, v_rs a multiple of 8; beyond the rank: zeros
-          xr[j] = t < p.T ? load16<T>((const T*)(p.v + t * p.v_rs), r + chunk * E, tr, true)
-                          : make_uint4(0, 0, 0, 0);
-        }
-        fetch_b((const T*)p.Qm + te * p.q_es, p.q_rs, p.q_ns, n0, p.N, r, tr, p.q_vec);
-        ok = put_step();
-      }
-    }
   }
 
   // ---- the accumulators, staged in shared memory
   __syncwarp();
+  if constexpr (!kShrink) {
+    if (kTma ? warp < 4 : warp == kProducerWarp)
+      for (int i = kTma ? threadIdx.x : lane; i < rows; i += kTma ? kBM : 32) {
+        const int64_t q = request_of(p, t0 + i);
+        row_e[i] = q < 0 ? kMixed : adapter_of(p, q);
+      }
+  }
   float* part = (float*)smem;
   constexpr int kLd = kBN + 4;
   int te = kNone;
@@ -519,78 +383,17 @@ __global__ void __launch_bounds__(kThreads, Kind<T>::kPlanes == 1 ? 2 : 1) k_ada
           if (n + i < p.N) bias[i] = to_f32(((const T*)p.bias)[n + i]);
       for (int row = rank + warp * split; row < rows; row += 8 * split) {
         const int64_t t = t0 + row;
-        const int64_t q = request_of(p, t);
-        if (q < 0 || n >= p.N || lane * 4 >= kBN) continue;
+        const int re = row_e[row];
+        if (re == kMixed || n >= p.N) continue;
         const float4 s = sum4(row, lane * 4);
         float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
-        if (te == kMixed || (te >= 0 && !g.q_tma)) {
-          const int re = adapter_of(p, q);
-          add_lowrank<T, kSub>(p, t, re, rank_of(p, re), n, a);
-        }
+        if (te == kMixed) add_lowrank<T, kSub>(p, t, re, rank_of(p, re), n, a);
         store4<T>(p, t, n, a);
       }
     }
   }
   __syncwarp();
   if (split > 1) cl.sync();  // nobody leaves while its part is read
-}
-
-// v for rows whose requests are short (a tile of the tensor cores would hold few rows of each):
-// one CTA per row and kRows columns of v.  Behind the rows, CTAs that plan row tiles.
-constexpr int kRowThreads = 256;
-template <bool kSub>
-constexpr int kRowCols = kSub ? 16 : kRowThreads / 32;
-
-template <typename T, bool kSub>
-__global__ void __launch_bounds__(kRowThreads) k_adapter_shrink_rows(const Problem p, int64_t m_tiles, int whole) {
-  launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t t = blockIdx.x;
-  if (t >= p.T) {
-    const int64_t tile = (t - p.T) * (kRowThreads / 32) + warp;
-    if (blockIdx.y == 0 && tile < m_tiles) plan_tile(p, tile, whole);
-    return;
-  }
-  const int e = adapter_of(p, request_of(p, t)), rank = rank_of(p, e);
-  const int r0 = blockIdx.y * kRowCols<kSub>;
-  if (r0 >= rank) return;
-  const T* x = (const T*)p.x + t * p.x_rs;
-  const T* P = (const T*)p.P + e * p.p_es;
-  if constexpr (kSub) {  // rows of r: 16 columns x 16 steps of k at a time
-    __shared__ float sums[kRowThreads / 32][16];
-    const int r = r0 + (threadIdx.x & 15);
-    float acc = 0.0f;
-    if (r < rank) {
-#pragma unroll 8
-      for (int64_t k = threadIdx.x >> 4; k < p.K; k += kRowThreads / 16)
-        acc = fmaf(to_f32(x[k]), to_f32(P[k * p.p_ks + r]), acc);
-    }
-    acc += __shfl_xor_sync(0xffffffffu, acc, 16);
-    if (lane < 16) sums[warp][lane] = acc;
-    __syncthreads();
-    if (threadIdx.x < 16 && r < rank) {
-      float v = 0.0f;
-      for (int i = 0; i < kRowThreads / 32; ++i) v += sums[i][threadIdx.x];
-      store_v(p, t, r, p.scale[e] * v);
-    }
-  } else {  // rows of k: a warp a column
-    constexpr int E = 16 / sizeof(T);
-    const int r = r0 + warp;
-    if (r >= rank) return;
-    P += r * p.p_rs;
-    float acc = 0.0f;
-#pragma unroll 4
-    for (int64_t k = lane * E; k < p.K; k += 32 * E) {
-      alignas(16) T a[E], b[E];
-      *(uint4*)a = load16<T>(x, k, p.K, p.x_vec);
-      *(uint4*)b = load16<T>(P, k, p.K, p.p_vec);
-#pragma unroll
-      for (int i = 0; i < E; ++i) acc = fmaf(to_f32(a[i]), to_f32(b[i]), acc);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
-    if (lane == 0) store_v(p, t, r, p.scale[e] * acc);
-  }
 }
 
 typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -626,7 +429,7 @@ cf_status encode(CUtensorMap* map, int dtype, const void* base, int64_t nx, int6
 template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
 cf_status launch(const char* what, const Problem& p, const Maps& maps, const Tiling& g, int64_t clusters,
                  cudaStream_t st) {
-  constexpr int smem = (kBM + kBN) * 128 * Kind<T>::kPlanes * kStages + 1024;
+  constexpr int smem = (kBM + kBN) * 128 * kStages + 1024;
   auto* kern = k_adapter_tile<T, kSub, kShrink, kTma, kBN, kStages>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
@@ -653,14 +456,6 @@ cf_status launch(const char* what, const Problem& p, const Maps& maps, const Til
   return check_launch(what);
 }
 
-// CTAs of a cluster: as many as keep the grid within two waves of single CTAs, each with at
-// least four steps of the contraction.
-int split_for(int64_t tiles, int64_t steps) {
-  int s = 1;
-  while (s < 8 && tiles * s * 2 <= 2 * 148 && steps >= s * 2 * 4) s *= 2;
-  return s;
-}
-
 template <typename T, bool kSub, bool kTma>
 cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cudaStream_t st) {
   constexpr int kStep = Kind<T>::kStep, kStages = 3;
@@ -669,18 +464,13 @@ cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cu
   Tiling g = {};
   g.m_tiles = m_tiles;
   g.x_rows = (int)(p.T < kBM ? ceil_div(p.T, 8) * 8 : kBM);
-  constexpr bool f32 = Kind<T>::kPlanes == 2;
   // float16's range does not hold every intermediate that float32 does: row by row instead
   const bool pair = kTma && dtype == CF_BF16 && lowrank_tma;
-  g.q_tma = pair || (f32 && !kTma);
-  g.whole = pair ? 16 : f32 ? 1 : 0;
+  g.q_tma = pair;
+  g.whole = pair ? 16 : 0;
   if (kTma) CF_TRY(encode(&maps.x, dtype, p.x, p.K, p.T, 1, p.x_rs, p.x_rs * p.T, g.x_rows));
   if (p.R > 0 && row_shrink) {
-    const int64_t blocks = p.T + ceil_div(m_tiles, kRowThreads / 32);
-    CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "adapter_matmul: too many rows");
-    const dim3 grid((unsigned)blocks, (unsigned)ceil_div(p.R, kRowCols<kSub>));
-    k_adapter_shrink_rows<T, kSub><<<grid, kRowThreads, 0, st>>>(p, m_tiles, g.whole);
-    CF_TRY(check_launch("k_adapter_shrink_rows"));
+    CF_TRY(launch_row_shrink(p, dtype, kSub, g.whole, st));
   } else if (p.R > 0) {
     const int bn = p.R <= 64 ? 64 : 128;
     const bool by_tma = kTma && lowrank_tma;
@@ -727,9 +517,6 @@ cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cu
 
 cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool tma, bool row_shrink, bool lowrank_tma,
                        cudaStream_t st) {
-  if (dtype == CF_F32)
-    return substitute ? run<float, true, false>(p, dtype, row_shrink, lowrank_tma, st)
-                      : run<float, false, false>(p, dtype, row_shrink, lowrank_tma, st);
   if (dtype == CF_BF16) {
     if (tma)
       return substitute ? run<__nv_bfloat16, true, true>(p, dtype, row_shrink, lowrank_tma, st)
@@ -744,19 +531,7 @@ cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool tma, b
                     : run<__half, false, false>(p, dtype, row_shrink, lowrank_tma, st);
 }
 
-cf_status check_waits(cudaStream_t st) {
-  int site = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(&site, g_err, sizeof(site), 0, cudaMemcpyDeviceToHost, st);
-  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess && site != 0) {
-    const int zero = 0;
-    e = cudaMemcpyToSymbolAsync(g_err, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, st);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  }
-  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "adapter_check: %s", cudaGetErrorString(e));
-  CF_REQUIRE(site == 0, CF_ERR_TIMEOUT, "adapter_matmul: a bounded wait gave up (site %d)", site);
-  return CF_OK;
-}
+cf_status take_site_tiles(int* site, cudaStream_t st) { return take_site(&g_err, site, st); }
 
 }  // namespace adapter
 }  // namespace cf
