@@ -128,10 +128,11 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
 
 extern "C" cf_status cf_adapter_check(void* stream) {
   clear_error();
-  int site = 0, site_f32 = 0;
-  CF_TRY(take_site_tiles(&site, as_stream(stream)));
-  CF_TRY(take_site_f32(&site_f32, as_stream(stream)));
-  CF_REQUIRE(site == 0 && site_f32 == 0, CF_ERR_TIMEOUT, "adapter_matmul: a bounded wait gave up (site %d)",
-             site ? site : site_f32);
+  int tiles = 0, wide = 0, f32 = 0;
+  CF_TRY(take_site_tiles(&tiles, as_stream(stream)));
+  CF_TRY(take_site_wide(&wide, as_stream(stream)));
+  CF_TRY(take_site_f32(&f32, as_stream(stream)));
+  const int site = tiles ? tiles : wide ? wide : f32;
+  CF_REQUIRE(site == 0, CF_ERR_TIMEOUT, "adapter_matmul: a bounded wait gave up (site %d)", site);
   return CF_OK;
 }

@@ -1,5 +1,6 @@
 // The adapter product as its kernels see it (cf_adapter.cu: entry point, checks and
-// workspace; the kernels: cf_adapter_tile.cu, cf_adapter_f32.cu, cf_adapter_rows.cu).
+// workspace; the kernels: cf_adapter_tile.cu,
+// cf_adapter_wide.cu, cf_adapter_f32.cu, cf_adapter_rows.cu).
 #pragma once
 #include "cf_common.cuh"
 #include "cf_elem.cuh"
@@ -11,6 +12,8 @@ constexpr int kBM = 128;  // rows of a tile
 // tile_e: what a tile's rows carry
 constexpr int kNone = -1;   // no adapter
 constexpr int kMixed = -2;  // several, or one that the tensor cores do not add: row by row
+constexpr int kFew = -3;    // several, of at most kFewRequests requests, all of them for the tensor cores
+constexpr int kFewRequests = 8;
 
 // Element (k, n) of M is at M + k*m_ks + n*m_ns; (k, r) of P_e at P + e*p_es + k*p_ks + r*p_rs;
 // (r, n) of Q_e at Qm + e*q_es + r*q_rs + n*q_ns.
@@ -61,41 +64,76 @@ __device__ __forceinline__ int rank_of(const Problem& p, int e) {
   return p.ranks ? min(max(p.ranks[e], 0), p.R) : p.R;
 }
 
+// f(adapter, rank, first row, end row) for the requests with an adapter that reach into row tile
+// m, in order, from request `from` on (the first that ends behind the tile's start); a warp
+// together, every lane with the same arguments.  f returns false to stop.
+template <typename F>
+__device__ __forceinline__ bool for_requests(const Problem& p, int64_t m, int64_t from, F&& f) {
+  const int lane = threadIdx.x & 31;
+  const int64_t t0 = m * kBM, t1 = min(t0 + kBM, p.T);
+  for (int64_t base = from; base < p.Q; base += 32) {
+    const int64_t q = base + lane;
+    int a = 0, b = 0, e = kNone, r = 0;
+    bool past = true;
+    if (q < p.Q) {
+      const int64_t o0 = p.offsets[q], o1 = p.offsets[q + 1];
+      past = o0 >= t1;
+      a = (int)(max(o0, t0) - t0);
+      b = (int)(max(min(o1, t1), t0) - t0);
+      if (!past && a < b) {
+        e = adapter_of(p, q);
+        r = rank_of(p, e);
+      }
+    }
+    for (uint32_t todo = __ballot_sync(0xffffffffu, r > 0); todo; todo &= todo - 1) {
+      const int i = __ffs(todo) - 1;
+      if (!f(__shfl_sync(0xffffffffu, e, i), __shfl_sync(0xffffffffu, r, i), __shfl_sync(0xffffffffu, a, i),
+             __shfl_sync(0xffffffffu, b, i)))
+        return false;
+    }
+    if (__any_sync(0xffffffffu, past)) break;
+  }
+  return true;
+}
+
 // tile_e and tile_q of row tile m, by one warp.  One adapter for all of the tile's rows can be added by the
 // tensor cores: a tile of several would multiply each row with every one of them, and an
 // infinity or NaN of one would reach the others' rows.  `whole`: the ranks that the tensor
 // cores take are R and the multiples of `whole` (0: none), so that nothing beyond an adapter's
 // own rank is multiplied.
 __device__ __forceinline__ void plan_tile(const Problem& p, int64_t m, int whole) {
-  const int lane = threadIdx.x & 31;
-  int lo = INT32_MAX, hi = INT32_MIN;
-  for (int i = lane; i < kBM; i += 32) {
-    const int64_t t = m * kBM + i;
-    const int64_t q = t < p.T ? request_of(p, t) : -1;
-    if (q < 0) continue;
-    int e = adapter_of(p, q);
-    if (rank_of(p, e) == 0) e = kNone;
-    lo = min(lo, e);
-    hi = max(hi, e);
-  }
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  int e = hi < 0 ? kNone : (lo == hi ? lo : kMixed);
-  if (e >= 0) {
-    const int r = rank_of(p, e);
-    if (!(whole > 0 && (r == p.R || r % whole == 0))) e = kMixed;
-  }
-  int64_t a = 0, b = p.Q;  // the first request that ends behind the tile's start
-  while (a < b) {
-    const int64_t mid = (a + b) / 2;
+  int64_t from = 0, b = p.Q;  // the first request that ends behind the tile's start
+  while (from < b) {
+    const int64_t mid = (from + b) / 2;
     if (p.offsets[mid + 1] > m * kBM)
       b = mid;
     else
-      a = mid + 1;
+      from = mid + 1;
   }
-  if (lane == 0) {
+  int first = kNone, requests = 0;
+  int64_t rows = 0;
+  bool one = true, fit = true;
+  for_requests(p, m, from, [&](int e, int r, int a, int b) {
+    if (requests == 0) first = e;
+    one &= e == first;
+    fit &= whole > 0 && (r == p.R || r % whole == 0);
+    rows += b - a;
+    ++requests;
+    return true;
+  });
+  // rows of requests: all of [offsets[0], offsets[Q]) within the tile
+  const int64_t t0 = m * kBM, t1 = min(t0 + kBM, p.T);
+  const int64_t owned = max(min(p.offsets[p.Q], t1) - max(p.offsets[0], t0), (int64_t)0);
+  int e = kMixed;
+  if (requests == 0)
+    e = kNone;
+  else if (fit && one && rows == owned)
+    e = first;
+  else if (fit && requests <= kFewRequests)
+    e = kFew;
+  if ((threadIdx.x & 31) == 0) {
     p.tile_e[m] = e;
-    p.tile_q[m] = (int32_t)a;
+    p.tile_q[m] = (int32_t)from;
   }
 }
 
@@ -121,6 +159,7 @@ cf_status launch_f32(const Problem& p, bool substitute, bool row_shrink, cudaStr
 cf_status launch_row_shrink(const Problem& p, int dtype, bool substitute, int whole, cudaStream_t st);
 // the first site at which a bounded device wait gave up since the last call on this device (0: none)
 cf_status take_site_tiles(int* site, cudaStream_t st);
+cf_status take_site_wide(int* site, cudaStream_t st);
 cf_status take_site_f32(int* site, cudaStream_t st);
 
 }  // namespace adapter

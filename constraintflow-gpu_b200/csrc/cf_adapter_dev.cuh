@@ -127,6 +127,62 @@ __device__ __forceinline__ void add_lowrank(const Problem& p, int64_t t, int e, 
   }
 }
 
+// The same for the 16 columns n .. n+15 of one thread's row.
+template <typename T, bool kSub>
+__device__ __forceinline__ void add_lowrank16(const Problem& p, int64_t t, int e, int rank, int64_t n,
+                                              float (&a)[16]) {
+  const float* v = p.v + t * p.v_rs;
+  const T* Q = (const T*)p.Qm + e * p.q_es;
+  constexpr int E = 16 / sizeof(T);
+  const bool vec = p.q_vec && n + 16 <= p.N;
+  if constexpr (kSub) {
+    if (vec) {
+#pragma unroll 4
+      for (int r = 0; r < rank; ++r) {
+        const T* q = Q + r * p.q_rs + n;
+        const float w = v[r];
+#pragma unroll
+        for (int c = 0; c < 16; c += E) {
+          alignas(16) T d[E];
+          *(uint4*)d = *(const uint4*)(q + c);
+#pragma unroll
+          for (int i = 0; i < E; ++i) a[c + i] = fmaf(w, to_f32(d[i]), a[c + i]);
+        }
+      }
+    } else {
+      for (int r = 0; r < rank; ++r) {
+        const T* q = Q + r * p.q_rs + n;
+        const float w = v[r];
+#pragma unroll
+        for (int c = 0; c < 16; ++c)
+          if (n + c < p.N) a[c] = fmaf(w, to_f32(q[c]), a[c]);
+      }
+    }
+  } else {
+    int r = 0;
+    if (vec) {
+      for (; r + E <= rank; r += E) {
+        float w[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i] = v[r + i];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          alignas(16) T d[E];
+          *(uint4*)d = *(const uint4*)(Q + (n + c) * p.q_ns + r);
+#pragma unroll
+          for (int i = 0; i < E; ++i) a[c] = fmaf(w[i], to_f32(d[i]), a[c]);
+        }
+      }
+    }
+    for (; r < rank; ++r) {
+      const float w = v[r];
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        if (n + c < p.N) a[c] = fmaf(w, to_f32(Q[(n + c) * p.q_ns + r]), a[c]);
+    }
+  }
+}
+
 // Read and clear a kernel file's error word.
 inline cf_status take_site(int* symbol, int* site, cudaStream_t st) {
   void* at = nullptr;

@@ -90,37 +90,6 @@ __device__ __forceinline__ bool tile_of(const Problem& p, const Tiling& g, int64
   return true;
 }
 
-// f(adapter, rank, first row, end row) for the requests with an adapter that reach into row tile
-// m, in order; a warp together, every lane with the same arguments.  f returns false to stop.
-template <typename F>
-__device__ __forceinline__ bool for_requests(const Problem& p, int64_t m, F&& f) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t0 = m * kBM, t1 = min(t0 + kBM, p.T);
-  for (int64_t base = p.tile_q[m]; base < p.Q; base += 32) {
-    const int64_t q = base + lane;
-    int a = 0, b = 0, e = kNone, r = 0;
-    bool past = true;
-    if (q < p.Q) {
-      const int64_t o0 = p.offsets[q], o1 = p.offsets[q + 1];
-      past = o0 >= t1;
-      a = (int)(max(o0, t0) - t0);
-      b = (int)(max(min(o1, t1), t0) - t0);
-      if (!past && a < b) {
-        e = adapter_of(p, q);
-        r = rank_of(p, e);
-      }
-    }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, r > 0); todo; todo &= todo - 1) {
-      const int i = __ffs(todo) - 1;
-      if (!f(__shfl_sync(0xffffffffu, e, i), __shfl_sync(0xffffffffu, r, i), __shfl_sync(0xffffffffu, a, i),
-             __shfl_sync(0xffffffffu, b, i)))
-        return false;
-    }
-    if (__any_sync(0xffffffffu, past)) break;
-  }
-  return true;
-}
-
 struct Bars {
   uint64_t full[kStages], empty[kStages], acc_full[kBufs], acc_empty[kBufs], done;
   uint32_t tmem;
@@ -255,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       if (lowrank && ok) {
         if (!waited) dependency_wait();
         waited = true;
-        ok = for_requests(p, w.m, [&](int e, int r, int, int) {
+        ok = for_requests(p, w.m, p.tile_q[w.m], [&](int e, int r, int, int) {
           for (int r0 = 0; r0 < r; r0 += kStep) {
             // rows of v are 16-byte aligned, v_rs a multiple of 8; beyond the rank: zeros
             fetch_x(one.x, p.v, p.v_rs, w.t0, r0, r, true);
@@ -300,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       if (lowrank && ok) {
         if (!waited) dependency_wait();
         waited = true;
-        ok = for_requests(p, w.m, [&](int, int r, int, int) {
+        ok = for_requests(p, w.m, p.tile_q[w.m], [&](int, int r, int, int) {
           for (int r0 = 0; r0 < r; r0 += kStep)
             if (!step((min(r - r0, kStep) + 7) / 8, true, true, id)) return false;
           return true;
@@ -351,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
         waited = true;
       }
       if (lowrank && ok)
-        ok = for_requests(p, w.m, [&](int, int r, int a, int b) {
+        ok = for_requests(p, w.m, p.tile_q[w.m], [&](int, int r, int a, int b) {
           for (int r0 = 0; r0 < r; r0 += kStep)
             if (!drain(row >= a && row < b)) return false;
           return true;

@@ -15,9 +15,8 @@
 //           lie, as MN-major images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
 //   loads:  any stride and alignment, by the epilogue's warps.
 #include <cooperative_groups.h>
-#include <cuda.h>
 
-#include "cf_adapter_dev.cuh"
+#include "cf_adapter_tma.cuh"
 
 namespace cg = cooperative_groups;
 
@@ -33,35 +32,6 @@ constexpr int kThreads = 320;
 
 // A bounded wait that gave up leaves its site here (cf_adapter_check).
 __device__ int g_err;
-
-__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-      "[%2];" ::"r"(dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
-      : "memory");
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                        uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
-// MN-major, 128-byte swizzle: 64 columns (128 B) x 8 contraction steps an atom; groups of 8 steps
-// 1024 B apart, blocks of 64 columns 64 steps x 128 B = 8192 B apart.
-__device__ __forceinline__ uint64_t mn_desc(uint32_t smem_addr) {
-  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-struct Maps {
-  CUtensorMap x, b, v_hi, v_lo, q;
-};
 
 struct Tiling {
   int64_t m_tiles, units;  // units: clusters that work on tiles; behind them, clusters that plan tiles
@@ -387,43 +357,13 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
         if (re == kMixed || n >= p.N) continue;
         const float4 s = sum4(row, lane * 4);
         float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
-        if (te == kMixed) add_lowrank<T, kSub>(p, t, re, rank_of(p, re), n, a);
+        if (te == kMixed || te == kFew) add_lowrank<T, kSub>(p, t, re, rank_of(p, re), n, a);
         store4<T>(p, t, n, a);
       }
     }
   }
   __syncwarp();
   if (split > 1) cl.sync();  // nobody leaves while its part is read
-}
-
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeFn encoder() {
-  static EncodeFn fn = [] {
-    void* f = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
-    return (EncodeFn)f;
-  }();
-  return fn;
-}
-
-// [z][y][x] of 16-bit elements, x contiguous, boxes of 64 x box_y, 128-byte swizzle, zeros outside
-cf_status encode(CUtensorMap* map, int dtype, const void* base, int64_t nx, int64_t ny, int64_t nz, int64_t ys,
-                 int64_t zs, int box_y) {
-  EncodeFn fn = encoder();
-  CF_REQUIRE(fn, CF_ERR_CUDA, "adapter_matmul: cuTensorMapEncodeTiled is not available");
-  const cuuint64_t dims[3] = {(cuuint64_t)nx, (cuuint64_t)ny, (cuuint64_t)nz};
-  const cuuint64_t strides[2] = {(cuuint64_t)ys * 2, (cuuint64_t)(nz > 1 ? zs : ys * ny) * 2};
-  const cuuint32_t box[3] = {64, (cuuint32_t)box_y, 1}, ones[3] = {1, 1, 1};
-  CUresult r = fn(map, dtype == CF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-                  const_cast<void*>(base), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  CF_REQUIRE(r == CUDA_SUCCESS, CF_ERR_CUDA, "adapter_matmul: tensor map: error %d", (int)r);
-  return CF_OK;
 }
 
 template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
@@ -494,18 +434,12 @@ cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cu
   }
   constexpr int bn = 128;
   if (kTma) {
-    if (kSub)
-      CF_TRY(encode(&maps.b, dtype, p.M, p.N, p.K, 1, p.m_ks, p.m_ks * p.K, 64));
-    else
-      CF_TRY(encode(&maps.b, dtype, p.M, p.K, p.N, 1, p.m_ns, p.m_ns * p.N, bn));
     if (pair && p.R > 0) {
       CF_TRY(encode(&maps.v_hi, dtype, p.v_hi, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
       CF_TRY(encode(&maps.v_lo, dtype, p.v_lo, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
-      if (kSub)
-        CF_TRY(encode(&maps.q, dtype, p.Qm, p.N, p.R, p.E, p.q_rs, p.q_es, 64));
-      else
-        CF_TRY(encode(&maps.q, dtype, p.Qm, p.R, p.N, p.E, p.q_ns, p.q_es, bn));
     }
+    if (m_tiles * ceil_div(p.N, 256) >= 148) return launch_wide(p, dtype, kSub, maps, g.q_tma, st);
+    CF_TRY(encode_weights(p, dtype, kSub, bn, g.q_tma, &maps));
   }
   g.dependent = p.R > 0;
   g.units = m_tiles * ceil_div(p.N, bn);

@@ -485,3 +485,11 @@ def test_adapters_then_rules():
     assert torch.equal(rival.cpu(), wj)
     ok = (v.gather(1, best[:, None])[:, 0] > -math.inf).cpu()
     assert (m.cpu()[ok] >= 0).all()
+
+
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_adapter_grid_of_wide_tiles(dtype, sub):
+    """Enough tiles that every SM walks over several, the last ones ragged in both directions."""
+    compare(make(4000, 72, 5208, 32, 5, 9, dtype, sub, seed=31, ranks=True, bias=True), sub)
+    compare(make(8000, 136, 2056, 72, 3, 60, dtype, sub, seed=32), sub)
