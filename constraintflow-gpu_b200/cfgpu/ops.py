@@ -7,6 +7,7 @@ cf_edit_logits, cf_answer_margin).
 Operands are CUDA tensors, possibly broadcast views (zero strides); results are new
 contiguous tensors.  PyTorch only allocates the memory and supplies the stream.
 """
+import contextlib
 import ctypes
 import operator
 
@@ -202,20 +203,18 @@ _DTYPES = {torch.float32: _lib.CF_F32, torch.bfloat16: _lib.CF_BF16, torch.float
 def _expect(name, t, dtype, shape, dev, strided=False):
     """Refuse a tensor that is not `dtype` on `dev` of `shape` (None: any size), its last
     dimension contiguous (strided) or all of them."""
-    ok = t.dtype == dtype and t.device == dev and t.dim() == len(shape) and \
-        all(w is None or s == w for s, w in zip(t.shape, shape))
-    if ok and strided:
-        ok = t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] <= 1
-    elif ok:
-        ok = t.is_contiguous()
-    if not ok:
-        raise Exception(f"SHAPE MISMATCH: {name} must be {dtype} {tuple('any' if w is None else w for w in shape)} on "
-                        f"{dev}{', its rows contiguous' if strided else ', contiguous'}; got {t.dtype} "
-                        f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+    if t.dtype is dtype and t.device == dev:
+        got = t.shape
+        if got == shape or (len(got) == len(shape) and all(w is None or g == w for g, w in zip(got, shape))):
+            if t.is_contiguous() or (strided and (t.stride(-1) == 1 or got[-1] <= 1)):
+                return
+    raise Exception(f"SHAPE MISMATCH: {name} must be {dtype} {tuple('any' if w is None else w for w in shape)} on "
+                    f"{dev}{', its rows contiguous' if strided else ', contiguous'}; got {t.dtype} "
+                    f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
 
 
 def _cuda(name, t):
-    if t.device.type != "cuda":
+    if not t.is_cuda:
         raise RuntimeError(f"{name} is on {t.device}: libcfgpu runs on CUDA tensors only (no CPU fallback)")
     return t.device
 
@@ -228,9 +227,17 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(dev):
-    """Make dev the current device, for the launch, where it is not."""
-    return torch.cuda.device(dev)
+    """dev as the current device, for a launch."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _raw_stream(dev):
+    """The handle of the current stream of dev."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 class AdapterLayer:
@@ -302,7 +309,7 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
         LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
         st = _lib.lib.cf_adapter_matmul(layer._ref, int(substitute), T, x.data_ptr(), _row_stride(x), Q,
                                         offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
-                                        ws.data_ptr(), need, _stream())
+                                        ws.data_ptr(), need, _raw_stream(dev))
     _lib.check(st, "cf_adapter_matmul")
     return out
 
@@ -310,7 +317,7 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
 def adapter_check(device=None):
     """Wait for the current stream and raise if a bounded device-side wait of an adapter_matmul
     on `device` gave up since the last check (its rows are not valid then)."""
-    with _on(torch.device("cuda") if device is None else device):
+    with torch.cuda.device(device):
         _lib.check(_lib.lib.cf_adapter_check(_stream()), "cf_adapter_check")
 
 
@@ -369,7 +376,7 @@ def _rules_rows(name, t, rules, dtype):
     dev = _cuda(name, t)
     if rules.device is not None and dev != rules.device:
         raise Exception(f"SHAPE MISMATCH: {name} is on {dev}, the rules are on {rules.device}")
-    if t.dim() == 2 and t.stride(1) != 1 and t.shape[1] > 1:
+    if t.stride(-1) != 1:
         t = t.contiguous()
     _expect(name, t, dtype, (rules.rows, rules.n), dev, strided=True)
     return t, dev
@@ -388,7 +395,7 @@ def edit_logits(logits, rules, out=None):
     with _on(dev):
         LAUNCHES[0] += 1
         st = _lib.lib.cf_edit_logits(rules._ref, _DTYPES[x.dtype], x.data_ptr(), _row_stride(x), out.data_ptr(),
-                                     _row_stride(out), _stream())
+                                     _row_stride(out), _raw_stream(dev))
     _lib.check(st, "cf_edit_logits")
     return out
 
@@ -400,14 +407,15 @@ def answer_margin(l, u, labels, rules):
     rival [rows] int32, that other answer (the lowest on equal bounds, -1: none is left).
     A label that is not allowed has margin -inf; a bound that is NaN bounds nothing."""
     l, dev = _rules_rows("l", l, rules, torch.float32)
-    u, _ = _rules_rows("u", u, rules, torch.float32)
-    _expect("u", u, torch.float32, (rules.rows, rules.n), dev, strided=True)
+    u, udev = _rules_rows("u", u, rules, torch.float32)
+    if udev != dev:
+        raise Exception(f"SHAPE MISMATCH: l is on {dev}, u on {udev}")
     _expect("labels", labels, torch.int64, (rules.rows,), dev)
     margin = torch.empty(rules.rows, dtype=torch.float32, device=dev)
     rival = torch.empty(rules.rows, dtype=torch.int32, device=dev)
     with _on(dev):
         LAUNCHES[0] += 1
         st = _lib.lib.cf_answer_margin(rules._ref, l.data_ptr(), _row_stride(l), u.data_ptr(), _row_stride(u),
-                                       labels.data_ptr(), margin.data_ptr(), rival.data_ptr(), _stream())
+                                       labels.data_ptr(), margin.data_ptr(), rival.data_ptr(), _raw_stream(dev))
     _lib.check(st, "cf_answer_margin")
     return margin, rival

@@ -452,7 +452,8 @@ cf_status cf_adapter_check(void* stream);
  * applied to a logit x of answer j, in float32, each step rounded:
  *   v = x; j in the history: v = v > 0 ? v / repetition : v * repetition; answered c > 0 times:
  *   v = v - frequency * c, v = v - presence; j has a bias: v = v + bias; not allowed: -inf.
- * Tokens and ids outside 0 .. n-1 are ignored, and offsets are held within their lists.  With
+ * Tokens and ids outside 0 .. n-1 are ignored, and offsets are held within their lists; n,
+ * n_tokens and n_biases are at most 2^30.  With
  * repetition > 0 every step is monotone: the edited bounds of a logit bound the edited logit. */
 typedef struct cf_answer_rules {
   int64_t rows, n;
