@@ -11,16 +11,17 @@
 // is monotone in x for repetition > 0: the edit of a lower (upper) bound is a lower (upper)
 // bound of the edit, rounding included, and no interval arithmetic is needed.
 //
-// Memory-bound: a row is read (and written) once, and only its mask is looked at on the way.
-// What the history and the biases touch is little, so it is put right afterwards: while a CTA has
-// the logits of its slice of the answers on their way into registers, it counts in shared memory
-// what they say about the slice, lists the touched answers, and edits those alone.  (A lookup for
-// every answer on the way, with the edit under a branch, took 228 us for 256 x 131072 bfloat16:
-// some lane of nearly every warp has one.)  Tables hold 16 bits an answer (seen, and 15 bits of
-// times; the place of the last bias); a row with a longer history or more biases is put right in
-// two halves of 32-bit tables.  Every CTA of a row walks its history, or, where histories are
-// long, a cluster shares the walk and counts through distributed shared memory.  Counts are
-// integers and "the last entry" is a maximum, so the order of the atomics changes nothing.
+// Memory-bound: a row is read (and written) once.  What the history and the biases touch is
+// little and is put right from their side: a CTA counts in shared memory what they say about its
+// slice of the answers, lists the answers that are touched, and edits those alone.  (A table
+// lookup for every answer on the way, the edit under a branch, took 228 us for 256 x 131072
+// bfloat16 with 1024 tokens a row: some lane of nearly every warp has one.)
+//
+// Tables hold 16 bits an answer, seen and 15 bits of times, and a bit for its having a bias.
+// Which of the (few) biases of one answer is the last is found by comparing them.  A row with more
+// than kMaxBiases biases, or one answer more than kTimes times, is done in quarters of a
+// slice, with 32 bits for the times and 32 for the place of the last bias.  Counts are integers
+// and "the last entry" is a maximum, so the order of the atomics changes nothing.
 #include <cooperative_groups.h>
 
 #include "cf_common.cuh"
@@ -31,11 +32,10 @@ namespace cg = cooperative_groups;
 namespace cf {
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u;  // in the history, prompt included
-constexpr int kThreads = 256;
-constexpr int kMaxCluster = 8;
-constexpr uint32_t kList = 1024;  // touched answers of a slice that are edited from a list
-constexpr int kMaxTimes = 0x7fff, kMaxPlace = 0xffff;  // of the 16-bit tables
+// of a table's entry, 16 bits (wide: the highest of 32)
+constexpr uint32_t kSeen = 0x8000u, kTimes = 0x7fffu, kWideTimes = 0x7fffffffu;
+constexpr uint32_t kMaxBiases = 1024;
+constexpr uint32_t kList = 2048;  // touched answers of a slice that are edited from a list
 
 struct Row {
   uint32_t h0, h1, answered;  // history, and where its answered part begins
@@ -47,7 +47,13 @@ struct Row {
 // x within 0 .. n
 __device__ __forceinline__ uint32_t clamp_to(int64_t x, int64_t n) { return (uint32_t)(x < 0 ? 0 : (x > n ? n : x)); }
 
-__device__ Row load_row(const cf_answer_rules& R, int64_t r) {
+__device__ __forceinline__ const uint32_t* mask_of(const cf_answer_rules& R, int64_t r) {
+  if (!R.allowed_dev) return nullptr;
+  const int64_t m = R.allowed_row_dev ? (int64_t)R.allowed_row_dev[r] : r;
+  return m >= 0 && m < R.n_masks ? (const uint32_t*)R.allowed_dev + m * R.allowed_words : nullptr;
+}
+
+__device__ __forceinline__ Row load_row(const cf_answer_rules& R, int64_t r) {
   Row w;
   w.h0 = w.h1 = w.b0 = w.b1 = 0;
   if (R.tokens_dev) {
@@ -62,96 +68,74 @@ __device__ Row load_row(const cf_answer_rules& R, int64_t r) {
   w.rep = R.repetition_dev ? R.repetition_dev[r] : 1.0f;
   w.freq = R.frequency_dev ? R.frequency_dev[r] : 0.0f;
   w.pres = R.presence_dev ? R.presence_dev[r] : 0.0f;
-  w.allowed = nullptr;
-  if (R.allowed_dev) {
-    const int64_t m = R.allowed_row_dev ? (int64_t)R.allowed_row_dev[r] : r;
-    if (m >= 0 && m < R.n_masks) w.allowed = (const uint32_t*)R.allowed_dev + m * R.allowed_words;
-  }
+  w.allowed = mask_of(R, r);
   return w;
 }
 
-__device__ __noinline__ float edit(float v, uint32_t c, uint32_t bias_at, const Row& w,
-                                   const float* biases) {
-  if (c) {
-    v = v > 0.0f ? __fdiv_rn(v, w.rep) : __fmul_rn(v, w.rep);
-    const uint32_t times = c & ~kSeen;
-    if (times) v = __fsub_rn(__fsub_rn(v, __fmul_rn(w.freq, (float)times)), w.pres);
+__device__ __forceinline__ bool is_allowed(const uint32_t* allowed, int j) {
+  return !allowed || (allowed[j >> 5] >> (j & 31) & 1u);
+}
+
+// The bits of `allowed` for answers j .. j+N-1, 0 for those outside 0 .. n-1.
+template <int N>
+__device__ __forceinline__ uint32_t open_bits(const uint32_t* allowed, int j, int n) {
+  uint32_t bits = 0;
+  if (j >= 0 && j + N <= n) {
+    if (!allowed) return (1u << N) - 1;
+    const int sh = j & 31;
+    bits = allowed[j >> 5] >> sh;
+    if (sh + N > 32) bits |= allowed[(j >> 5) + 1] << (32 - sh);
+    return bits & ((1u << N) - 1);
   }
-  if (bias_at) v = __fadd_rn(v, biases[w.b0 + bias_at - 1]);
+  for (int e = 0; e < N; ++e)
+    if (j + e >= 0 && j + e < n && is_allowed(allowed, j + e)) bits |= 1u << e;
+  return bits;
+}
+
+// c: times, kSeen (in the history, the given part included)
+__device__ __noinline__ float edit(float v, bool seen, uint32_t times, float rep, float freq, float pres) {
+  if (seen) {
+    v = v > 0.0f ? __fdiv_rn(v, rep) : __fmul_rn(v, rep);
+    if (times) v = __fsub_rn(__fsub_rn(v, __fmul_rn(freq, (float)times)), pres);
+  }
   return v;
 }
 
-// A slice's tables: S entries of 16 bits each or, wide, half of them of 32 bits; and the list of
-// its touched entries.
+// ------------------------------------------------------------------ what a row touches
+// Shared memory of a CTA that edits a slice of 1 << log_s answers.
 struct Tables {
-  uint32_t *cnt, *pos;
-  uint32_t* listed;  // touched entries; the list holds the first kList
-  uint16_t* list;    // an entry; kBias: because of a bias
+  uint32_t* words;   // 16-bit entries of a slice; wide: 32-bit counts, then places, of a quarter
+  uint32_t* biased;  // a bit for each answer
+  uint32_t* listed;  // touched answers; the list holds the first kList
+  uint32_t* over;    // an answer has more than kTimes
+  uint16_t* list;    // places in the slice (quarter)
+  int32_t* ids;      // the row's biases (not wide)
   int log_s;
-  bool wide, hist, bias;
+  bool wide;
 };
-constexpr uint32_t kBias = 0x8000u;
 
-// Another CTA's tables.
-__device__ __forceinline__ Tables of_rank(const Tables& t, cg::cluster_group& cl, uint32_t rank) {
-  Tables o = t;
-  o.cnt = cl.map_shared_rank(t.cnt, rank);
-  o.pos = cl.map_shared_rank(t.pos, rank);
-  o.listed = cl.map_shared_rank(t.listed, rank);
-  o.list = cl.map_shared_rank(t.list, rank);
-  return o;
+size_t tables_bytes(int log_s) {
+  return ((size_t)2 << log_s) + ((size_t)1 << (log_s - 3)) + 16 + kList * 2 + kMaxBiases * 4;
 }
 
-__device__ __forceinline__ void put(const Tables& t, uint32_t i) {
-  const uint32_t at = atomicAdd(t.listed, 1u);
-  if (at < kList) t.list[at] = (uint16_t)i;
+__device__ __forceinline__ Tables tables_of(const Row& w, uint32_t* smem, int log_s) {
+  Tables t;
+  t.words = smem;
+  t.biased = smem + (1u << (log_s - 1));
+  t.listed = t.biased + (1u << (log_s - 5));
+  t.over = t.listed + 1;
+  t.list = (uint16_t*)(t.listed + 4);
+  t.ids = (int32_t*)(t.list + kList);
+  t.log_s = log_s;
+  t.wide = w.b1 - w.b0 > kMaxBiases;
+  return t;
 }
 
-// Count a token of entry i of the slice (k: of its table), listed at the first.
-__device__ __forceinline__ void add_times(const Tables& t, uint32_t i, uint32_t k, bool answered) {
-  uint32_t old;
-  if (t.wide) {
-    old = answered ? atomicAdd(t.cnt + k, 1u) : atomicOr(t.cnt + k, kSeen);
-  } else {
-    const uint32_t sh = (k & 1) * 16;
-    old = answered ? atomicAdd(t.cnt + (k >> 1), 1u << sh) : atomicOr(t.cnt + (k >> 1), 0x8000u << sh);
-    old = (old >> sh) & 0xffffu;
-  }
-  if (old == 0) put(t, i);
-}
-
-__device__ __forceinline__ void max_place(const Tables& t, uint32_t i, uint32_t k, uint32_t place) {
-  uint32_t first;
-  if (t.wide) {
-    first = atomicMax(t.pos + k, place);
-  } else {
-    const uint32_t sh = (k & 1) * 16;
-    uint32_t old = *(volatile uint32_t*)(t.pos + (k >> 1));
-    for (;;) {
-      first = (old >> sh) & 0xffffu;
-      if (first >= place) break;
-      const uint32_t seen = atomicCAS(t.pos + (k >> 1), old, (old & ~(0xffffu << sh)) | (place << sh));
-      if (seen == old) break;
-      old = seen;
-    }
-  }
-  if (first == 0) put(t, i | kBias);
-}
-
-__device__ __forceinline__ void sync_all(cg::cluster_group& cl) {
-  if (cl.num_blocks() > 1)
-    cl.sync();
-  else
-    __syncthreads();
-}
-
-// f(list[i], i) for this CTA's share of [from, end), kBatch loads in flight.
-template <typename F>
-__device__ __forceinline__ void walk(const int32_t* list, uint32_t from, uint32_t end, uint32_t nc, uint32_t rank,
-                                     F&& f) {
-  constexpr int kBatch = 4;
-  const uint32_t step = nc * kThreads;
-  for (uint32_t i = from + rank * kThreads + threadIdx.x; i < end; i += kBatch * step) {
+// f(list[i], i) over [from, end) by the CTA, kBatch loads in flight a thread.
+template <int kBatch, typename F>
+__device__ __forceinline__ void walk(const int32_t* list, uint32_t from, uint32_t end, F&& f) {
+  const uint32_t step = blockDim.x;
+  for (uint32_t i = from + threadIdx.x; i < end; i += kBatch * step) {
     int32_t j[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) j[b] = i + b * step < end ? list[i + b * step] : -1;
@@ -161,233 +145,227 @@ __device__ __forceinline__ void walk(const int32_t* list, uint32_t from, uint32_
   }
 }
 
-// The slices [lo + rank * S, + S) of a cluster's CTAs; lo counts answers and may start before the
-// first (the row's own alignment).  Wide: half `side` of each slice.
-struct Span {
-  int32_t lo, n;
-  int side;
-};
-
-// Fill the tables.  Every CTA of the cluster calls it.
-__device__ __forceinline__ void fill(const cf_answer_rules& R, const Row& w, const Tables& t, const Span& s,
-                                     cg::cluster_group& cl) {
-  const uint32_t S = 1u << t.log_s, nc = cl.num_blocks(), rank = cl.block_rank();
-  for (uint32_t i = threadIdx.x * 4; i < S / 2; i += kThreads * 4) {
-    if (t.hist) *(uint4*)(t.cnt + i) = make_uint4(0, 0, 0, 0);
-    if (t.bias) *(uint4*)(t.pos + i) = make_uint4(0, 0, 0, 0);
+// The counts of answers [lo, lo + size) from the row's history, and the list of those it holds.
+// False: to be done wide.
+__device__ __forceinline__ bool count(const cf_answer_rules& R, const Row& w, const Tables& t, int lo, uint32_t size) {
+  const uint32_t words = t.wide ? size : (size + 1) / 2;
+  for (uint32_t i = threadIdx.x * 4; i < words; i += blockDim.x * 4) {
+    *(uint4*)(t.words + i) = make_uint4(0, 0, 0, 0);
+    if (t.wide) *(uint4*)(t.words + (1u << (t.log_s - 2)) + i) = make_uint4(0, 0, 0, 0);
   }
-  if (threadIdx.x == 0) *t.listed = 0;
-  sync_all(cl);
-  const uint32_t mask = (S >> (t.wide ? 1 : 0)) - 1;
-  // f(owner's tables, entry of the slice, of the table) where answer j is of this span and half
-  auto at = [&](int32_t j, auto&& f) {
-    const uint32_t rel = (uint32_t)(j - s.lo);
-    if (j < 0 || j >= s.n || rel >= nc << t.log_s) return;
-    const uint32_t i = rel & (S - 1);
-    if (t.wide && (int)(i >> (t.log_s - 1)) != s.side) return;
-    if (nc > 1)
-      f(of_rank(t, cl, rel >> t.log_s), i, i & mask);
-    else
-      f(t, i, i & mask);
-  };
-  walk(R.tokens_dev, w.h0, w.h1, nc, rank, [&](int32_t j, uint32_t h) {
-    at(j, [&](const Tables& o, uint32_t i, uint32_t k) { add_times(o, i, k, h >= w.answered); });
-  });
-  walk(R.bias_ids_dev, w.b0, w.b1, nc, rank, [&](int32_t j, uint32_t b) {
-    at(j, [&](const Tables& o, uint32_t i, uint32_t k) { max_place(o, i, k, b - w.b0 + 1u); });
-  });
-  sync_all(cl);
-}
-
-// Entry i of the slice: its count (seen in the highest bit) and the place of its bias, or 0.
-__device__ __forceinline__ void look(const Tables& t, uint32_t i, uint32_t& c, uint32_t& p) {
-  c = p = 0;
-  if (t.wide) {
-    i &= (1u << (t.log_s - 1)) - 1;
-    if (t.hist) c = t.cnt[i];
-    if (t.bias) p = t.pos[i];
-  } else {
-    const uint32_t sh = (i & 1) * 16;
-    if (t.hist) {
-      c = (t.cnt[i >> 1] >> sh) & 0xffffu;
-      c = (c & 0x7fffu) | (c & 0x8000u) << 16;
+  if (w.b1 > w.b0)
+    for (uint32_t i = threadIdx.x; i < (size + 31) / 32; i += blockDim.x) t.biased[i] = 0;
+  if (threadIdx.x == 0) *t.listed = *t.over = 0;
+  if (!t.wide)
+    for (uint32_t i = w.b0 + threadIdx.x; i < w.b1; i += blockDim.x) t.ids[i - w.b0] = R.bias_ids_dev[i];
+  __syncthreads();
+  walk<8>(R.tokens_dev, w.h0, w.h1, [&](int32_t j, uint32_t h) {
+    const uint32_t k = (uint32_t)(j - lo);
+    if (k >= size) return;
+    const bool answered = h >= w.answered;
+    uint32_t old;
+    if (t.wide) {
+      old = answered ? atomicAdd(t.words + k, 1u) : atomicOr(t.words + k, kSeen << 16);
+    } else {
+      const uint32_t sh = (k & 1) * 16;
+      old = answered ? atomicAdd(t.words + (k >> 1), 1u << sh) : atomicOr(t.words + (k >> 1), kSeen << sh);
+      old = old >> sh & 0xffffu;
+      if (answered && (old & kTimes) == kTimes) *(volatile uint32_t*)t.over = 1;
     }
-    if (t.bias) p = (t.pos[i >> 1] >> sh) & 0xffffu;
-  }
-}
-
-// Entry at place `at` of the list with what touches it; false: listed for its bias, and for its
-// count as well.
-__device__ __forceinline__ bool listed_entry(const Tables& t, uint32_t at, uint32_t& i, uint32_t& c, uint32_t& p) {
-  const uint32_t e = t.list[at];
-  i = e & ~kBias;
-  look(t, i, c, p);
-  return !(e & kBias) || c == 0;
-}
-
-// bit e: entry i + e of four is touched
-__device__ __forceinline__ uint32_t touched4(const Tables& t, uint32_t i) {
-  if (t.wide) {
-    i &= (1u << (t.log_s - 1)) - 1;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (t.hist) v = *(const uint4*)(t.cnt + i);
-    if (t.bias) {
-      const uint4 q = *(const uint4*)(t.pos + i);
-      v.x |= q.x, v.y |= q.y, v.z |= q.z, v.w |= q.w;
+    if (old == 0) {
+      const uint32_t at = atomicAdd(t.listed, 1u);
+      if (at < kList) t.list[at] = (uint16_t)k;
     }
-    return (v.x != 0) | (v.y != 0) << 1 | (v.z != 0) << 2 | (v.w != 0) << 3;
-  }
-  uint2 v = make_uint2(0, 0);
-  if (t.hist) v = *(const uint2*)(t.cnt + i / 2);
-  if (t.bias) {
-    const uint2 q = *(const uint2*)(t.pos + i / 2);
-    v.x |= q.x, v.y |= q.y;
-  }
-  if (!(v.x | v.y)) return 0;
-  return ((v.x & 0xffffu) != 0) | (v.x >> 16 != 0) << 1 | ((v.y & 0xffffu) != 0) << 2 | (v.y >> 16 != 0) << 3;
+  });
+  if (t.wide)
+    walk<4>(R.bias_ids_dev, w.b0, w.b1, [&](int32_t j, uint32_t b) {
+      const uint32_t k = (uint32_t)(j - lo);
+      if (k < size) atomicMax(t.words + (1u << (t.log_s - 2)) + k, b - w.b0 + 1u);
+    });
+  __syncthreads();
+  return t.wide || *t.over == 0;
 }
 
-__device__ __forceinline__ Tables tables_of(const cf_answer_rules& R, const Row& w, uint32_t* smem, int log_s) {
-  const uint32_t words = 1u << (log_s - 1);
-  Tables t;
-  t.log_s = log_s;
-  t.hist = w.h1 > w.h0;
-  t.bias = w.b1 > w.b0;
-  t.wide = w.h1 - w.h0 > kMaxTimes || w.b1 - w.b0 > kMaxPlace;
-  t.cnt = smem;
-  t.pos = smem + words;
-  t.listed = smem + words * (R.bias_ids_dev ? 2 : 1);
-  t.list = (uint16_t*)(t.listed + 4);
-  return t;
+// Entry k: 0 if the history does not hold it, else kSeen or its times, in 32 bits.
+__device__ __forceinline__ uint32_t entry(const Tables& t, uint32_t k) {
+  return t.wide ? t.words[k] : t.words[k >> 1] >> (k & 1) * 16 & 0xffffu;
+}
+__device__ __forceinline__ uint32_t times(const Tables& t, uint32_t entry) {
+  return entry & (t.wide ? kWideTimes : kTimes);
+}
+__device__ __forceinline__ bool is_biased(const Row& w, const Tables& t, uint32_t k) {
+  return w.b1 > w.b0 && (t.biased[k >> 5] >> (k & 31) & 1u);
 }
 
+// f(answer, seen, times, bias) for each answer of the slice that has a bias; it is marked.
+template <typename F>
+__device__ __forceinline__ void for_biased(const cf_answer_rules& R, const Row& w, const Tables& t, int lo,
+                                           uint32_t size, F&& f) {
+  for (uint32_t b = w.b0 + threadIdx.x; b < w.b1; b += blockDim.x) {
+    const int j = t.wide ? R.bias_ids_dev[b] : t.ids[b - w.b0];
+    const uint32_t k = (uint32_t)(j - lo);
+    if (k >= size) continue;
+    bool last = true;
+    if (t.wide) {
+      last = t.words[(1u << (t.log_s - 2)) + k] == b - w.b0 + 1u;
+    } else {
+      const uint32_t n = w.b1 - w.b0;
+#pragma unroll 4
+      for (uint32_t i = b - w.b0 + 1; i < n; ++i) last &= t.ids[i] != j;
+    }
+    if (!last) continue;
+    atomicOr(t.biased + (k >> 5), 1u << (k & 31));
+    const uint32_t c = entry(t, k);
+    f(j, c != 0, times(t, c), R.bias_values_dev[b]);
+  }
+}
+
+// f(answer, times, x[answer]) for each allowed answer of the slice that the history holds and
+// that has no bias; kBatch loads of x in flight a thread.
+template <typename T, typename F>
+__device__ __forceinline__ void for_seen(const Row& w, const Tables& t, int lo, uint32_t size, const T* x, F&& f) {
+  constexpr int kBatch = 8;
+  const uint32_t listed = *t.listed;
+  const bool all = listed > kList;  // more than the list holds: entry by entry
+  const uint32_t n = all ? size : listed;
+  for (uint32_t i = threadIdx.x; i < n; i += kBatch * blockDim.x) {
+    uint32_t k[kBatch], c[kBatch];
+    T v[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const uint32_t at = i + b * blockDim.x;
+      k[b] = all ? at : at < n ? t.list[at] : 0u;
+      c[b] = at < n ? entry(t, k[b]) : 0u;
+      if (c[b] && is_biased(w, t, k[b])) c[b] = 0;
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (c[b] && !is_allowed(w.allowed, lo + (int)k[b])) c[b] = 0;
+      v[b] = c[b] ? x[lo + (int)k[b]] : from_f32<T>(0.0f);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (c[b]) f(lo + (int)k[b], times(t, c[b]), to_f32(v[b]));
+  }
+}
+
+// 16 bytes of a row, moved whole; rows are read once and written once, past the caches' own order.
 template <typename T>
 struct alignas(16) Vec {
   static constexpr int N = 16 / sizeof(T);
   T v[N];
+  __device__ __forceinline__ void load(const T* p) { *(uint4*)v = __ldcs((const uint4*)p); }
+  __device__ __forceinline__ void store(T* p) const { __stcs((uint4*)p, *(const uint4*)v); }
 };
 
-// The bits of `allowed` for N answers from j on, all of them answers.
-template <int N>
-__device__ __forceinline__ uint32_t allowed_bits(const uint32_t* allowed, int32_t j) {
-  if (!allowed) return 0xffffffffu;
-  const int sh = (int)(j & 31);
-  uint32_t bits = allowed[j >> 5] >> sh;
-  if (sh + N > 32) bits |= allowed[(j >> 5) + 1] << (32 - sh);
-  return bits;
-}
+// ---------------------------------------------------------------------- edit_logits
+// out = allowed ? in : -inf, by a grid that is resident all at once; chunks of 256 x kUnroll
+// vectors.  Where out is in, only vectors that hold something not allowed are written.
+constexpr int kStreamThreads = 256, kUnroll = 4;
 
-// Elements [j, j + V) of a row of n: whole vectors where they are, zeros outside.
 template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* x, int32_t j, int32_t n) {
-  constexpr int V = Vec<T>::N;
-  if (j >= 0 && j + V <= n) return *(const Vec<T>*)(x + j);
-  Vec<T> t;
+__global__ void __launch_bounds__(kStreamThreads)
+    k_answer_stream(const cf_answer_rules R, const T* in, int64_t in_rs, T* out, int64_t out_rs, int chunks,
+                    int64_t units) {
+  constexpr int V = Vec<T>::N, kChunk = kStreamThreads * kUnroll * V;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int n = (int)R.n;
+  const bool in_place = in == out && in_rs == out_rs;
+  int64_t r = blockIdx.x / chunks;
+  int c = (int)(blockIdx.x - r * chunks);
+  const int64_t step_r = gridDim.x / chunks;
+  const int step_c = (int)(gridDim.x - step_r * chunks);
+  for (int64_t unit = blockIdx.x; unit < units; unit += gridDim.x) {
+    const T* x = in + r * in_rs;
+    T* y = out + r * out_rs;
+    // vectors start at 16-byte boundaries of the row's memory
+    const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+    const bool aligned = (((uintptr_t)y - (uintptr_t)mis * sizeof(T)) & 15) == 0;
+    const uint32_t* allowed = mask_of(R, r);
+    const int j0 = c * kChunk - mis + (int)threadIdx.x * V;
+    if (!in_place || allowed) {
+      Vec<T> t[kUnroll];
 #pragma unroll
-  for (int e = 0; e < V; ++e) t.v[e] = j + e >= 0 && j + e < n ? x[j + e] : from_f32<T>(0.0f);
-  return t;
+      for (int i = 0; i < kUnroll; ++i) {
+        const int j = j0 + i * kStreamThreads * V;
+        if (j >= 0 && j + V <= n) {
+          t[i].load(x + j);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (j + e >= 0 && j + e < n) t[i].v[e] = x[j + e];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        const int j = j0 + i * kStreamThreads * V;
+        if (j >= n) break;
+        const uint32_t bits = open_bits<V>(allowed, j, n);
+        if (in_place && bits == (1u << V) - 1) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (!(bits >> e & 1u)) t[i].v[e] = from_f32<T>(-INFINITY);
+        if (aligned && j >= 0 && j + V <= n) {
+          t[i].store(y + j);
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (j + e >= 0 && j + e < n) y[j + e] = t[i].v[e];
+        }
+      }
+    }
+    r += step_r;
+    c += step_c;
+    if (c >= chunks) {
+      c -= chunks;
+      ++r;
+    }
+  }
 }
 
-// bit e: answer j + e exists and is allowed
-template <int V>
-__device__ __forceinline__ uint32_t open_bits(const uint32_t* allowed, int32_t j, int32_t n) {
-  if (j >= 0 && j + V <= n) return allowed_bits<V>(allowed, j);
-  uint32_t bits = 0;
-  for (int e = 0; e < V; ++e)
-    if (j + e >= 0 && j + e < n) bits |= (allowed_bits<1>(allowed, j + e) & 1u) << e;
-  return bits;
-}
+// The answers that the history and the biases touch, one CTA per slice of a row, after the stream.
+constexpr int kEditThreads = 512;
 
-// One CTA per slice of a row, `spans` clusters of slices a row.  mis: answers between the 16-byte
-// boundary below the row's start and the start, so that whole vectors are aligned.  A slice is
-// kVpt vectors a thread.
-template <typename T, int kVpt>
-__global__ void __launch_bounds__(kThreads, 4)
-    k_edit_logits(const cf_answer_rules R, const T* in, int64_t in_rs, T* out, int64_t out_rs, int log_s, int spans) {
+template <typename T>
+__global__ void __launch_bounds__(kEditThreads)
+    k_answer_edits(const cf_answer_rules R, const T* in, int64_t in_rs, T* out, int64_t out_rs, int log_s, int slices) {
   extern __shared__ __align__(16) uint32_t smem[];
-  constexpr int V = Vec<T>::N;
-  cg::cluster_group cl = cg::this_cluster();
-  const int nc = (int)cl.num_blocks(), n = (int)R.n;
-  const int64_t cluster = blockIdx.x / nc;
-  const int64_t r = cluster / spans;
+  const int64_t r = blockIdx.x / slices;
+  const int slice = (int)(blockIdx.x - r * slices);
+  const Row w = load_row(R, r);
+  if (w.h0 == w.h1 && w.b0 == w.b1) return;
   const T* x = in + r * in_rs;
   T* y = out + r * out_rs;
-  const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
-  Span s;
-  s.lo = (((int)(cluster - r * spans) * nc) << log_s) - mis;
-  s.n = n;
-  s.side = 0;
-  const int mine = s.lo + ((int)cl.block_rank() << log_s);
-  Vec<T> t[kVpt];
-#pragma unroll
-  for (int i = 0; i < kVpt; ++i) {
-    const int j = mine + (i * kThreads + (int)threadIdx.x) * V;
-    if (j < n) t[i] = load_vec(x, j, n);
-  }
-  const Row w = load_row(R, r);
-  const Tables tab = tables_of(R, w, smem, log_s);
-  const bool aligned = (((uintptr_t)y - (uintptr_t)mis * sizeof(T)) & 15) == 0;
-  auto store = [&](int j, const Vec<T>& v) {
-    if (aligned && j >= 0 && j + V <= n) {
-      *(Vec<T>*)(y + j) = v;
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (j + e >= 0 && j + e < n) y[j + e] = v.v[e];
+  Tables t = tables_of(w, smem, log_s);
+  const int n = (int)R.n;
+  const int end = (int)min((int64_t)n, (int64_t)(slice + 1) << log_s);
+  bool waited = false;
+  uint32_t size;
+  for (int lo = slice << log_s; lo < end; lo += (int)size) {
+    size = (uint32_t)min(1 << (t.wide ? log_s - 2 : log_s), end - lo);
+    if (waited) __syncthreads();  // the tables are filled anew
+    if (!count(R, w, t, lo, size)) {
+      t.wide = true;
+      size = 0;
+      __syncthreads();
+      continue;
     }
-  };
-  const bool touch = tab.hist || tab.bias;
-  if (touch) fill(R, w, tab, s, cl);
-#pragma unroll
-  for (int i = 0; i < kVpt; ++i) {
-    const int j = mine + (i * kThreads + (int)threadIdx.x) * V;
-    if (j >= n) break;
-    const uint32_t bits = open_bits<V>(w.allowed, j, n);
-#pragma unroll
-    for (int e = 0; e < V; ++e)
-      if (!((bits >> e) & 1u)) t[i].v[e] = from_f32<T>(-INFINITY);
-    store(j, t[i]);
-  }
-  if (!touch) return;
-  // Answers that are not allowed stay as they are; the others' logits are as they were, also
-  // where the result takes the logits' place.
-  for (;;) {
-    __syncthreads();
-    const uint32_t listed = *tab.listed;
-    uint32_t i, c, p;
-    if (listed <= kList) {
-      for (uint32_t k = threadIdx.x; k < listed; k += kThreads) {
-        if (!listed_entry(tab, k, i, c, p)) continue;
-        const int j = mine + (int)i;
-        if (!(allowed_bits<1>(w.allowed, j) & 1u)) continue;
-        y[j] = from_f32<T>(edit(to_f32(x[j]), c, p, w, R.bias_values_dev));
-      }
-    } else {  // many: vector by vector
-#pragma unroll 1
-      for (int k = 0; k < kVpt; ++k) {
-        i = (k * kThreads + threadIdx.x) * V;
-        const int j = mine + (int)i;
-        if (j >= n || (tab.wide && (int)(i >> (log_s - 1)) != s.side)) continue;
-        const uint32_t bits = open_bits<V>(w.allowed, j, n);
-        Vec<T> v = load_vec(x, j, n);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          look(tab, i + e, c, p);
-          if (!((bits >> e) & 1u))
-            v.v[e] = from_f32<T>(-INFINITY);
-          else if (c | p)
-            v.v[e] = from_f32<T>(edit(to_f32(v.v[e]), c, p, w, R.bias_values_dev));
-        }
-        store(j, v);
-      }
-    }
-    if (!tab.wide || s.side == 1) return;
-    s.side = 1;
-    sync_all(cl);  // the tables are filled anew
-    fill(R, w, tab, s, cl);
+    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // the stream is done
+    waited = true;
+    // What is not allowed stays -inf; the other logits are as they were, also where the result
+    // takes the logits' place.
+    for_biased(R, w, t, lo, size, [&](int j, bool seen, uint32_t times, float bias) {
+      if (is_allowed(w.allowed, j))
+        y[j] = from_f32<T>(__fadd_rn(edit(to_f32(x[j]), seen, times, w.rep, w.freq, w.pres), bias));
+    });
+    if (w.b1 > w.b0) __syncthreads();  // the marks
+    for_seen(w, t, lo, size, x, [&](int j, uint32_t times, float v) {
+      y[j] = from_f32<T>(edit(v, true, times, w.rep, w.freq, w.pres));
+    });
   }
 }
 
+// --------------------------------------------------------------------- answer_margin
 struct Best {
   float v;
   int32_t j;
@@ -402,102 +380,126 @@ __device__ __forceinline__ void take(Best& a, float v, int32_t j) {
 }
 
 constexpr int32_t kNone = INT32_MAX;
+constexpr int kMarginThreads = 256, kMaxCluster = 8;
 
-// One cluster per row: the label's edited lower bound less the best edited upper bound among the
-// other answers.
-template <int kVpt>
-__global__ void __launch_bounds__(kThreads, 3)
+// the larger, NaN if one is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// One cluster per row, a slice a CTA: the label's edited lower bound less the best edited upper
+// bound among the other answers.  On the way over the bounds a vector is looked into only where it
+// holds something above the best so far; what is touched is left to its own pass.
+__global__ void __launch_bounds__(kMarginThreads, 4)
     k_answer_margin(const cf_answer_rules R, const float* __restrict__ l, int64_t l_rs, const float* __restrict__ u,
                     int64_t u_rs, const int64_t* __restrict__ labels, float* margin, int32_t* rival, int log_s,
-                    int spans) {
+                    int slices) {
   extern __shared__ __align__(16) uint32_t smem[];
-  __shared__ Best part[kThreads / 32];
+  __shared__ Best part_best[kMarginThreads / 32];
   __shared__ Best joined[kMaxCluster];
   __shared__ float label_l;
-  constexpr int V = 4;
+  constexpr int V = 4, kVpt = 4, kChunk = kMarginThreads * V * kVpt;
   cg::cluster_group cl = cg::this_cluster();
   const int nc = (int)cl.num_blocks(), n = (int)R.n;
   const int64_t r = blockIdx.x / nc;
   const float* x = u + r * u_rs;
   const int mis = (int)(((uintptr_t)x & 15) / 4);
   Vec<float> t[kVpt];
-  auto first = [&](int span) {  // answer of this CTA's slice
-    return ((span * nc + (int)cl.block_rank()) << log_s) - mis;
-  };
-  auto load = [&](int span) {
+  // vector i of this thread of the chunk at j0 (j0 + mis a multiple of 4)
+  auto load = [&](int i, int j0, int end) {
+    const int j = j0 + (i * kMarginThreads + (int)threadIdx.x) * V;
+    if (j >= end) return;
+    if (j >= 0 && j + V <= n) {
+      *(float4*)t[i].v = *(const float4*)(x + j);
+    } else {
 #pragma unroll
-    for (int i = 0; i < kVpt; ++i) {
-      const int j = first(span) + (i * kThreads + (int)threadIdx.x) * V;
-      if (j < n) t[i] = load_vec(x, j, n);
+      for (int e = 0; e < V; ++e) t[i].v[e] = j + e >= 0 && j + e < n ? x[j + e] : 0.0f;
     }
   };
-  load(0);
+  auto load_all = [&](int j0, int end) {
+#pragma unroll
+    for (int i = 0; i < kVpt; ++i) load(i, j0, end);
+  };
+  // a slice's answers [lo, end), the first vector's place
+  auto first = [&](int lo) { return ((lo + mis) & ~3) - mis; };
+  const int slice0 = (int)cl.block_rank();
+  if (slice0 < slices) load_all(first(slice0 << log_s), (int)min((int64_t)n, (int64_t)(slice0 + 1) << log_s));
   const Row w = load_row(R, r);
   const int label = labels[r] >= 0 && labels[r] < n ? (int)labels[r] : INT32_MIN;  // or no answer
-  const Tables tab = tables_of(R, w, smem, log_s);
-  const bool touch = tab.hist || tab.bias;
+  Tables tab = tables_of(w, smem, log_s);
+  const bool touch = w.h1 > w.h0 || w.b1 > w.b0;
   if (threadIdx.x == 0) label_l = -INFINITY;
-  sync_all(cl);  // the label's bound is written to the first CTA below
+  cl.sync();  // the label's bound is written to the first CTA below
   Best best{-INFINITY, kNone};
-  // allowed answer j of upper bound `bound` with what touches it
-  auto answer = [&](int j, float bound, uint32_t c, uint32_t p) {
-    if (j == label) {
-      float v = l[r * l_rs + label];
-      if (c | p) v = edit(v, c, p, w, R.bias_values_dev);
-      *cl.map_shared_rank(&label_l, 0) = v != v ? -INFINITY : v;  // a bound that is no number bounds nothing
-    } else {
-      const float v = c | p ? edit(bound, c, p, w, R.bias_values_dev) : bound;
-      take(best, v != v ? INFINITY : v, j);
-    }
+  // the edited bound v of allowed answer j
+  auto bound = [&](int j, float v) { take(best, v != v ? INFINITY : v, j); };
+  auto own = [&](float v) {  // a bound that is no number bounds nothing
+    *cl.map_shared_rank(&label_l, 0) = v != v ? -INFINITY : v;
   };
-  for (int span = 0; span < spans; ++span) {
-    Span s;
-    s.lo = ((span * nc) << log_s) - mis;
-    s.n = n;
-    const int mine = first(span);
-    for (s.side = 0; s.side < (tab.wide ? 2 : 1); ++s.side) {
+  bool loaded = true, counted = false;
+  for (int slice = slice0; slice < slices; slice += nc) {
+    const int end = (int)min((int64_t)n, (int64_t)(slice + 1) << log_s);
+    uint32_t size;
+    for (int lo = slice << log_s; lo < end; lo += (int)size) {
+      const int stop = min(lo + (1 << (tab.wide ? log_s - 2 : log_s)), end);
+      size = (uint32_t)(stop - lo);
       if (touch) {
-        if (span + s.side > 0) sync_all(cl);  // the tables are filled anew
-        fill(R, w, tab, s, cl);
+        if (counted) __syncthreads();  // the tables are filled anew
+        counted = true;
+        if (!count(R, w, tab, lo, size)) {
+          tab.wide = true;
+          size = 0;
+          continue;
+        }
+        for_biased(R, w, tab, lo, size, [&](int j, bool seen, uint32_t times, float bias) {
+          if (!is_allowed(w.allowed, j)) return;
+          if (j == label)
+            own(__fadd_rn(edit(l[r * l_rs + j], seen, times, w.rep, w.freq, w.pres), bias));
+          else
+            bound(j, __fadd_rn(edit(x[j], seen, times, w.rep, w.freq, w.pres), bias));
+        });
+        if (w.b1 > w.b0) __syncthreads();  // the marks
+        for_seen(w, tab, lo, size, x, [&](int j, uint32_t times, float v) {
+          v = edit(j == label ? l[r * l_rs + j] : v, true, times, w.rep, w.freq, w.pres);
+          if (j == label)
+            own(v);
+          else
+            bound(j, v);
+        });
       }
-      // what nothing touches
+      auto touched = [&](int j) {
+        const uint32_t k = (uint32_t)(j - lo);
+        return touch && (entry(tab, k) != 0 || is_biased(w, tab, k));
+      };
+      if (label >= lo && label < stop && threadIdx.x == 0 && is_allowed(w.allowed, label) && !touched(label))
+        own(l[r * l_rs + label]);
+      __syncwarp();
+      for (int j0 = first(lo); j0 < stop; j0 += kChunk) {
+        if (!loaded) load_all(j0, stop);
+        loaded = j0 + kChunk < stop;  // by the end of this chunk
+        float floor = best.v;  // the warp's best
 #pragma unroll
-      for (int i = 0; i < kVpt; ++i) {
-        const uint32_t at = (i * kThreads + threadIdx.x) * V;
-        const int j = mine + (int)at;
-        if (j >= n || (tab.wide && (int)(at >> (log_s - 1)) != s.side)) continue;
-        uint32_t bits = open_bits<V>(w.allowed, j, n);
-        if (touch) bits &= ~touched4(tab, at);
-        const uint32_t own = (uint32_t)label - (uint32_t)j;
-        if (own < V && (bits >> own & 1u)) {
-          answer(label, 0.0f, 0u, 0u);
-          bits &= ~(1u << own);
-        }
+        for (int off = 16; off > 0; off >>= 1) floor = fmaxf(floor, __shfl_xor_sync(0xffffffffu, floor, off));
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float v = t[i].v[e] != t[i].v[e] ? INFINITY : t[i].v[e];
-          if ((bits >> e & 1u) && v > best.v) best = Best{v, j + e};  // ascending: the lowest of equal ones
-        }
-      }
-      if (!touch) continue;
-      const uint32_t listed = *tab.listed;
-      uint32_t i, c, p;
-      if (listed <= kList) {
-        for (uint32_t k = threadIdx.x; k < listed; k += kThreads) {
-          if (!listed_entry(tab, k, i, c, p)) continue;
-          const int j = mine + (int)i;
-          if (allowed_bits<1>(w.allowed, j) & 1u) answer(j, x[j], c, p);
-        }
-      } else {  // many: entry by entry
-        for (i = threadIdx.x; i < 1u << log_s; i += kThreads) {
-          const int j = mine + (int)i;
-          if (j < 0 || j >= n || (tab.wide && (int)(i >> (log_s - 1)) != s.side)) continue;
-          look(tab, i, c, p);
-          if ((c | p) && (allowed_bits<1>(w.allowed, j) & 1u)) answer(j, x[j], c, p);
+        for (int i = 0; i < kVpt; ++i) {
+          const int j = j0 + (i * kMarginThreads + (int)threadIdx.x) * V;
+          if (j >= stop) break;
+          const Vec<float> a = t[i];
+          load(i, j0 + kChunk, stop);
+          const float top = max_nan(max_nan(a.v[0], a.v[1]), max_nan(a.v[2], a.v[3]));
+          if (top < floor) continue;
+          const uint32_t bits = open_bits<V>(w.allowed, j, n);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float v = a.v[e] != a.v[e] ? INFINITY : a.v[e];
+            if (v >= floor && (bits >> e & 1u) && j + e >= lo && j + e < stop && j + e != label && !touched(j + e))
+              take(best, v, j + e);
+          }
         }
       }
     }
-    if (span + 1 < spans) load(span + 1);
   }
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
@@ -505,15 +507,15 @@ __global__ void __launch_bounds__(kThreads, 3)
     const int32_t j = __shfl_xor_sync(0xffffffffu, best.j, off);
     take(best, v, j);
   }
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = best;
+  if ((threadIdx.x & 31) == 0) part_best[threadIdx.x >> 5] = best;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < (int)blockDim.x / 32; ++i) take(best, part[i].v, part[i].j);
+    for (int i = 1; i < kMarginThreads / 32; ++i) take(best, part_best[i].v, part_best[i].j);
     cl.map_shared_rank(joined, 0)[cl.block_rank()] = best;
   }
   cl.sync();
   if (cl.block_rank() == 0 && threadIdx.x == 0) {
-    for (int i = 0; i < (int)cl.num_blocks(); ++i) take(best, joined[i].v, joined[i].j);
+    for (int i = 0; i < nc; ++i) take(best, joined[i].v, joined[i].j);
     const bool any = best.v > -INFINITY;
     const float m = label_l - best.v;
     margin[r] = m != m ? -INFINITY : m;  // an infinite bound less itself says nothing
@@ -521,49 +523,39 @@ __global__ void __launch_bounds__(kThreads, 3)
   }
 }
 
-struct Shape {
-  int vpt, cluster, log_s, spans;
-  size_t smem;
-};
-
-// How a row's n answers are dealt out to slices of 256 vpt vectors of V answers.  A slice is as
-// large (up to 8192 answers) as still makes four CTAs an SM; `mis` answers of slack cover a row that
-// starts off a 16-byte boundary.  one_cluster: the whole row stays with one cluster (its results
-// are joined there).  Else a cluster shares the walk through histories that are long on average.
-constexpr int64_t kLongHistory = 1024;
-Shape shape_for(const cf_answer_rules& R, int V, int64_t mis, bool one_cluster) {
-  const int kMaxVpt = 32 / V;  // 8192 answers
-  Shape s;
-  const int64_t n = R.n + mis;
-  const bool hist = R.tokens_dev && R.n_tokens > 0, bias = R.bias_ids_dev && R.n_biases > 0;
-  s.vpt = 1;
-  while (s.vpt < kMaxVpt && ceil_div(n, (int64_t)kThreads * V * s.vpt * 2) * R.rows >= 148 * 4) s.vpt *= 2;
-  const int64_t slice = (int64_t)kThreads * V * s.vpt, slices = ceil_div(n, slice);
-  s.log_s = 0;
-  while (((int64_t)1 << s.log_s) < slice) ++s.log_s;
-  s.cluster = 1;
-  if (one_cluster || (hist && R.n_tokens / R.rows > kLongHistory))
-    while (s.cluster < kMaxCluster && s.cluster < slices) s.cluster *= 2;
-  s.spans = (int)ceil_div(slices, s.cluster);
-  s.smem = (hist || bias) ? (size_t)slice * (R.bias_ids_dev ? 4 : 2) + 16 + kList * 2 : 0;
-  return s;
+// ------------------------------------------------------------------------------ host
+bool has_edits(const cf_answer_rules& R) {
+  return (R.tokens_dev && R.n_tokens > 0) || (R.bias_ids_dev && R.n_biases > 0);
 }
 
 template <typename F, typename... Args>
-cf_status launch(const char* what, F* kern, const Shape& s, int64_t clusters, cudaStream_t st, Args... args) {
-  const int64_t blocks = clusters * s.cluster;
+cf_status launch(const char* what, F* kern, int64_t blocks, int threads, size_t smem, int cluster, bool dependent,
+                 cudaStream_t st, Args... args) {
   CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "%s: too many rows", what);
+  if (smem > 48 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = s.smem;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)s.cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (cluster > 0) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = (unsigned)cluster;
+    at[n].val.clusterDim.y = at[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  if (dependent) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = n;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
   if (e != cudaSuccess) {
     set_error("%s: %s", what, cudaGetErrorString(e));
@@ -576,8 +568,8 @@ cf_status check_rules(const cf_answer_rules* R, const char* what) {
   CF_REQUIRE(R, CF_ERR_NULL, "%s: NULL rules", what);
   CF_REQUIRE(R->rows >= 0 && R->n >= 0 && R->n_tokens >= 0 && R->n_biases >= 0 && R->n_masks >= 0, CF_ERR_SHAPE,
              "%s: negative size", what);
-  CF_REQUIRE(R->n <= 1 << 30 && R->n_tokens <= 1 << 30 && R->n_biases <= 1 << 30, CF_ERR_SHAPE,
-             "%s: at most 2^30 answers, tokens and biases", what);
+  CF_REQUIRE(R->n < 1 << 30 && R->n_tokens < 1 << 30 && R->n_biases < 1 << 30, CF_ERR_SHAPE,
+             "%s: fewer than 2^30 answers, tokens and biases", what);
   CF_REQUIRE((R->tokens_dev != nullptr) == (R->token_offsets_dev != nullptr), CF_ERR_NULL,
              "%s: tokens and their offsets go together", what);
   CF_REQUIRE(R->tokens_dev || (!R->prompt_len_dev && !R->repetition_dev && !R->frequency_dev && !R->presence_dev),
@@ -599,15 +591,24 @@ cf_status check_rules(const cf_answer_rules* R, const char* what) {
 template <typename T>
 cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, void* out, int64_t out_rs,
                       cudaStream_t st) {
+  constexpr int V = Vec<T>::N, kChunk = kStreamThreads * kUnroll * V;
   CF_REQUIRE(((uintptr_t)in | (uintptr_t)out) % sizeof(T) == 0, CF_ERR_SHAPE, "edit_logits: unaligned rows");
-  const bool flat = (uintptr_t)in % 16 == 0 && (R.rows == 1 || in_rs * sizeof(T) % 16 == 0);
-  const Shape s = shape_for(R, Vec<T>::N, flat ? 0 : Vec<T>::N - 1, false);
-  auto* kern = s.vpt == 1   ? k_edit_logits<T, 1>
-               : s.vpt == 2 ? k_edit_logits<T, 2>
-               : s.vpt == 4 ? k_edit_logits<T, 4>
-                            : k_edit_logits<T, 32 / Vec<T>::N>;
-  return launch("k_edit_logits", kern, s, R.rows * s.spans, st, R, (const T*)in, in_rs, (T*)out, out_rs, s.log_s,
-                s.spans);
+  if (R.rows == 1) in_rs = out_rs;
+  const bool stream = in != out || in_rs != out_rs || R.allowed_dev;
+  if (stream) {
+    const int chunks = (int)ceil_div(R.n + V - 1, kChunk);
+    const int64_t units = R.rows * chunks, most = 148 * 4;  // four CTAs an SM
+    CF_TRY(launch("k_answer_stream", k_answer_stream<T>, units < most ? units : most, kStreamThreads, 0, 0, false, st,
+                  R, (const T*)in, in_rs, (T*)out, out_rs, chunks, units));
+  }
+  if (!has_edits(R)) return CF_OK;
+  // 32768 answers a slice (64 KB of tables, three CTAs an SM), fewer where that leaves SMs idle
+  int log_s = 15;
+  while (log_s > 11 && R.rows * ceil_div(R.n, (int64_t)1 << log_s) < 148) --log_s;
+  while (log_s > 11 && (int64_t)1 << (log_s - 1) >= R.n) --log_s;
+  const int slices = (int)ceil_div(R.n, (int64_t)1 << log_s);
+  return launch("k_answer_edits", k_answer_edits<T>, R.rows * slices, kEditThreads, tables_bytes(log_s), 0, stream, st,
+                R, (const T*)in, in_rs, (T*)out, out_rs, log_s, slices);
 }
 
 }  // namespace
@@ -622,6 +623,7 @@ extern "C" cf_status cf_edit_logits(const cf_answer_rules* R, int32_t dtype, con
   CF_TRY(check_rules(R, "edit_logits"));
   CF_REQUIRE(in_rs >= 0 && (R->rows <= 1 || out_rs >= R->n), CF_ERR_SHAPE, "edit_logits: rows of %lld overlap",
              (long long)R->n);
+  CF_REQUIRE(in != out || R->rows <= 1 || in_rs == out_rs, CF_ERR_SHAPE, "edit_logits: rows change places");
   CF_REQUIRE(dtype == CF_F32 || dtype == CF_BF16 || dtype == CF_F16, CF_ERR_UNSUPPORTED, "edit_logits: dtype %d",
              dtype);
   if (R->rows * R->n == 0) return CF_OK;
@@ -642,12 +644,15 @@ extern "C" cf_status cf_answer_margin(const cf_answer_rules* R, const float* l, 
   if (R->rows == 0) return CF_OK;
   CF_REQUIRE(l && u && labels && margin && rival, CF_ERR_NULL, "answer_margin: NULL argument");
   CF_REQUIRE(((uintptr_t)l | (uintptr_t)u) % 4 == 0, CF_ERR_SHAPE, "answer_margin: unaligned rows");
-  const bool flat = (uintptr_t)u % 16 == 0 && (R->rows == 1 || u_rs % 4 == 0);
-  const Shape s = shape_for(*R, 4, flat ? 0 : 3, true);
-  auto* kern = s.vpt == 1   ? k_answer_margin<1>
-               : s.vpt == 2 ? k_answer_margin<2>
-               : s.vpt == 4 ? k_answer_margin<4>
-                            : k_answer_margin<8>;
-  return launch("k_answer_margin", kern, s, R->rows, as_stream(stream), *R, l, l_rs, u, u_rs, labels, margin, rival,
-                s.log_s, s.spans);
+  // 16384 answers a slice, fewer for a short row or few rows; a cluster of up to eight for a row
+  int log_s = 14;
+  while (log_s > 11 && ((int64_t)1 << (log_s - 1) >= R->n ||
+                        (R->rows * ceil_div(R->n, (int64_t)1 << log_s) < 148 && (int64_t)8 << (log_s - 1) >= R->n)))
+    --log_s;
+  const int slices = (int)ceil_div(R->n, (int64_t)1 << log_s);
+  int cluster = 1;
+  while (cluster < kMaxCluster && cluster < slices) cluster *= 2;
+  return launch("k_answer_margin", k_answer_margin, R->rows * cluster, kMarginThreads,
+                has_edits(*R) ? tables_bytes(log_s) : 0, cluster, false, as_stream(stream), *R, l, l_rs, u, u_rs,
+                labels, margin, rival, log_s, slices);
 }

@@ -453,7 +453,7 @@ cf_status cf_adapter_check(void* stream);
  *   v = x; j in the history: v = v > 0 ? v / repetition : v * repetition; answered c > 0 times:
  *   v = v - frequency * c, v = v - presence; j has a bias: v = v + bias; not allowed: -inf.
  * Tokens and ids outside 0 .. n-1 are ignored, and offsets are held within their lists; n,
- * n_tokens and n_biases are at most 2^30.  With
+ * n_tokens and n_biases are below 2^30.  With
  * repetition > 0 every step is monotone: the edited bounds of a logit bound the edited logit. */
 typedef struct cf_answer_rules {
   int64_t rows, n;
