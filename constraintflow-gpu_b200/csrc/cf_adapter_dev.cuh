@@ -28,6 +28,31 @@ struct Kind<__half> {
   static constexpr int kStep = 64, kPlanes = 1, kAb = 0;
 };
 
+// Loads that stay where they are written, zeros where not `ok`: a thread has two steps' loads in
+// flight, and neither a move of them to their uses nor a selection behind them may wait for one.
+__device__ __forceinline__ uint4 ldg16_if(const void* p, bool ok) {
+  uint4 v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+      : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w)
+      : "l"(p), "r"((int)ok));
+  return v;
+}
+__device__ __forceinline__ uint32_t ldg4_if(const void* p, bool ok) {
+  uint32_t v;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %2, 0;\n\t"
+      "mov.b32 %0, 0;\n\t"
+      "@p ld.global.u32 %0, [%1];\n\t}"
+      : "=&r"(v)
+      : "l"(p), "r"((int)ok));
+  return v;
+}
+
 // 16 bytes of row `row` (elements k .. of n_k), zero beyond
 template <typename T>
 __device__ __forceinline__ uint4 load16(const T* row, int64_t k, int64_t n_k, bool vec) {

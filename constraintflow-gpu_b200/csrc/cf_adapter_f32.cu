@@ -22,6 +22,8 @@
 // parts in rank order.
 #include <cooperative_groups.h>
 
+#include <type_traits>
+
 #include "cf_adapter_dev.cuh"
 
 namespace cg = cooperative_groups;
@@ -34,13 +36,25 @@ using namespace tc;
 
 constexpr int kDrain = 256, kLoad = 256;  // threads of the two groups
 constexpr int kMmaWarp = 16;
-constexpr int kThreads = 544;
+constexpr int kThreads = 640;  // five warpgroups; warps 17-19 idle
+// Registers a thread: 96 at launch (640 x 96 = 61440).  The drain holds 64 sums and the loads two
+// steps of chunks, so they take what the MMA group gives up: 128 (2 x 104 + 2 x 112 + 40) = 60416.
+constexpr int kDrainRegs = 104, kLoadRegs = 112, kMmaRegs = 40;
 constexpr int kStep = 32;   // contraction of a stage: 128 bytes
 constexpr int kChunk = 2;   // steps of one accumulation
 constexpr int kStages = 2, kBufs = 2;
 
 // A bounded wait that gave up leaves its site here (cf_adapter_check).
 __device__ int g_err;
+
+template <int kRegs>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
 
 struct Tiling {
   int64_t m_tiles, units, clusters;  // clusters: on tiles; behind them, clusters that plan row tiles
@@ -148,47 +162,68 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
   const int kb = (int)((int64_t)n_k * rank / split), ke = (int)((int64_t)n_k * (rank + 1) / split);
   // the requests' low-rank parts as chunks
   const bool lowrank = !kShrink && p.R > 0 && !g.rowwise && rank == 0;
+  Tile w = {};
+  // v up to the adapter's rank, and zeros up to the next multiple of 4
+  auto put_v = [&](int64_t t, int r, float v) {
+    if (r < (w.e_rank + 3) / 4 * 4) store_v(p, t, r, r < w.e_rank ? v : 0.0f);
+  };
   bool waited = !g.dependent;
   bool ok = true;
-  Tile w = {};
 
   if (warp >= 8 && warp < kMmaWarp) {
     // ---------------------------------------------------------------- loads
+    more_registers<kLoadRegs>();
     const int tid = threadIdx.x - kDrain, chunk = tid & 7, prow = tid >> 3;
     int it = 0;
-    auto fetch_x = [&](uint4(&d)[kBM * 8 / kLoad], const float* x, int64_t rs, int64_t t0, int64_t k, int64_t n_kk,
-                       bool vec) {
-#pragma unroll
-      for (int j = 0; j < kBM * 8 / kLoad; ++j) {
-        const int64_t t = t0 + prow + j * (kLoad / 8);
-        d[j] = t < p.T ? load16<float>(x + t * rs, k + chunk * 4, n_kk, vec) : make_uint4(0, 0, 0, 0);
+    // four elements of a row with contiguous k from k on, of n_kk; vec: 16-byte aligned, n_kk a
+    // multiple of 4
+    auto row4 = [&](auto vec, const float* row, int k, int n_kk, bool ok) -> uint4 {
+      if constexpr (decltype(vec)::value) {
+        return ldg16_if(row + k, ok && k < n_kk);
+      } else {
+        uint4 d;
+        d.x = ldg4_if(row + k, ok && k < n_kk);
+        d.y = ldg4_if(row + k + 1, ok && k + 1 < n_kk);
+        d.z = ldg4_if(row + k + 2, ok && k + 2 < n_kk);
+        d.w = ldg4_if(row + k + 3, ok && k + 3 < n_kk);
+        return d;
       }
     };
-    auto fetch_b = [&](uint4(&d)[kBN * 8 / kLoad], const float* B, int64_t ks, int64_t ns, int64_t c0, int64_t n_c,
-                       int64_t k0, int64_t n_kk, bool vec) {
+    auto fetch_x = [&](auto vec, uint4(&d)[kBM * 8 / kLoad], const float* x, int64_t rs, int k, int n_kk) {
+      const float* row = x + (w.t0 + prow) * rs;
+      const int rows = (int)min(p.T - w.t0, (int64_t)kBM);
+#pragma unroll
+      for (int j = 0; j < kBM * 8 / kLoad; ++j)
+        d[j] = row4(vec, row + j * (kLoad / 8) * rs, k + chunk * 4, n_kk, prow + j * (kLoad / 8) < rows);
+    };
+    // columns [0, n_c) of B, contraction k .. of n_kk
+    auto fetch_b = [&](auto vec, uint4(&d)[kBN * 8 / kLoad], const float* B, int64_t ks, int64_t ns, int n_c, int k,
+                       int n_kk) {
 #pragma unroll
       for (int j = 0; j < kBN * 8 / kLoad; ++j) {
         if constexpr (kSub) {  // columns contiguous: consecutive threads, consecutive columns
-          const int task = j * kLoad + tid;
-          const int64_t c = c0 + task % kBN, k = k0 + task / kBN * 4;
-          float f[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) f[i] = c < n_c && k + i < n_kk ? B[(k + i) * ks + c * ns] : 0.0f;
-          d[j] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                            __float_as_uint(f[3]));
+          const int task = j * kLoad + tid, c = task % kBN, kk = k + task / kBN * 4;
+          const float* at = B + kk * ks + c;
+          const bool ok = c < n_c;
+          d[j].x = ldg4_if(at, ok && kk < n_kk);
+          d[j].y = ldg4_if(at + ks, ok && kk + 1 < n_kk);
+          d[j].z = ldg4_if(at + 2 * ks, ok && kk + 2 < n_kk);
+          d[j].w = ldg4_if(at + 3 * ks, ok && kk + 3 < n_kk);
         } else {
-          const int64_t c = c0 + prow + j * (kLoad / 8);
-          d[j] = c < n_c ? load16<float>(B + c * ns, k0 + chunk * 4, n_kk, vec) : make_uint4(0, 0, 0, 0);
+          const int c = prow + j * (kLoad / 8);
+          d[j] = row4(vec, B + c * ns, k + chunk * 4, n_kk, c < n_c);
         }
       }
     };
-    auto fetch = [&](Chunks<kBN>& d, int k) {
-      fetch_x(d.x, (const float*)p.x, p.x_rs, w.t0, (int64_t)k * kStep, p.K, p.x_vec);
+    const int K = (int)p.K;
+    auto fetch = [&](auto vec, Chunks<kBN>& d, int k) {
+      fetch_x(vec, d.x, (const float*)p.x, p.x_rs, k * kStep, K);
       if constexpr (kShrink)
-        fetch_b(d.b, (const float*)p.P + w.e * p.p_es, p.p_ks, p.p_rs, w.r0, w.e_rank, (int64_t)k * kStep, p.K,
-                p.p_vec);
+        fetch_b(vec, d.b, (const float*)p.P + w.e * p.p_es + w.r0 * p.p_rs, p.p_ks, p.p_rs, w.e_rank - w.r0, k * kStep,
+                K);
       else
-        fetch_b(d.b, (const float*)p.M, p.m_ks, p.m_ns, w.n0, p.N, (int64_t)k * kStep, p.K, p.m_vec);
+        fetch_b(vec, d.b, (const float*)p.M + w.n0 * p.m_ns, p.m_ks, p.m_ns, (int)min(p.N - w.n0, (int64_t)kBN),
+                k * kStep, K);
     };
     auto store = [&](const Chunks<kBN>& d) -> bool {
       const int s = it % kStages, round = it / kStages;
@@ -210,33 +245,43 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       ++it;
       return true;
     };
-    for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
-      if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
-      Chunks<kBN> one, two;
-      if (kb < ke) fetch(one, kb);
-      for (int k = kb; k < ke && ok; k += 2) {
-        if (k + 1 < ke) fetch(two, k + 1);
-        ok = store(one);
-        if (!ok || k + 1 >= ke) break;
-        if (k + 2 < ke) fetch(one, k + 2);
-        ok = store(two);
+    auto tiles = [&](auto vec) {
+      for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
+        if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
+        Chunks<kBN> one, two;
+        if (kb < ke) fetch(vec, one, kb);
+        for (int k = kb; k < ke && ok; k += 2) {
+          if (k + 1 < ke) fetch(vec, two, k + 1);
+          ok = store(one);
+          if (!ok || k + 1 >= ke) break;
+          if (k + 2 < ke) fetch(vec, one, k + 2);
+          ok = store(two);
+        }
+        if (lowrank && ok) {
+          if (!waited) dependency_wait();
+          waited = true;
+          ok = for_requests(p, w.m, p.tile_q[w.m], [&](int e, int r, int, int) {
+            for (int r0 = 0; r0 < r; r0 += kStep) {
+              // rows of v are 16-byte aligned and zero from the rank to the next multiple of 4
+              fetch_x(std::true_type{}, one.x, p.v, p.v_rs, r0, r);
+              fetch_b(std::false_type{}, one.b, (const float*)p.Qm + e * p.q_es + w.n0 * p.q_ns, p.q_rs, p.q_ns,
+                      (int)min(p.N - w.n0, (int64_t)kBN), r0, r);
+              if (!store(one)) return false;
+            }
+            return true;
+          });
+        }
       }
-      if (lowrank && ok) {
-        if (!waited) dependency_wait();
-        waited = true;
-        ok = for_requests(p, w.m, p.tile_q[w.m], [&](int e, int r, int, int) {
-          for (int r0 = 0; r0 < r; r0 += kStep) {
-            // rows of v are 16-byte aligned, v_rs a multiple of 8; beyond the rank: zeros
-            fetch_x(one.x, p.v, p.v_rs, w.t0, r0, r, true);
-            fetch_b(one.b, (const float*)p.Qm + e * p.q_es, p.q_rs, p.q_ns, w.n0, p.N, r0, r, p.q_vec);
-            if (!store(one)) return false;
-          }
-          return true;
-        });
-      }
-    }
-  } else if (warp == kMmaWarp) {
+    };
+    const bool vec = p.x_vec && (kShrink ? p.p_vec : p.m_vec) && p.K % 4 == 0;
+    if (vec || (kSub && p.x_vec && p.K % 4 == 0))
+      tiles(std::true_type{});
+    else
+      tiles(std::false_type{});
+  } else if (warp >= kMmaWarp) {
     // ---------------------------------------------------------------- MMAs
+    fewer_registers<kMmaRegs>();
+    if (warp == kMmaWarp) {
     int it = 0, ch = 0;
     // one step into chunk ch; first / last of its chunk
     auto step = [&](int mmas, bool first, bool last, uint32_t id) -> bool {
@@ -278,8 +323,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     }
     if (lane == 0) mma_commit(&bars.done);
     mbar_wait_drain(&bars.done, 0, err, 63);  // every MMA has run before tensor memory is given up
-  } else if (warp < 8) {
+    }
+  } else {
     // ---------------------------------------------------------------- chunks, tiles
+    more_registers<kDrainRegs>();
     const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (kBN / 2);
     const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
     int ch = 0;
@@ -339,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
           const int r = a + i / quads, c = i % quads * 4;
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            if (w.r0 + c + j < w.e_rank) store_v(p, w.t0 + r, w.r0 + c + j, scale * part[r * kLd + c + j]);
+            put_v(w.t0 + r, w.r0 + c + j, scale * part[r * kLd + c + j]);
         }
       } else {
         const int64_t n = w.n0 + lane * 4;
@@ -391,8 +438,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
         const float4 s = sum4(r, c);
         const float v[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (w.r0 + c + j < w.e_rank) store_v(p, w.t0 + r, w.r0 + c + j, scale * v[j]);
+        for (int j = 0; j < 4; ++j) put_v(w.t0 + r, w.r0 + c + j, scale * v[j]);
       }
     } else {
       const int rows = (int)min((int64_t)kBM, p.T - w.t0);
