@@ -7,7 +7,6 @@ cf_edit_logits, cf_answer_margin).
 Operands are CUDA tensors, possibly broadcast views (zero strides); results are new
 contiguous tensors.  PyTorch only allocates the memory and supplies the stream.
 """
-import contextlib
 import ctypes
 import operator
 
@@ -227,17 +226,18 @@ def _row_stride(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-_HERE = contextlib.nullcontext()
+def _plain(t, dtype, gpu, shape):
+    """A contiguous tensor as expected; anything else goes through _expect, which says why not."""
+    return t.dtype is dtype and t.get_device() == gpu and t.shape == shape and t.is_contiguous()
 
 
-def _on(dev):
-    """dev as the current device, for a launch."""
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _raw_stream(dev):
-    """The handle of the current stream of dev."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _launch(gpu, fn, *args):
+    """fn(*args, stream): a libcfgpu call on the current stream of that GPU, made the current device
+    where it is not."""
+    if gpu == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
+    with torch.cuda.device(gpu):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
 
 
 class AdapterLayer:
@@ -267,7 +267,8 @@ class AdapterLayer:
             _expect("ranks", ranks, torch.int32, (self.n_adapters,), dev)
         if bias is not None:
             _expect("bias", bias, dt, (self.n_out,), dev)
-        self.device, self.dtype = dev, dt
+        self.device, self.dtype, self.gpu = dev, dt, dev.index
+        self._need = {}           # workspace bytes by (substitute, T, n_requests)
         self._keep = (W, A, B, scale, ranks, bias)
 
         def strides(t):
@@ -291,26 +292,31 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
     ids [n_requests] int32: its adapter, any value outside 0 .. n_adapters-1 none.  Both are
     read on the device, without a synchronisation.  Rows of no request are left as they were in
     `out`, and are 0 in a new result.  `out` must not overlap x."""
-    dev = layer.device
+    dev, gpu, dt = layer.device, layer.gpu, layer.dtype
     K, N = (layer.n_out, layer.n_in) if substitute else (layer.n_in, layer.n_out)
-    if x.stride(-1) != 1:
+    if x.dim() == 2 and x.stride(1) != 1:
         x = x.contiguous()
-    _expect("x", x, layer.dtype, (None, K), dev, strided=True)
-    T, Q = int(x.shape[0]), int(ids.shape[0])
-    _expect("offsets", offsets, torch.int64, (Q + 1,), dev)
-    _expect("ids", ids, torch.int32, (None,), dev)
-    if out is not None:
-        _expect("out", out, layer.dtype, (T, N), dev, strided=True)
-    with _on(dev):
-        if out is None:
-            out = torch.zeros(T, N, dtype=layer.dtype, device=dev)
-        need = _lib.lib.cf_adapter_workspace_bytes(layer._ref, int(substitute), T, Q)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
-        st = _lib.lib.cf_adapter_matmul(layer._ref, int(substitute), T, x.data_ptr(), _row_stride(x), Q,
-                                        offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out),
-                                        ws.data_ptr(), need, _raw_stream(dev))
-    _lib.check(st, "cf_adapter_matmul")
+    T, Q = x.shape[0], ids.shape[0]
+    if not _plain(x, dt, gpu, (T, K)):
+        _expect("x", x, dt, (None, K), dev, strided=True)
+    if not _plain(offsets, torch.int64, gpu, (Q + 1,)):
+        _expect("offsets", offsets, torch.int64, (Q + 1,), dev)
+    if not _plain(ids, torch.int32, gpu, (Q,)):
+        _expect("ids", ids, torch.int32, (None,), dev)
+    if out is None:
+        out = torch.zeros(T, N, dtype=dt, device=dev)
+    elif not _plain(out, dt, gpu, (T, N)):
+        _expect("out", out, dt, (T, N), dev, strided=True)
+    key = (substitute, T, Q)
+    need = layer._need.get(key)
+    if need is None:
+        need = layer._need[key] = _lib.lib.cf_adapter_workspace_bytes(layer._ref, 1 if substitute else 0, T, Q)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
+    st = _launch(gpu, _lib.lib.cf_adapter_matmul, layer._ref, 1 if substitute else 0, T, x.data_ptr(), _row_stride(x), Q,
+                 offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out), ws.data_ptr(), need)
+    if st:
+        _lib.check(st, "cf_adapter_matmul")
     return out
 
 
@@ -370,33 +376,37 @@ class AnswerRules:
                                     0 if allowed is None else int(allowed.shape[1]), count["allowed"], 0,
                                     *[_ptr(t) for t in given.values()])
         self._ref = ctypes.byref(self.c)
+        self.launches = 1 + (count["tokens"] + count["bias_ids"] > 0)   # the stream, the edits
 
 
-def _rules_rows(name, t, rules, dtype):
-    dev = _cuda(name, t)
-    if rules.device is not None and dev != rules.device:
-        raise Exception(f"SHAPE MISMATCH: {name} is on {dev}, the rules are on {rules.device}")
-    if t.stride(-1) != 1:
+def _rules_rows(name, t, rules, dtype, gpu):
+    """t as rows for the rules: [rows, n] of `dtype` on `gpu`, its last dimension contiguous."""
+    if rules.device is not None and gpu != rules.device.index:
+        raise Exception(f"SHAPE MISMATCH: {name} is on GPU {gpu}, the rules are on {rules.device}")
+    if t.dim() == 2 and t.stride(1) != 1:
         t = t.contiguous()
-    _expect(name, t, dtype, (rules.rows, rules.n), dev, strided=True)
-    return t, dev
+    if not _plain(t, dtype, gpu, (rules.rows, rules.n)):
+        _expect(name, t, dtype, (rules.rows, rules.n), torch.device("cuda", gpu), strided=True)
+    return t
 
 
 def edit_logits(logits, rules, out=None):
     """The rules applied to logits [rows, n] (float32, bfloat16, float16), in float32, rounded
     once to the logits' dtype; `out` may be the logits themselves."""
-    if logits.dtype not in _DTYPES:
-        raise NotImplementedError(f"logits of {logits.dtype} (float32, bfloat16 and float16 are supported)")
-    x, dev = _rules_rows("logits", logits, rules, logits.dtype)
+    dt = logits.dtype
+    if dt not in _DTYPES:
+        raise NotImplementedError(f"logits of {dt} (float32, bfloat16 and float16 are supported)")
+    gpu = _cuda("logits", logits).index
+    x = _rules_rows("logits", logits, rules, dt, gpu)
     if out is None:
-        out = torch.empty(rules.rows, rules.n, dtype=x.dtype, device=dev)
-    else:
-        _expect("out", out, x.dtype, (rules.rows, rules.n), dev, strided=True)
-    with _on(dev):
-        LAUNCHES[0] += 1
-        st = _lib.lib.cf_edit_logits(rules._ref, _DTYPES[x.dtype], x.data_ptr(), _row_stride(x), out.data_ptr(),
-                                     _row_stride(out), _raw_stream(dev))
-    _lib.check(st, "cf_edit_logits")
+        out = torch.empty(rules.rows, rules.n, dtype=dt, device=x.device)
+    elif not _plain(out, dt, gpu, (rules.rows, rules.n)):
+        _expect("out", out, dt, (rules.rows, rules.n), x.device, strided=True)
+    LAUNCHES[0] += rules.launches
+    st = _launch(gpu, _lib.lib.cf_edit_logits, rules._ref, _DTYPES[dt], x.data_ptr(), _row_stride(x), out.data_ptr(),
+                 _row_stride(out))
+    if st:
+        _lib.check(st, "cf_edit_logits")
     return out
 
 
@@ -406,16 +416,17 @@ def answer_margin(l, u, labels, rules):
     the best edited upper bound among the other answers (> 0: the answer is the label), and
     rival [rows] int32, that other answer (the lowest on equal bounds, -1: none is left).
     A label that is not allowed has margin -inf; a bound that is NaN bounds nothing."""
-    l, dev = _rules_rows("l", l, rules, torch.float32)
-    u, udev = _rules_rows("u", u, rules, torch.float32)
-    if udev != dev:
-        raise Exception(f"SHAPE MISMATCH: l is on {dev}, u on {udev}")
-    _expect("labels", labels, torch.int64, (rules.rows,), dev)
+    dev = _cuda("l", l)
+    gpu = dev.index
+    l = _rules_rows("l", l, rules, torch.float32, gpu)
+    u = _rules_rows("u", u, rules, torch.float32, gpu)
+    if not _plain(labels, torch.int64, gpu, (rules.rows,)):
+        _expect("labels", labels, torch.int64, (rules.rows,), dev)
     margin = torch.empty(rules.rows, dtype=torch.float32, device=dev)
     rival = torch.empty(rules.rows, dtype=torch.int32, device=dev)
-    with _on(dev):
-        LAUNCHES[0] += 1
-        st = _lib.lib.cf_answer_margin(rules._ref, l.data_ptr(), _row_stride(l), u.data_ptr(), _row_stride(u),
-                                       labels.data_ptr(), margin.data_ptr(), rival.data_ptr(), _raw_stream(dev))
-    _lib.check(st, "cf_answer_margin")
+    LAUNCHES[0] += 1
+    st = _launch(gpu, _lib.lib.cf_answer_margin, rules._ref, l.data_ptr(), _row_stride(l), u.data_ptr(), _row_stride(u),
+                 labels.data_ptr(), margin.data_ptr(), rival.data_ptr())
+    if st:
+        _lib.check(st, "cf_answer_margin")
     return margin, rival

@@ -53,6 +53,29 @@ __device__ __forceinline__ int64_t request_of(const Problem& p, int64_t t) {
   return lo;
 }
 
+// Whether row t is some request's.
+__device__ __forceinline__ bool is_owned(const Problem& p, int64_t t) {
+  return t >= p.offsets[0] && t < p.offsets[p.Q];
+}
+
+// The first index in [lo, hi) at which `pred`, false up to some point and true from there on, is
+// true, else hi.  A warp together: 32 places a turn, where a binary search would wait for one
+// load after the other.
+template <typename F>
+__device__ __forceinline__ int64_t warp_search(int64_t lo, int64_t hi, F&& pred) {
+  const int lane = threadIdx.x & 31;
+  while (lo < hi) {
+    const int64_t step = (hi - lo + 31) / 32, at = lo + (lane + 1) * step - 1;
+    const uint32_t found = __ballot_sync(0xffffffffu, at >= hi - 1 ? at < hi + step && pred(hi - 1) : pred(at));
+    if (!found) return hi;  // the last lane in range tried hi - 1
+    const int first = __ffs(found) - 1;
+    hi = min(lo + (first + 1) * step - 1, hi - 1);
+    lo = lo + first * step;
+    if (step == 1) return hi;
+  }
+  return lo;
+}
+
 __device__ __forceinline__ int adapter_of(const Problem& p, int64_t q) {
   if (q < 0) return kNone;
   const int e = p.ids[q];
@@ -64,36 +87,47 @@ __device__ __forceinline__ int rank_of(const Problem& p, int e) {
   return p.ranks ? min(max(p.ranks[e], 0), p.R) : p.R;
 }
 
-// f(adapter, rank, first row, end row) for the requests with an adapter that reach into row tile
-// m, in order, from request `from` on (the first that ends behind the tile's start); a warp
-// together, every lane with the same arguments.  f returns false to stop.
-template <typename F>
-__device__ __forceinline__ bool for_requests(const Problem& p, int64_t m, int64_t from, F&& f) {
-  const int lane = threadIdx.x & 31;
-  const int64_t t0 = m * kBM, t1 = min(t0 + kBM, p.T);
-  for (int64_t base = from; base < p.Q; base += 32) {
-    const int64_t q = base + lane;
-    int a = 0, b = 0, e = kNone, r = 0;
-    bool past = true;
-    if (q < p.Q) {
-      const int64_t o0 = p.offsets[q], o1 = p.offsets[q + 1];
-      past = o0 >= t1;
-      a = (int)(max(o0, t0) - t0);
-      b = (int)(max(min(o1, t1), t0) - t0);
-      if (!past && a < b) {
-        e = adapter_of(p, q);
-        r = rank_of(p, e);
-      }
+// A lane's request of 32 that may reach into a row tile: its adapter and rank (0: none, or no row of
+// the tile) and its rows [a, b) of the tile.
+struct Reach {
+  int e, r, a, b;
+  bool past;  // this request and those behind it start behind the tile
+};
+
+__device__ __forceinline__ Reach reach(const Problem& p, int64_t m, int64_t base) {
+  const int64_t t0 = m * kBM, t1 = min(t0 + kBM, p.T), q = base + (threadIdx.x & 31);
+  Reach w{kNone, 0, 0, 0, true};
+  if (q < p.Q) {
+    const int64_t o0 = p.offsets[q], o1 = p.offsets[q + 1];
+    const int e = adapter_of(p, q);
+    w.past = o0 >= t1;
+    w.a = (int)(max(o0, t0) - t0);
+    w.b = (int)(max(min(o1, t1), t0) - t0);
+    if (!w.past && w.a < w.b) {
+      w.e = e;
+      w.r = rank_of(p, e);
     }
-    for (uint32_t todo = __ballot_sync(0xffffffffu, r > 0); todo; todo &= todo - 1) {
+  }
+  return w;
+}
+
+// f(adapter, rank, first row, end row) for the requests with an adapter that reach into row tile
+// m, in order, from request `from` on (the first that ends behind the tile's start; `w`: its and
+// the next 31's reach); a warp together, every lane with the same arguments.  f returns false to
+// stop.
+template <typename F>
+__device__ __forceinline__ bool for_requests(const Problem& p, int64_t m, int64_t from, Reach w, F&& f) {
+  for (;;) {
+    for (uint32_t todo = __ballot_sync(0xffffffffu, w.r > 0); todo; todo &= todo - 1) {
       const int i = __ffs(todo) - 1;
-      if (!f(__shfl_sync(0xffffffffu, e, i), __shfl_sync(0xffffffffu, r, i), __shfl_sync(0xffffffffu, a, i),
-             __shfl_sync(0xffffffffu, b, i)))
+      if (!f(__shfl_sync(0xffffffffu, w.e, i), __shfl_sync(0xffffffffu, w.r, i), __shfl_sync(0xffffffffu, w.a, i),
+             __shfl_sync(0xffffffffu, w.b, i)))
         return false;
     }
-    if (__any_sync(0xffffffffu, past)) break;
+    if (__any_sync(0xffffffffu, w.past)) return true;
+    from += 32;
+    w = reach(p, m, from);
   }
-  return true;
 }
 
 // tile_e and tile_q of row tile m, by one warp.  One adapter for all of the tile's rows can be added by the
@@ -102,18 +136,12 @@ __device__ __forceinline__ bool for_requests(const Problem& p, int64_t m, int64_
 // cores take are R and the multiples of `whole` (0: none), so that nothing beyond an adapter's
 // own rank is multiplied.
 __device__ __forceinline__ void plan_tile(const Problem& p, int64_t m, int whole) {
-  int64_t from = 0, b = p.Q;  // the first request that ends behind the tile's start
-  while (from < b) {
-    const int64_t mid = (from + b) / 2;
-    if (p.offsets[mid + 1] > m * kBM)
-      b = mid;
-    else
-      from = mid + 1;
-  }
+  // the first request that ends behind the tile's start
+  const int64_t from = warp_search(0, p.Q, [&](int64_t q) { return p.offsets[q + 1] > m * kBM; });
   int first = kNone, requests = 0;
   int64_t rows = 0;
   bool one = true, fit = true;
-  for_requests(p, m, from, [&](int e, int r, int a, int b) {
+  for_requests(p, m, from, reach(p, m, from), [&](int e, int r, int a, int b) {
     if (requests == 0) first = e;
     one &= e == first;
     fit &= whole > 0 && (r == p.R || r % whole == 0);

@@ -223,12 +223,14 @@ inline cf_status take_site(int* symbol, int* site, cudaStream_t st) {
   return CF_OK;
 }
 
-// CTAs of a cluster: as many as keep the grid within two waves of single CTAs, each with at
-// least four steps of the contraction.
+// CTAs of a cluster that share a tile's contraction, at least four steps each: as many as still
+// have an SM to themselves.  Clusters do not pack the GPU's processor clusters fully, so 128 CTAs
+// count as full and 64 in clusters of eight (4096 x 4096 for one token, 32 tiles: 11.1 us with 4,
+// 12.9 with 3, 15.5 with 5, 17.0 with 8; 16 tiles: 10.5 with 6, 13.7 with 8).
 inline int split_for(int64_t tiles, int64_t steps) {
-  int s = 1;
-  while (s < 8 && tiles * s * 2 <= 2 * 148 && steps >= s * 2 * 4) s *= 2;
-  return s;
+  for (int s : {8, 6, 4, 3, 2})
+    if (tiles * s <= (s == 8 ? 64 : 128) && steps >= s * 4) return s;
+  return 1;
 }
 
 }  // namespace adapter

@@ -37,9 +37,9 @@ using namespace tc;
 constexpr int kDrain = 256, kLoad = 256;  // threads of the two groups
 constexpr int kMmaWarp = 16;
 constexpr int kThreads = 640;  // five warpgroups; warps 17-19 idle
-// Registers a thread: 96 at launch (640 x 96 = 61440).  The drain holds 64 sums and the loads two
-// steps of chunks, so they take what the MMA group gives up: 128 (2 x 104 + 2 x 112 + 40) = 60416.
-constexpr int kDrainRegs = 104, kLoadRegs = 112, kMmaRegs = 40;
+// Registers a thread: 96 at launch (640 x 96 = 61440).  The loads hold two steps of chunks and take
+// what the MMA group gives up: 128 (2 x 96 + 2 x 112 + 64) = 61440.
+constexpr int kLoadRegs = 112, kMmaRegs = 64;
 constexpr int kStep = 32;   // contraction of a stage: 128 bytes
 constexpr int kChunk = 2;   // steps of one accumulation
 constexpr int kStages = 2, kBufs = 2;
@@ -64,11 +64,11 @@ struct Tiling {
 };
 
 struct Tile {
-  int64_t m, t0, n0, row0, row1;  // shrink: rows [row0, row1)
-  int e, e_rank, r0, cols;
+  int32_t m, t0, n0, row0, row1;  // shrink: rows [row0, row1) of the tile
+  int32_t e, e_rank, r0, cols;
 };
 
-// The tile of a unit; false: nothing to do.
+// The tile of a unit, by a warp together; false: nothing to do.
 template <bool kShrink, int kBN>
 __device__ __forceinline__ bool tile_of(const Problem& p, const Tiling& g, int64_t unit, Tile& w) {
   w.n0 = w.row0 = w.row1 = 0;
@@ -78,26 +78,22 @@ __device__ __forceinline__ bool tile_of(const Problem& p, const Tiling& g, int64
     w.r0 = (int)(unit - u * blocks_r) * kBN;
     // tile + request numbers the overlapping (tile, request) pairs; request q of unit u is the
     // first that ends behind tile u - q's start
-    int64_t lo = 0, hi = p.Q;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (p.offsets[mid + 1] + kBM * mid > kBM * u)
-        hi = mid;
-      else
-        lo = mid + 1;
-    }
+    const int64_t lo = warp_search(0, p.Q, [&](int64_t q) { return p.offsets[q + 1] + kBM * q > kBM * u; });
     if (lo >= p.Q) return false;
-    w.m = u - lo;
-    if (w.m < 0 || w.m >= g.m_tiles) return false;
-    w.row0 = max(p.offsets[lo], w.m * kBM);
-    w.row1 = min(min(p.offsets[lo + 1], (w.m + 1) * kBM), p.T);
+    const int64_t m = u - lo;
+    if (m < 0 || m >= g.m_tiles) return false;
+    const int64_t t0 = m * kBM, row0 = max(p.offsets[lo], t0), row1 = min(min(p.offsets[lo + 1], t0 + kBM), p.T);
     w.e = adapter_of(p, lo);
     w.e_rank = rank_of(p, w.e);
-    if (w.row0 >= w.row1 || w.r0 >= w.e_rank) return false;
+    if (row0 >= row1 || w.r0 >= w.e_rank) return false;
+    w.m = (int)m;
+    w.row0 = (int)(row0 - t0);
+    w.row1 = (int)(row1 - t0);
     w.cols = min(kBN, (w.e_rank - w.r0 + 15) / 16 * 16);
   } else {
-    w.m = unit % g.m_tiles;
-    w.n0 = unit / g.m_tiles * kBN;
+    const int n_tile = (int)(unit / g.m_tiles);
+    w.m = (int)(unit - n_tile * g.m_tiles);
+    w.n0 = n_tile * kBN;
     w.cols = kBN;
   }
   w.t0 = w.m * kBM;
@@ -189,9 +185,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
         return d;
       }
     };
-    auto fetch_x = [&](auto vec, uint4(&d)[kBM * 8 / kLoad], const float* x, int64_t rs, int k, int n_kk) {
-      const float* row = x + (w.t0 + prow) * rs;
-      const int rows = (int)min(p.T - w.t0, (int64_t)kBM);
+    auto fetch_x = [&](auto vec, uint4(&d)[kBM * 8 / kLoad], const float* x, int64_t rs, int t0, int k,
+                       int n_kk) {
+      const float* row = x + (int64_t)(t0 + prow) * rs;
+      const int rows = (int)min(p.T - t0, (int64_t)kBM);
 #pragma unroll
       for (int j = 0; j < kBM * 8 / kLoad; ++j)
         d[j] = row4(vec, row + j * (kLoad / 8) * rs, k + chunk * 4, n_kk, prow + j * (kLoad / 8) < rows);
@@ -216,8 +213,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       }
     };
     const int K = (int)p.K;
-    auto fetch = [&](auto vec, Chunks<kBN>& d, int k) {
-      fetch_x(vec, d.x, (const float*)p.x, p.x_rs, k * kStep, K);
+    auto fetch = [&](auto vec, Chunks<kBN>& d, const Tile& w, int k) {
+      fetch_x(vec, d.x, (const float*)p.x, p.x_rs, w.t0, k * kStep, K);
       if constexpr (kShrink)
         fetch_b(vec, d.b, (const float*)p.P + w.e * p.p_es + w.r0 * p.p_rs, p.p_ks, p.p_rs, w.e_rank - w.r0, k * kStep,
                 K);
@@ -249,21 +246,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
         if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
         Chunks<kBN> one, two;
-        if (kb < ke) fetch(vec, one, kb);
+        if (kb < ke) fetch(vec, one, w, kb);
         for (int k = kb; k < ke && ok; k += 2) {
-          if (k + 1 < ke) fetch(vec, two, k + 1);
+          if (k + 1 < ke) fetch(vec, two, w, k + 1);
           ok = store(one);
           if (!ok || k + 1 >= ke) break;
-          if (k + 2 < ke) fetch(vec, one, k + 2);
+          if (k + 2 < ke) fetch(vec, one, w, k + 2);
           ok = store(two);
         }
         if (lowrank && ok) {
           if (!waited) dependency_wait();
           waited = true;
-          ok = for_requests(p, w.m, p.tile_q[w.m], [&](int e, int r, int, int) {
+          const int from = p.tile_q[w.m];
+          ok = for_requests(p, w.m, from, reach(p, w.m, from), [&](int e, int r, int, int) {
             for (int r0 = 0; r0 < r; r0 += kStep) {
               // rows of v are 16-byte aligned and zero from the rank to the next multiple of 4
-              fetch_x(std::true_type{}, one.x, p.v, p.v_rs, r0, r);
+              fetch_x(std::true_type{}, one.x, p.v, p.v_rs, w.t0, r0, r);
               fetch_b(std::false_type{}, one.b, (const float*)p.Qm + e * p.q_es + w.n0 * p.q_ns, p.q_rs, p.q_ns,
                       (int)min(p.N - w.n0, (int64_t)kBN), r0, r);
               if (!store(one)) return false;
@@ -314,7 +312,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       if (lowrank && ok) {
         if (!waited) dependency_wait();
         waited = true;
-        ok = for_requests(p, w.m, p.tile_q[w.m], [&](int, int r, int, int) {
+        const int from = p.tile_q[w.m];
+        ok = for_requests(p, w.m, from, reach(p, w.m, from), [&](int, int r, int, int) {
           for (int r0 = 0; r0 < r; r0 += kStep)
             if (!step((min(r - r0, kStep) + 7) / 8, true, true, id)) return false;
           return true;
@@ -326,7 +325,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     }
   } else {
     // ---------------------------------------------------------------- chunks, tiles
-    more_registers<kDrainRegs>();
     const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (kBN / 2);
     const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
     int ch = 0;
@@ -335,8 +333,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       const int rows = (int)min((int64_t)kBM, p.T - w.t0);
       if constexpr (!kShrink) {
         if (threadIdx.x < rows) {
-          const int64_t q = request_of(p, w.t0 + threadIdx.x);
-          row_e[threadIdx.x] = q < 0 ? kMixed : adapter_of(p, q);
+          const int64_t t = w.t0 + (int)threadIdx.x;
+          row_e[threadIdx.x] = !is_owned(p, t) ? kMixed : g.rowwise ? adapter_of(p, request_of(p, t)) : kNone;
         }
       }
       float acc[kBN / 2];
@@ -366,12 +364,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
         dependency_wait();
         waited = true;
       }
-      if (lowrank && ok)
-        ok = for_requests(p, w.m, p.tile_q[w.m], [&](int, int r, int a, int b) {
+      if (lowrank && ok) {
+        const int from = p.tile_q[w.m];
+        ok = for_requests(p, w.m, from, reach(p, w.m, from), [&](int, int r, int a, int b) {
           for (int r0 = 0; r0 < r; r0 += kStep)
             if (!drain(row >= a && row < b)) return false;
           return true;
         });
+      }
 #pragma unroll
       for (int i = 0; i < kBN / 2; i += 4)
         *(float4*)(part + row * kLd + c0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       drain_sync();
       ok = *(volatile int*)&gave_up == 0;
       if constexpr (kShrink) {
-        const int a = (int)(w.row0 - w.t0), b = (int)(w.row1 - w.t0), quads = w.cols / 4;
+        const int a = w.row0, b = w.row1, quads = w.cols / 4;
         const float scale = p.scale[w.e];
         for (int i = threadIdx.x; i < (b - a) * quads; i += kDrain) {
           const int r = a + i / quads, c = i % quads * 4;
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
           for (int i = 0; i < 4; ++i)
             if (n + i < p.N) bias[i] = ((const float*)p.bias)[n + i];
         if (n < p.N) {
-#pragma unroll 4
+#pragma unroll 1
           for (int r = warp; r < rows; r += 8) {
             const int re = row_e[r];
             if (re == kMixed) continue;
@@ -431,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       return s;
     };
     if constexpr (kShrink) {
-      const int a = (int)(w.row0 - w.t0), b = (int)(w.row1 - w.t0), quads = w.cols / 4;
+      const int a = w.row0, b = w.row1, quads = w.cols / 4;
       const float scale = p.scale[w.e];
       for (int i = rank * kDrain + threadIdx.x; i < (b - a) * quads; i += split * kDrain) {
         const int r = a + i / quads, c = i % quads * 4;

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       if (ok && te >= 0) ok = lowrank(te, tr, 0, 0);
-      if (ok && te == kFew) ok = for_requests(p, m, p.tile_q[m], lowrank);
+      if (ok && te == kFew) ok = for_requests(p, m, p.tile_q[m], reach(p, m, p.tile_q[m]), lowrank);
     }
     if (!ok)  // copies in flight land before shared memory is given up
       for (int i = max(0, it - kStages); i < it; ++i)
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!ok) break;
       publish(buf);
       if (te == kFew)
-        ok = for_requests(p, m, p.tile_q[m], [&](int, int rank, int, int) {
+        ok = for_requests(p, m, p.tile_q[m], reach(p, m, p.tile_q[m]), [&](int, int rank, int, int) {
           if (!claim(buf ^ 1) || !lowrank(buf ^ 1, rank, true)) return false;
           publish(buf ^ 1);
           return true;
@@ -195,9 +195,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         dependency_wait();
         waited = true;
       }
-      const int64_t q = t < p.T ? request_of(p, t) : -1;
+      const bool own = t < p.T && is_owned(p, t);
       const int te = p.R > 0 ? p.tile_e[m] : kNone;
-      const int e = te == kMixed || te == kFew ? adapter_of(p, q) : kNone, rank = rank_of(p, e);
+      const int e = own && (te == kMixed || te == kFew) ? adapter_of(p, request_of(p, t)) : kNone;
+      const int rank = rank_of(p, e);
       const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
       // The warp's rows in `rows` from accumulator buf, `more` added: kBoth: of the other accumulator,
       // kRows: v Q_e of each row's adapter.
@@ -253,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
       };
-      const uint32_t owned = __ballot_sync(0xffffffffu, q >= 0);
+      const uint32_t owned = __ballot_sync(0xffffffffu, own);
       ok = full(buf);
       if (!ok) break;
       if (te != kFew) {
@@ -261,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         const uint32_t plain = owned & __ballot_sync(0xffffffffu, rank == 0);
         if (plain) write(plain, kPlain);
-        ok = for_requests(p, m, p.tile_q[m], [&](int, int, int a, int b) {
+        ok = for_requests(p, m, p.tile_q[m], reach(p, m, p.tile_q[m]), [&](int, int, int a, int b) {
           if (!full(buf ^ 1)) return false;
           const uint32_t mine = __ballot_sync(0xffffffffu, row >= a && row < b);
           if (mine) write(mine, kBoth);
