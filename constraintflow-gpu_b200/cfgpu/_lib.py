@@ -109,7 +109,7 @@ def _load():
         "cf_conv_scale": (_i32, [P(CfConvGeom), _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _vp, _vp]),
         "cf_conv_transpose": (_i32, [P(CfConvGeom), _i64, _i64, _vp, _i64, _i64, _i64, _vp, _i32, _i32, _vp, _i64,
                                      _i64, _i64, _vp]),
-        "cf_adapter_workspace_bytes": (_sz, [P(CfAdapterLayer), _i32, _i64, _i64]),
+        "cf_adapter_workspace_bytes": (_sz, [P(CfAdapterLayer), _i32, _i64, _vp, _i64, _i64]),
         "cf_adapter_matmul": (_i32, [P(CfAdapterLayer), _i32, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _sz,
                                      _vp]),
         "cf_adapter_check": (_i32, [_vp]),

@@ -268,7 +268,7 @@ class AdapterLayer:
         if bias is not None:
             _expect("bias", bias, dt, (self.n_out,), dev)
         self.device, self.dtype, self.gpu = dev, dt, dev.index
-        self._need = {}           # workspace bytes by (substitute, T, n_requests)
+        self._need = {}           # workspace bytes by sizes and alignment
         self._keep = (W, A, B, scale, ranks, bias)
 
         def strides(t):
@@ -307,13 +307,14 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
         out = torch.zeros(T, N, dtype=dt, device=dev)
     elif not _plain(out, dt, gpu, (T, N)):
         _expect("out", out, dt, (T, N), dev, strided=True)
-    key = (substitute, T, Q)
+    xp, rs = x.data_ptr(), _row_stride(x)
+    key = (substitute, T, Q, xp % 16, rs)
     need = layer._need.get(key)
     if need is None:
-        need = layer._need[key] = _lib.lib.cf_adapter_workspace_bytes(layer._ref, 1 if substitute else 0, T, Q)
+        need = layer._need[key] = _lib.lib.cf_adapter_workspace_bytes(layer._ref, 1 if substitute else 0, T, xp, rs, Q)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
-    st = _launch(gpu, _lib.lib.cf_adapter_matmul, layer._ref, 1 if substitute else 0, T, x.data_ptr(), _row_stride(x), Q,
+    st = _launch(gpu, _lib.lib.cf_adapter_matmul, layer._ref, 1 if substitute else 0, T, xp, rs, Q,
                  offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out), ws.data_ptr(), need)
     if st:
         _lib.check(st, "cf_adapter_matmul")

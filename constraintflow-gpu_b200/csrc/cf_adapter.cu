@@ -36,36 +36,91 @@ namespace {
 
 size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-// The workspace's parts, from `base` on; returns its bytes.
-size_t workspace(const cf_adapter_layer& L, int64_t T, char* base, Problem* p) {
-  if (T <= 0 || L.rank <= 0 || L.n_adapters <= 0) return 0;
-  const int64_t ld = ceil_div(L.rank, 8) * 8;
+struct Operand {
+  const void* p;
+  int64_t entries, rows, cols, es, rs;
+  int64_t pad = 0;  // zeros in place of no columns
+};
+
+// What the kernels cannot read where it lies is copied (16-bit data only): TMA wants 16-byte
+// aligned rows and adapters, and adapters that do not overlap.
+bool aligned(const Operand& o, int64_t size) {
+  return o.cols > 0 && (uintptr_t)o.p % 16 == 0 && o.rs * size % 16 == 0 && o.rs >= o.cols &&
+         (o.entries == 1 || (o.es * size % 16 == 0 && o.es >= o.rows * o.rs));
+}
+
+// (no columns of x: nothing to adapt)
+bool has_adapters(const cf_adapter_layer& L, int64_t K) { return L.n_adapters > 0 && L.rank > 0 && K > 0; }
+
+// With few rows a request, a tile of the tensor cores would be multiplied once for each of its
+// requests: v row by row on the CUDA cores instead.
+bool rows_alone(int64_t T, int64_t n_requests) { return T < 16 * n_requests; }
+
+// The workspace's parts, from `base` on (NULL: only their sizes are asked for); returns its bytes.
+// x, M, A and B are pointed to their copies where they have one.
+size_t workspace(const cf_adapter_layer& L, int64_t T, int64_t n_requests, Operand& x, Operand& W, Operand& A,
+                 Operand& B, char* base, Problem* p, Pack* pack) {
+  if (T <= 0) return 0;
+  const bool adapters = has_adapters(L, x.cols);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     char* q = base ? base + at : nullptr;
     at += align256(bytes);
     return q;
   };
-  char* v = take((size_t)T * ld * 4);
-  char *hi = nullptr, *lo = nullptr;
-  if (L.dtype == CF_BF16) {
-    hi = take((size_t)T * ld * 2);
-    lo = take((size_t)T * ld * 2);
+  if (adapters) {
+    const int64_t ld = ceil_div(L.rank, 8) * 8;
+    char* v = take((size_t)T * ld * 4);
+    char *hi = nullptr, *lo = nullptr;
+    if (L.dtype == CF_BF16) {
+      hi = take((size_t)T * ld * 2);
+      lo = take((size_t)T * ld * 2);
+    }
+    char* tile_e = take((size_t)ceil_div(T, kBM) * 4);
+    char* tile_q = take((size_t)ceil_div(T, kBM) * 4);
+    if (p) {
+      p->v = (float*)v, p->v_rs = ld;
+      p->v_hi = (__nv_bfloat16*)hi, p->v_lo = (__nv_bfloat16*)lo;
+      p->tile_e = (int32_t*)tile_e, p->tile_q = (int32_t*)tile_q;
+    }
   }
-  char* tile_e = take((size_t)ceil_div(T, kBM) * 4);
-  char* tile_q = take((size_t)ceil_div(T, kBM) * 4);
-  if (p) {
-    p->v = (float*)v, p->v_rs = ld;
-    p->v_hi = (__nv_bfloat16*)hi, p->v_lo = (__nv_bfloat16*)lo;
-    p->tile_e = (int32_t*)tile_e, p->tile_q = (int32_t*)tile_q;
+  if (L.dtype == CF_F32) return at;
+  auto copy = [&](Operand& o, int64_t cols) {  // rows of `cols` elements, zeros behind the data's
+    if (aligned(o, 2)) return;
+    const int64_t rs = ceil_div(cols, 8) * 8;
+    char* to = take((size_t)o.entries * o.rows * rs * 2);
+    if (!pack) return;
+    pack->item[pack->n++] = {o.p, to, o.entries, o.rows, o.cols, o.es, o.rs, rs};
+    o.p = to, o.rs = rs, o.es = o.rows * rs;
+  };
+  copy(x, x.cols > 0 ? x.cols : 8);
+  copy(W, W.cols > 0 ? W.cols : W.pad);
+  if (adapters && !rows_alone(T, n_requests)) {
+    copy(A, A.cols);
+    copy(B, B.cols);
   }
   return at;
 }
 
+Operand operand_x(const void* x, int64_t T, int64_t K, int64_t x_rs) {
+  return {x, 1, T, K, 0, T > 1 ? x_rs : (x_rs >= K ? x_rs : K)};
+}
+// A contraction over nothing is one over eight zeros.
+Operand operand_W(const cf_adapter_layer& L, bool substitute) {
+  if (substitute && L.n_out == 0) return {nullptr, 1, 8, 0, 0, 0, L.n_in};
+  return {L.W_dev, 1, L.n_out, L.n_in, 0, L.w_rs, 8};
+}
+Operand operand_A(const cf_adapter_layer& L) { return {L.A_dev, L.n_adapters, L.rank, L.n_in, L.a_es, L.a_rs}; }
+Operand operand_B(const cf_adapter_layer& L) { return {L.B_dev, L.n_adapters, L.n_out, L.rank, L.b_es, L.b_rs}; }
+
 }  // namespace
 
-extern "C" size_t cf_adapter_workspace_bytes(const cf_adapter_layer* L, int32_t, int64_t T, int64_t) {
-  return L ? workspace(*L, T, nullptr, nullptr) : 0;
+extern "C" size_t cf_adapter_workspace_bytes(const cf_adapter_layer* L, int32_t substitute, int64_t T, const void* x,
+                                             int64_t x_rs, int64_t n_requests) {
+  if (!L || T <= 0) return 0;
+  Operand ox = operand_x(x, T, substitute ? L->n_out : L->n_in, x_rs), W = operand_W(*L, substitute != 0), A = operand_A(*L),
+          B = operand_B(*L);
+  return workspace(*L, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
 }
 
 extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substitute, int64_t T, const void* x,
@@ -79,51 +134,50 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   CF_REQUIRE(T < 0x7fffff00 && n_requests < 0x7fffff00, CF_ERR_SHAPE, "adapter_matmul: too many rows");
   CF_REQUIRE(T <= 1 || (x_rs >= 0 && y_rs >= N), CF_ERR_SHAPE, "adapter_matmul: rows of y overlap");
   if (T == 0 || N == 0 || n_requests == 0) return CF_OK;
-  const bool adapters = L->n_adapters > 0 && L->rank > 0;
+  const bool adapters = has_adapters(*L, K);
   CF_REQUIRE(y && offsets && ids && (K == 0 || (x && L->W_dev)), CF_ERR_NULL, "adapter_matmul: NULL argument");
   CF_REQUIRE(!adapters || (L->A_dev && L->B_dev && L->scale_dev), CF_ERR_NULL, "adapter_matmul: NULL adapters");
-  const size_t need = workspace(*L, T, nullptr, nullptr);
-  CF_REQUIRE(ws_bytes >= need && (need == 0 || ws), CF_ERR_WORKSPACE, "adapter_matmul: workspace of %zu bytes, needs %zu",
-             ws_bytes, need);
-  CF_REQUIRE((uintptr_t)ws % 256 == 0, CF_ERR_WORKSPACE, "adapter_matmul: the workspace must be 256-byte aligned");
   const int64_t size = elem_bytes(L->dtype);
   CF_REQUIRE(((uintptr_t)x | (uintptr_t)y | (uintptr_t)L->W_dev | (uintptr_t)L->A_dev | (uintptr_t)L->B_dev |
               (uintptr_t)L->bias_dev) % size == 0,
              CF_ERR_SHAPE, "adapter_matmul: unaligned data");
+  Operand ox = operand_x(x, T, K, x_rs), W = operand_W(*L, substitute != 0), A = operand_A(*L), B = operand_B(*L);
+  const size_t need = workspace(*L, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
+  CF_REQUIRE(ws_bytes >= need && (need == 0 || ws), CF_ERR_WORKSPACE, "adapter_matmul: workspace of %zu bytes, needs %zu",
+             ws_bytes, need);
+  CF_REQUIRE((uintptr_t)ws % 256 == 0, CF_ERR_WORKSPACE, "adapter_matmul: the workspace must be 256-byte aligned");
   Problem p = {};
+  Pack pack = {};
+  workspace(*L, T, n_requests, ox, W, A, B, (char*)ws, &p, &pack);
   p.T = T, p.K = K, p.N = N;
   p.R = adapters ? L->rank : 0, p.E = adapters ? L->n_adapters : 0, p.Q = n_requests;
-  p.x = x, p.x_rs = x_rs, p.M = L->W_dev, p.y = y, p.y_rs = y_rs;
+  p.x = ox.p, p.x_rs = ox.rs, p.M = W.p, p.y = y, p.y_rs = y_rs;
   p.scale = L->scale_dev, p.ranks = L->ranks_dev, p.offsets = offsets, p.ids = ids;
   if (substitute) {
-    p.m_ks = L->w_rs, p.m_ns = 1;
-    p.P = L->B_dev, p.p_es = L->b_es, p.p_ks = L->b_rs, p.p_rs = 1;
-    p.Qm = L->A_dev, p.q_es = L->a_es, p.q_rs = L->a_rs, p.q_ns = 1;
+    p.m_ks = W.rs, p.m_ns = 1;
+    p.P = B.p, p.p_es = B.es, p.p_ks = B.rs, p.p_rs = 1;
+    p.Qm = A.p, p.q_es = A.es, p.q_rs = A.rs, p.q_ns = 1;
   } else {
     p.bias = L->bias_dev;
-    p.m_ks = 1, p.m_ns = L->w_rs;
-    p.P = L->A_dev, p.p_es = L->a_es, p.p_ks = 1, p.p_rs = L->a_rs;
-    p.Qm = L->B_dev, p.q_es = L->b_es, p.q_rs = 1, p.q_ns = L->b_rs;
+    p.m_ks = 1, p.m_ns = W.rs;
+    p.P = A.p, p.p_es = A.es, p.p_ks = 1, p.p_rs = A.rs;
+    p.Qm = B.p, p.q_es = B.es, p.q_rs = 1, p.q_ns = B.rs;
   }
   auto vec = [&](const void* base, int64_t s0, int64_t s1) {
     return (uintptr_t)base % 16 == 0 && s0 * size % 16 == 0 && s1 * size % 16 == 0;
   };
-  p.x_vec = vec(x, T > 1 ? x_rs : 0, 0);
-  p.m_vec = vec(L->W_dev, L->w_rs, 0);
-  const bool a_vec = adapters && vec(L->A_dev, L->a_rs, L->a_es), b_vec = adapters && vec(L->B_dev, L->b_rs, L->b_es);
+  p.x_vec = vec(ox.p, T > 1 ? ox.rs : 0, 0);
+  p.m_vec = vec(W.p, W.rs, 0);
+  const bool a_vec = adapters && vec(A.p, A.rs, A.es), b_vec = adapters && vec(B.p, B.rs, B.es);
   p.p_vec = substitute ? b_vec : a_vec;
   p.q_vec = substitute ? a_vec : b_vec;
   p.y_vec = vec(y, T > 1 ? y_rs : 0, 0);
-  workspace(*L, T, (char*)ws, &p);
-  // Tensor maps want 16-byte strides, and adapters that do not overlap.
-  const bool tma = L->dtype != CF_F32 && K > 0 && p.x_vec && p.m_vec && x_rs * size % 16 == 0 && x_rs >= K;
-  const bool lowrank = a_vec && b_vec && (L->n_adapters == 1 || (L->a_es >= L->rank * L->a_rs &&
-                                                                 L->b_es >= L->n_out * L->b_rs));
-  // With few rows a request, a tile of the tensor cores would be multiplied once for each of
-  // its requests: v row by row on the CUDA cores instead.
-  const bool rows = T < 16 * n_requests;
+  const bool rows = rows_alone(T, n_requests);
   if (L->dtype == CF_F32) return launch_f32(p, substitute != 0, rows, as_stream(stream));
-  return launch_tiles(p, L->dtype, substitute != 0, tma, rows, lowrank, as_stream(stream));
+  CF_TRY(launch_pack(pack, as_stream(stream)));
+  if (K == 0) p.K = 8;
+  return launch_tiles(p, L->dtype, substitute != 0, rows, adapters && aligned(A, 2) && aligned(B, 2),
+                      as_stream(stream));
 }
 
 extern "C" cf_status cf_adapter_check(void* stream) {

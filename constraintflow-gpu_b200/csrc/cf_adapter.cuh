@@ -177,9 +177,21 @@ __device__ __forceinline__ void store_v(const Problem& p, int64_t t, int r, floa
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// 16-bit data (cf_adapter_tile.cu).  tma: 16-byte aligned operands, read by TMA; lowrank_tma: the
-// adapters too.  row_shrink: v row by row on the CUDA cores (requests of few rows).
-cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool tma, bool row_shrink, bool lowrank_tma,
+// Copies of 16-bit matrices [entries][rows][cols] with rows of dst_rs elements, a multiple of 8.
+struct Pack {
+  struct Item {
+    const void* src;
+    void* dst;
+    int64_t entries, rows, cols, src_es, src_rs, dst_rs;
+  } item[4];
+  int n;
+};
+cf_status launch_pack(const Pack& pack, cudaStream_t st);  // cf_adapter_rows.cu
+
+// 16-bit data, x and M 16-byte aligned (cf_adapter_tile.cu).  row_shrink: v row by row on the CUDA
+// cores (requests of few rows); lowrank_tma: the adapters are 16-byte aligned too, as they must
+// be without row_shrink.
+cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool row_shrink, bool lowrank_tma,
                        cudaStream_t st);
 // float32 data (cf_adapter_f32.cu)
 cf_status launch_f32(const Problem& p, bool substitute, bool row_shrink, cudaStream_t st);

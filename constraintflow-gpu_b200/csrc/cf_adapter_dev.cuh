@@ -131,18 +131,19 @@ __device__ __forceinline__ void add_lowrank(const Problem& p, int64_t t, int e, 
     constexpr int E = 16 / sizeof(T);
     int r = 0;
     if (p.q_vec) {
+#pragma unroll 2
       for (; r + E <= rank; r += E) {
         float w[E];
+        uint4 d[4];
 #pragma unroll
-        for (int i = 0; i < E; ++i) w[i] = v[r + i];
+        for (int i = 0; i < E; i += 4) *(float4*)(w + i) = *(const float4*)(v + r + i);  // rows of v are aligned
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (n + c >= p.N) break;
-          alignas(16) T d[E];
-          *(uint4*)d = *(const uint4*)(Q + (n + c) * p.q_ns + r);
+        for (int c = 0; c < 4; ++c)
+          d[c] = n + c < p.N ? *(const uint4*)(Q + (n + c) * p.q_ns + r) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-          for (int i = 0; i < E; ++i) a[c] = fmaf(w[i], to_f32(d[i]), a[c]);
-        }
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < E; ++i) a[c] = fmaf(w[i], to_f32(((const T*)&d[c])[i]), a[c]);
       }
     }
     for (; r < rank; ++r)

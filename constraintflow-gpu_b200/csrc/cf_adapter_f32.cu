@@ -39,7 +39,7 @@ constexpr int kMmaWarp = 16;
 constexpr int kThreads = 640;  // five warpgroups; warps 17-19 idle
 // Registers a thread: 96 at launch (640 x 96 = 61440).  The loads hold two steps of chunks and take
 // what the MMA group gives up: 128 (2 x 96 + 2 x 112 + 64) = 61440.
-constexpr int kLoadRegs = 112, kMmaRegs = 64;
+constexpr int kDrainRegs = 96, kLoadRegs = 112, kMmaRegs = 64;
 constexpr int kStep = 32;   // contraction of a stage: 128 bytes
 constexpr int kChunk = 2;   // steps of one accumulation
 constexpr int kStages = 2, kBufs = 2;
@@ -325,6 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     }
   } else {
     // ---------------------------------------------------------------- chunks, tiles
+    more_registers<kDrainRegs>();  // the compiler allots by it
     const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (kBN / 2);
     const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
     int ch = 0;

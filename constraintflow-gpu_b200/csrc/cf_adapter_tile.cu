@@ -11,9 +11,8 @@
 // other tiles add it row by row on the CUDA cores, where a row reads its own adapter only.
 //
 // Operands in shared memory are 128-byte-swizzled images, 128 bytes of the contraction a row:
-//   TMA:    16-bit data by tensor maps; M and Q_e with n contiguous (substitution) stay as they
-//           lie, as MN-major images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
-//   loads:  any stride and alignment, by the epilogue's warps.
+// loaded by tensor maps; M and Q_e with n contiguous (substitution) stay as they lie, as MN-major
+// images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
 #include <cooperative_groups.h>
 
 #include "cf_adapter_tma.cuh"
@@ -26,7 +25,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kWorkers = 256;  // warps 0-7: loads, epilogue
+constexpr int kWorkers = 256;  // warps 0-7: epilogue
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 320;
 
@@ -48,17 +47,18 @@ struct Bars {
   uint32_t tmem;
 };
 
-template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
+template <typename T, bool kSub, bool kShrink, int kBN, int kStages>
 __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, const __grid_constant__ Maps maps,
                                                            const Tiling g) {
   constexpr int kStep = Kind<T>::kStep;
-  constexpr bool kMn = kTma && kSub;  // B images lie n-contiguous
+  constexpr bool kMn = kSub;  // B images lie n-contiguous
   constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128;
   constexpr uint32_t kStageBytes = kABytes + kBBytes;
   static_assert((kBM * (kBN + 4)) * 4 <= kStageBytes * kStages, "the tile is staged where the operands were");
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars<kStages> bars;
-  __shared__ int row_e[kShrink ? 1 : kBM];  // each row's adapter, kMixed for a row of no request
+  // each row's adapter, kMixed for a row of no request, and that adapter's rank
+  __shared__ int row_e[kShrink ? 1 : kBM], row_rank[kShrink ? 1 : kBM];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
   cg::cluster_group cl = cg::this_cluster();
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
   if (warp == kMmaWarp) tmem_alloc(&bars.tmem, kBN < 32 ? 32 : kBN);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
-      mbar_init(&bars.full[i], kTma ? 1 : kWorkers);
+      mbar_init(&bars.full[i], 1);
       mbar_init(&bars.empty[i], 1);
     }
     mbar_init(&bars.done, 1);
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
   };
 
   bool ok = true;
-  if (kTma && warp == kProducerWarp && lane == 0) {
+  if (warp == kProducerWarp && lane == 0) {
     int it = 0, te, tr;
     auto stage_for = [&](uint32_t bytes) -> int {
       const int s = it % kStages, round = it / kStages;
@@ -207,81 +207,16 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
     }
     mma_commit(&bars.done);
     if (!ok) mbar_wait_drain(&bars.done, 0, err, 22);
-  } else if (!kTma && warp < kProducerWarp) {
-    // ---- loads: the chunks of the next step are in registers while the MMAs run
-    constexpr int kXTasks = kBM * 8 / kWorkers, kBTasks = kBN * 8 / kWorkers;
-    constexpr int E = 16 / sizeof(T);
-    uint4 xr[kXTasks], br[kBTasks];
-    const int chunk = threadIdx.x & 7, prow = threadIdx.x >> 3;  // K-contiguous rows
-    // one operand row's chunk with k scattered (n contiguous in memory)
-    auto gather = [&](const T* base, int64_t ks, int64_t k, int64_t n_kk) -> uint4 {
-      alignas(16) T t[E];
-#pragma unroll
-      for (int i = 0; i < E; ++i) t[i] = k + i < n_kk ? base[(k + i) * ks] : from_f32<T>(0.0f);
-      return *(const uint4*)t;
-    };
-    auto fetch_b = [&](const T* B, int64_t ks, int64_t ns, int64_t c0, int64_t n_c, int64_t k0, int64_t n_kk,
-                       bool vec) {
-#pragma unroll
-      for (int j = 0; j < kBTasks; ++j) {
-        if constexpr (kSub) {  // consecutive threads: consecutive columns
-          const int task = j * kWorkers + threadIdx.x;
-          const int64_t c = c0 + task % kBN, k = k0 + (task / kBN) * E;
-          br[j] = c < n_c ? gather(B + c * ns, ks, k, n_kk) : make_uint4(0, 0, 0, 0);
-        } else {
-          const int64_t c = c0 + prow + j * (kWorkers / 8), k = k0 + chunk * E;
-          br[j] = c < n_c ? load16<T>(B + c * ns, k, n_kk, vec) : make_uint4(0, 0, 0, 0);
-        }
-      }
-    };
-    int it = 0;
-    auto put_step = [&]() -> bool {
-      const int s = it % kStages, round = it / kStages;
-      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 31)) return false;
-      const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
-#pragma unroll
-      for (int j = 0; j < kXTasks; ++j) put<T>(a, kABytes, prow + j * (kWorkers / 8), chunk, xr[j]);
-#pragma unroll
-      for (int j = 0; j < kBTasks; ++j) {
-        if constexpr (kSub) {
-          const int task = j * kWorkers + threadIdx.x;
-          put<T>(b, kBBytes, task % kBN, task / kBN, br[j]);
-        } else {
-          put<T>(b, kBBytes, prow + j * (kWorkers / 8), chunk, br[j]);
-        }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&bars.full[s]);
-      ++it;
-      return true;
-    };
-    auto fetch = [&](int k) {
-#pragma unroll
-      for (int j = 0; j < kXTasks; ++j) {
-        const int64_t t = t0 + prow + j * (kWorkers / 8);
-        xr[j] = t < p.T ? load16<T>((const T*)p.x + t * p.x_rs, (int64_t)k * kStep + chunk * E, p.K, p.x_vec)
-                        : make_uint4(0, 0, 0, 0);
-      }
-      if constexpr (kShrink)
-        fetch_b((const T*)p.P + e * p.p_es, p.p_ks, p.p_rs, r0, min(e_rank, r0 + kBN), (int64_t)k * kStep, p.K,
-                p.p_vec);
-      else
-        fetch_b((const T*)p.M, p.m_ks, p.m_ns, n0, p.N, (int64_t)k * kStep, p.K, p.m_vec);
-    };
-    if (kb < ke) fetch(kb);
-    for (int k = kb; k < ke && ok; ++k) {
-      ok = put_step();
-      if (k + 1 < ke) fetch(k + 1);
-    }
   }
 
   // ---- the accumulators, staged in shared memory
   __syncwarp();
   if constexpr (!kShrink) {
-    if (kTma ? warp < 4 : warp == kProducerWarp)
-      for (int i = kTma ? threadIdx.x : lane; i < rows; i += kTma ? kBM : 32) {
+    if (warp < 4)
+      for (int i = threadIdx.x; i < rows; i += kBM) {
         const int64_t t = t0 + i;
         row_e[i] = !is_owned(p, t) ? kMixed : p.R > 0 ? adapter_of(p, request_of(p, t)) : kNone;
+        row_rank[i] = rank_of(p, row_e[i]);
       }
   }
   float* part = (float*)smem;
@@ -344,13 +279,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           if (n + i < p.N) bias[i] = to_f32(((const T*)p.bias)[n + i]);
+#pragma unroll 2
       for (int row = rank + warp * split; row < rows; row += 8 * split) {
         const int64_t t = t0 + row;
         const int re = row_e[row];
         if (re == kMixed || n >= p.N) continue;
         const float4 s = sum4(row, lane * 4);
         float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
-        if (te == kMixed || te == kFew) add_lowrank<T, kSub>(p, t, re, rank_of(p, re), n, a);
+        if (te == kMixed || te == kFew) add_lowrank<T, kSub>(p, t, re, row_rank[row], n, a);
         store4<T>(p, t, n, a);
       }
     }
@@ -359,11 +295,11 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
   if (split > 1) cl.sync();  // nobody leaves while its part is read
 }
 
-template <typename T, bool kSub, bool kShrink, bool kTma, int kBN, int kStages>
+template <typename T, bool kSub, bool kShrink, int kBN, int kStages>
 cf_status launch(const char* what, const Problem& p, const Maps& maps, const Tiling& g, int64_t clusters,
                  cudaStream_t st) {
   constexpr int smem = (kBM + kBN) * 128 * kStages + 1024;
-  auto* kern = k_adapter_tile<T, kSub, kShrink, kTma, kBN, kStages>;
+  auto* kern = k_adapter_tile<T, kSub, kShrink, kBN, kStages>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
   const int64_t blocks = clusters * g.split;
@@ -389,7 +325,7 @@ cf_status launch(const char* what, const Problem& p, const Maps& maps, const Til
   return check_launch(what);
 }
 
-template <typename T, bool kSub, bool kTma>
+template <typename T, bool kSub>
 cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cudaStream_t st) {
   constexpr int kStep = Kind<T>::kStep, kStages = 3;
   const int64_t steps = ceil_div(p.K, kStep), m_tiles = ceil_div(p.T, kBM);
@@ -398,66 +334,53 @@ cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cu
   g.m_tiles = m_tiles;
   g.x_rows = (int)(p.T < kBM ? ceil_div(p.T, 8) * 8 : kBM);
   // float16's range does not hold every intermediate that float32 does: row by row instead
-  const bool pair = kTma && dtype == CF_BF16 && lowrank_tma;
-  g.q_tma = pair;
-  g.whole = pair ? 16 : 0;
-  if (kTma) CF_TRY(encode(&maps.x, dtype, p.x, p.K, p.T, 1, p.x_rs, p.x_rs * p.T, g.x_rows));
+  g.q_tma = dtype == CF_BF16 && lowrank_tma;
+  g.whole = g.q_tma ? 16 : 0;
+  CF_TRY(encode(&maps.x, dtype, p.x, p.K, p.T, 1, p.x_rs, p.x_rs * p.T, g.x_rows));
   if (p.R > 0 && row_shrink) {
     CF_TRY(launch_row_shrink(p, dtype, kSub, g.whole, st));
   } else if (p.R > 0) {
     const int bn = p.R <= 64 ? 64 : 128;
-    const bool by_tma = kTma && lowrank_tma;
-    if (by_tma) {
-      if (kSub)
-        CF_TRY(encode(&maps.b, dtype, p.P, p.R, p.K, p.E, p.p_ks, p.p_es, 64));
-      else
-        CF_TRY(encode(&maps.b, dtype, p.P, p.K, p.R, p.E, p.p_rs, p.p_es, bn));
-    }
+    if (kSub)
+      CF_TRY(encode(&maps.b, dtype, p.P, p.R, p.K, p.E, p.p_ks, p.p_es, 64));
+    else
+      CF_TRY(encode(&maps.b, dtype, p.P, p.K, p.R, p.E, p.p_rs, p.p_es, bn));
     g.units = (m_tiles + p.Q - 1) * ceil_div(p.R, bn);
     g.split = split_for(m_tiles, steps);
-    const int64_t plans = ceil_div(m_tiles, (int64_t)g.split * (kThreads / 32));
-    const int64_t clusters = g.units + plans;
+    const int64_t clusters = g.units + ceil_div(m_tiles, (int64_t)g.split * (kThreads / 32));
     const char* what = "k_adapter_tile (shrink)";
-    if (by_tma)
-      CF_TRY(bn == 64 ? (launch<T, kSub, true, kTma, 64, kStages>(what, p, maps, g, clusters, st))
-                      : (launch<T, kSub, true, kTma, 128, kStages>(what, p, maps, g, clusters, st)));
-    else
-      CF_TRY(bn == 64 ? (launch<T, kSub, true, false, 64, kStages>(what, p, maps, g, clusters, st))
-                      : (launch<T, kSub, true, false, 128, kStages>(what, p, maps, g, clusters, st)));
+    CF_TRY(bn == 64 ? (launch<T, kSub, true, 64, kStages>(what, p, maps, g, clusters, st))
+                    : (launch<T, kSub, true, 128, kStages>(what, p, maps, g, clusters, st)));
   }
   constexpr int bn = 128;
-  if (kTma) {
-    if (pair && p.R > 0) {
-      CF_TRY(encode(&maps.v_hi, dtype, p.v_hi, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
-      CF_TRY(encode(&maps.v_lo, dtype, p.v_lo, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
-    }
-    if (m_tiles * ceil_div(p.N, 256) >= 148) return launch_wide(p, dtype, kSub, maps, g.q_tma, st);
-    CF_TRY(encode_weights(p, dtype, kSub, bn, g.q_tma, &maps));
+  if (g.q_tma && p.R > 0) {
+    CF_TRY(encode(&maps.v_hi, dtype, p.v_hi, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
+    CF_TRY(encode(&maps.v_lo, dtype, p.v_lo, p.R, p.T, 1, p.v_rs, p.v_rs * p.T, g.x_rows));
   }
   g.dependent = p.R > 0;
   g.units = m_tiles * ceil_div(p.N, bn);
+  // More 128-column tiles than a wave: 256-column ones, one CTA an SM (1024 x 4096 x 4096: 29 us
+  // against 52; 512 x 4096 x 4096, 128 tiles: 28 both).  Where row tiles may hold several requests,
+  // whose low-rank parts the wide kernel puts on the tensor cores and this one does not, from a
+  // quarter of a wave on (384 x 4096 x 4096, 5 requests, rank 16: 36 against 54).
+  if (g.units > (g.q_tma && p.R > 0 && !row_shrink ? 64 : 128)) 
+    return launch_wide(p, dtype, kSub, maps, g.q_tma, g.x_rows, st);
+  CF_TRY(encode_weights(p, dtype, kSub, bn, g.q_tma, &maps));
   g.split = split_for(g.units, steps);
   // tiles for more than half of the SMs: three CTAs a tile, two an SM (86 tiles: 25.2 us, 28.6 with one)
   if (g.units > 64 && g.units <= 88 && steps >= 12) g.split = 3;
-  return launch<T, kSub, false, kTma, bn, kStages>("k_adapter_tile", p, maps, g, g.units, st);
+  return launch<T, kSub, false, bn, kStages>("k_adapter_tile", p, maps, g, g.units, st);
 }
 
 }  // namespace
 
-cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool tma, bool row_shrink, bool lowrank_tma,
+cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool row_shrink, bool lowrank_tma,
                        cudaStream_t st) {
-  if (dtype == CF_BF16) {
-    if (tma)
-      return substitute ? run<__nv_bfloat16, true, true>(p, dtype, row_shrink, lowrank_tma, st)
-                        : run<__nv_bfloat16, false, true>(p, dtype, row_shrink, lowrank_tma, st);
-    return substitute ? run<__nv_bfloat16, true, false>(p, dtype, row_shrink, lowrank_tma, st)
-                      : run<__nv_bfloat16, false, false>(p, dtype, row_shrink, lowrank_tma, st);
-  }
-  if (tma)
-    return substitute ? run<__half, true, true>(p, dtype, row_shrink, lowrank_tma, st)
-                      : run<__half, false, true>(p, dtype, row_shrink, lowrank_tma, st);
-  return substitute ? run<__half, true, false>(p, dtype, row_shrink, lowrank_tma, st)
-                    : run<__half, false, false>(p, dtype, row_shrink, lowrank_tma, st);
+  if (dtype == CF_BF16)
+    return substitute ? run<__nv_bfloat16, true>(p, dtype, row_shrink, lowrank_tma, st)
+                      : run<__nv_bfloat16, false>(p, dtype, row_shrink, lowrank_tma, st);
+  return substitute ? run<__half, true>(p, dtype, row_shrink, lowrank_tma, st)
+                    : run<__half, false>(p, dtype, row_shrink, lowrank_tma, st);
 }
 
 cf_status take_site_tiles(int* site, cudaStream_t st) { return take_site(&g_err, site, st); }

@@ -77,8 +77,10 @@ inline cf_status encode_weights(const Problem& p, int dtype, bool substitute, in
   return encode(&maps->q, dtype, p.Qm, p.R, p.N, p.E, p.q_ns, p.q_es, bn);
 }
 
-// The 16-bit product in 128 x 256 tiles (cf_adapter_wide.cu); maps.x, v_hi and v_lo are set.
-cf_status launch_wide(const Problem& p, int dtype, bool substitute, Maps maps, bool q_tma, cudaStream_t st);
+// The 16-bit product in 128 x 256 tiles (cf_adapter_wide.cu); maps.x, v_hi and v_lo are set, with
+// boxes of x_rows rows.
+cf_status launch_wide(const Problem& p, int dtype, bool substitute, Maps maps, bool q_tma, int x_rows,
+                      cudaStream_t st);
 
 }  // namespace adapter
 }  // namespace cf

@@ -36,7 +36,8 @@ struct Bars {
 
 template <typename T, bool kSub>
 __global__ void __launch_bounds__(kThreads, 1)
-    k_adapter_wide(const Problem p, const __grid_constant__ Maps maps, int64_t m_tiles, int64_t units, int q_tma) {
+    k_adapter_wide(const Problem p, const __grid_constant__ Maps maps, int64_t m_tiles, int64_t units, int q_tma,
+                   uint32_t x_bytes) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int s = it % kStages;
       if (!mbar_wait(&bars.empty[s], ((it / kStages) & 1) ^ 1, err, 81)) return false;
       if (lane == 0) {
-        mbar_arrive_expect_tx(&bars.full[s], kStageBytes);
+        mbar_arrive_expect_tx(&bars.full[s], x_bytes + kBBytes);
         const uint32_t dst = sbase + s * kStageBytes;
         tma_3d(dst, x, xk, (int)t0, 0, &bars.full[s]);
         if constexpr (kSub) {
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 template <typename T, bool kSub>
-cf_status launch(const Problem& p, const Maps& maps, bool q_tma, cudaStream_t st) {
+cf_status launch(const Problem& p, const Maps& maps, bool q_tma, int x_rows, cudaStream_t st) {
   auto* kern = k_adapter_wide<T, kSub>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "k_adapter_wide: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -298,7 +299,8 @@ cf_status launch(const Problem& p, const Maps& maps, bool q_tma, cudaStream_t st
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.R > 0 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kern, p, maps, m_tiles, units, (int)(q_tma && p.R > 0));
+  e = cudaLaunchKernelEx(&cfg, kern, p, maps, m_tiles, units, (int)(q_tma && p.R > 0),
+                         (uint32_t)x_rows * 128u);
   if (e != cudaSuccess) {
     set_error("k_adapter_wide: %s", cudaGetErrorString(e));
     return CF_ERR_CUDA;
@@ -308,12 +310,13 @@ cf_status launch(const Problem& p, const Maps& maps, bool q_tma, cudaStream_t st
 
 }  // namespace
 
-cf_status launch_wide(const Problem& p, int dtype, bool substitute, Maps maps, bool q_tma, cudaStream_t st) {
+cf_status launch_wide(const Problem& p, int dtype, bool substitute, Maps maps, bool q_tma, int x_rows,
+                      cudaStream_t st) {
   CF_TRY(encode_weights(p, dtype, substitute, kBN, q_tma, &maps));
   if (dtype == CF_BF16)
-    return substitute ? launch<__nv_bfloat16, true>(p, maps, q_tma, st)
-                      : launch<__nv_bfloat16, false>(p, maps, q_tma, st);
-  return substitute ? launch<__half, true>(p, maps, q_tma, st) : launch<__half, false>(p, maps, q_tma, st);
+    return substitute ? launch<__nv_bfloat16, true>(p, maps, q_tma, x_rows, st)
+                      : launch<__nv_bfloat16, false>(p, maps, q_tma, x_rows, st);
+  return substitute ? launch<__half, true>(p, maps, q_tma, x_rows, st) : launch<__half, false>(p, maps, q_tma, x_rows, st);
 }
 
 cf_status take_site_wide(int* site, cudaStream_t st) { return take_site(&g_err, site, st); }

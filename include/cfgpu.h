@@ -431,9 +431,10 @@ typedef struct cf_adapter_layer {
  * do not overlap.  A request's rows depend on its own adapter only: infinities or NaN in another
  * adapter or in rows of other requests do not reach them.  Products are accumulated in float32;
  * float32 data is multiplied as 3xTF32, as in the chained substitution.  The workspace
- * (256-byte aligned, >= cf_adapter_workspace_bytes) belongs to the call until it has run. */
+ * (256-byte aligned, >= cf_adapter_workspace_bytes for these arguments) belongs to the call until
+ * it has run; 16-bit operands whose rows are not 16-byte aligned are copied into it. */
 size_t cf_adapter_workspace_bytes(const cf_adapter_layer* layer, int32_t substitute, int64_t T,
-                                  int64_t n_requests);
+                                  const void* x_dev, int64_t x_rs, int64_t n_requests);
 cf_status cf_adapter_matmul(const cf_adapter_layer* layer, int32_t substitute, int64_t T, const void* x_dev,
                             int64_t x_rs, int64_t n_requests, const int64_t* offsets_dev, const int32_t* ids_dev,
                             void* y_dev, int64_t y_rs, void* workspace_dev, size_t workspace_bytes, void* stream);

@@ -239,6 +239,36 @@ def test_adapter_streams_and_graphs(dtype, T, Q):
     V.check(outs[0], *oracle(t, False))
 
 
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_adapter_few_rows_many_columns(dtype, sub):
+    """Less than a tile of rows through enough columns for the wide tiles, aligned and not."""
+    compare(make(40, 72, 20008, 16, 3, 4, dtype, sub, seed=41, ranks=True), sub)
+    compare(make(5, 72, 17001, 5, 3, 2, dtype, sub, seed=42, ranks=True), sub)
+
+
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_a_contraction_over_nothing(dtype, sub):
+    o = ops()
+    n_out, n_in = (0, 24) if sub else (24, 0)
+    z = lambda *s: torch.zeros(*s, dtype=dtype, device="cuda")
+    bias = None if sub else torch.randn(24, generator=gen(0)).to(dtype).cuda()
+    L = o.AdapterLayer(z(n_out, n_in), z(2, 4, n_in), z(2, n_out, 4), torch.ones(2, device="cuda"), bias=bias)
+    got = o.adapter_matmul(z(33, 0), L, torch.tensor([0, 20, 33]).cuda(), torch.tensor([0, 1]).int().cuda(),
+                           substitute=sub)
+    assert torch.equal(got, z(33, 24) if sub else bias.expand(33, 24))
+
+
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("K,N,R", [(65, 130, 7), (200, 131, 16), (67, 264, 16), (129, 136, 24)])
+@pytest.mark.parametrize("T,Q", [(3, 3), (40, 40), (300, 4), (2500, 30)])
+def test_adapter_unaligned_sizes(dtype, sub, K, N, R, T, Q):
+    compare(make(T, K, N, R, 4, Q, dtype, sub, seed=T + K, style="tokens" if Q == T else "ragged", ranks=True,
+                 bias=True), sub)
+
+
 # ------------------------------------------------------------------------ answer rules
 def make_rules(rows, n, seed=0, hist=20, biases=5, masks=2, penalties=True, prompt=True):
     g = gen(seed)

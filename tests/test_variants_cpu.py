@@ -19,7 +19,7 @@ def c_layer(**kw):
 
 def call(L, substitute=0, T=8, x=256, x_rs=16, q=2, off=256, ids=256, y=4096, y_rs=32, ws=1 << 16, wsb=None):
     if wsb is None:
-        wsb = _lib.lib.cf_adapter_workspace_bytes(ctypes.byref(L), substitute, T, q)
+        wsb = _lib.lib.cf_adapter_workspace_bytes(ctypes.byref(L), substitute, T, x, x_rs, q)
     return _lib.lib.cf_adapter_matmul(ctypes.byref(L), substitute, T, x, x_rs, q, off, ids, y, y_rs, ws, wsb, None)
 
 
