@@ -11,13 +11,15 @@
 // is monotone in x for repetition > 0: the edit of a lower (upper) bound is a lower (upper)
 // bound of the edit, rounding included, and no interval arithmetic is needed.
 //
-// Memory-bound: a row is read (and written) once.  What the history and the biases touch is
-// little and is put right from their side: a CTA counts in shared memory what they say about its
-// slice of the answers, lists the answers that are touched, and edits those alone.  (A table
-// lookup for every answer on the way, the edit under a branch, took 228 us for 256 x 131072
-// bfloat16 with 1024 tokens a row: some lane of nearly every warp has one.)
+// Memory-bound: a row is read (and written) once, and only its mask is looked at on the way.
+// What the history and the biases touch is little and is put right from their side, in the result
+// that the stream has left in the cache.  For 256 x 131072 bfloat16 and 1024 tokens a row: a lookup
+// for every answer on the way 228 us (some lane of nearly every warp edits), edits of each slice in
+// shared memory on its way 50, the stream 22 and behind it the edits.
 //
-// Tables hold 16 bits an answer, seen and 15 bits of times, and a bit for its having a bias.
+// Short histories go into a hash table of the answers they touch, one CTA a row, whatever the row's
+// length.  Long ones are counted slice by slice in tables of all answers: 16 bits an answer, seen
+// and 15 bits of times, and a bit for its having a bias.
 // Which of the (few) biases of one answer is the last is found by comparing them.  A row with more
 // than kMaxBiases biases, or one answer more than kTimes times, is done in quarters of a
 // slice, with 32 bits for the times and 32 for the place of the last bias.  Counts are integers
@@ -35,7 +37,9 @@ namespace {
 // of a table's entry, 16 bits (wide: the highest of 32)
 constexpr uint32_t kSeen = 0x8000u, kTimes = 0x7fffu, kWideTimes = 0x7fffffffu;
 constexpr uint32_t kMaxBiases = 1024;
-constexpr uint32_t kList = 2048;  // touched answers of a slice that are edited from a list
+// Touched answers of a slice are edited from a list where a row has at most kListed tokens; a longer
+// row's would wait for one another at the list's counter, and are many anyhow.
+constexpr uint32_t kList = 1024, kListed = 4096;
 
 struct Row {
   uint32_t h0, h1, answered;  // history, and where its answered part begins
@@ -106,12 +110,12 @@ __device__ __noinline__ float edit(float v, bool seen, uint32_t times, float rep
 struct Tables {
   uint32_t* words;   // 16-bit entries of a slice; wide: 32-bit counts, then places, of a quarter
   uint32_t* biased;  // a bit for each answer
-  uint32_t* listed;  // touched answers; the list holds the first kList
   uint32_t* over;    // an answer has more than kTimes
+  uint32_t* listed;  // touched answers, the list holds the first kList
   uint16_t* list;    // places in the slice (quarter)
   int32_t* ids;      // the row's biases (not wide)
   int log_s;
-  bool wide;
+  bool wide, listing;
 };
 
 size_t tables_bytes(int log_s) {
@@ -122,10 +126,11 @@ __device__ __forceinline__ Tables tables_of(const Row& w, uint32_t* smem, int lo
   Tables t;
   t.words = smem;
   t.biased = smem + (1u << (log_s - 1));
-  t.listed = t.biased + (1u << (log_s - 5));
-  t.over = t.listed + 1;
-  t.list = (uint16_t*)(t.listed + 4);
+  t.over = t.biased + (1u << (log_s - 5));
+  t.listed = t.over + 1;
+  t.list = (uint16_t*)(t.over + 4);
   t.ids = (int32_t*)(t.list + kList);
+  t.listing = w.h1 - w.h0 <= kListed;
   t.log_s = log_s;
   t.wide = w.b1 - w.b0 > kMaxBiases;
   return t;
@@ -145,7 +150,7 @@ __device__ __forceinline__ void walk(const int32_t* list, uint32_t from, uint32_
   }
 }
 
-// The counts of answers [lo, lo + size) from the row's history, and the list of those it holds.
+// The counts of answers [lo, lo + size) from the row's history.
 // False: to be done wide.
 __device__ __forceinline__ bool count(const cf_answer_rules& R, const Row& w, const Tables& t, int lo, uint32_t size) {
   const uint32_t words = t.wide ? size : (size + 1) / 2;
@@ -155,7 +160,7 @@ __device__ __forceinline__ bool count(const cf_answer_rules& R, const Row& w, co
   }
   if (w.b1 > w.b0)
     for (uint32_t i = threadIdx.x; i < (size + 31) / 32; i += blockDim.x) t.biased[i] = 0;
-  if (threadIdx.x == 0) *t.listed = *t.over = 0;
+  if (threadIdx.x == 0) *t.over = *t.listed = 0;
   if (!t.wide)
     for (uint32_t i = w.b0 + threadIdx.x; i < w.b1; i += blockDim.x) t.ids[i - w.b0] = R.bias_ids_dev[i];
   __syncthreads();
@@ -172,7 +177,7 @@ __device__ __forceinline__ bool count(const cf_answer_rules& R, const Row& w, co
       old = old >> sh & 0xffffu;
       if (answered && (old & kTimes) == kTimes) *(volatile uint32_t*)t.over = 1;
     }
-    if (old == 0) {
+    if (t.listing && old == 0) {
       const uint32_t at = atomicAdd(t.listed, 1u);
       if (at < kList) t.list[at] = (uint16_t)k;
     }
@@ -221,41 +226,61 @@ __device__ __forceinline__ void for_biased(const cf_answer_rules& R, const Row& 
 }
 
 // f(answer, times, x[answer]) for each allowed answer of the slice that the history holds and
-// that has no bias; kBatch loads of x in flight a thread.
+// that has no bias; several a thread at a time, their loads of x in flight together.
 template <typename T, typename F>
 __device__ __forceinline__ void for_seen(const Row& w, const Tables& t, int lo, uint32_t size, const T* x, F&& f) {
-  constexpr int kBatch = 8;
-  const uint32_t listed = *t.listed;
-  const bool all = listed > kList;  // more than the list holds: entry by entry
-  const uint32_t n = all ? size : listed;
-  for (uint32_t i = threadIdx.x; i < n; i += kBatch * blockDim.x) {
-    uint32_t k[kBatch], c[kBatch];
-    T v[kBatch];
+  if (t.listing && *t.listed <= kList) {
+    constexpr int kBatch = 4;
+    const uint32_t n = *t.listed;
+    for (uint32_t i = threadIdx.x; i < n; i += kBatch * blockDim.x) {
+      uint32_t k[kBatch], c[kBatch];
+      T v[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const uint32_t at = i + b * blockDim.x;
-      k[b] = all ? at : at < n ? t.list[at] : 0u;
-      c[b] = at < n ? entry(t, k[b]) : 0u;
-      if (c[b] && is_biased(w, t, k[b])) c[b] = 0;
+      for (int b = 0; b < kBatch; ++b) {
+        const bool ok = i + b * blockDim.x < n;
+        k[b] = ok ? t.list[i + b * blockDim.x] : 0u;
+        c[b] = ok && !is_biased(w, t, k[b]) && is_allowed(w.allowed, lo + (int)k[b]) ? entry(t, k[b]) : 0u;
+        v[b] = c[b] ? x[lo + (int)k[b]] : from_f32<T>(0.0f);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        if (c[b]) f(lo + (int)k[b], times(t, c[b]), to_f32(v[b]));
+    }
+    return;
+  }
+  for (uint32_t k0 = threadIdx.x * 8; k0 < size; k0 += blockDim.x * 8) {
+    uint32_t c[8];
+    if (t.wide) {
+      *(uint4*)c = *(const uint4*)(t.words + k0);
+      *(uint4*)(c + 4) = *(const uint4*)(t.words + k0 + 4);
+    } else {
+      const uint4 d = *(const uint4*)(t.words + k0 / 2);
+      if (!(d.x | d.y | d.z | d.w)) continue;
+      const uint32_t h[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+      for (int b = 0; b < 8; ++b) c[b] = h[b / 2] >> (b & 1) * 16 & 0xffffu;
+    }
+    T v[8];
+#pragma unroll
+    for (int b = 0; b < 8; ++b) {
+      const int j = lo + (int)k0 + b;
+      if (k0 + b >= size || (c[b] && (is_biased(w, t, k0 + b) || !is_allowed(w.allowed, j)))) c[b] = 0;
+      v[b] = c[b] ? x[j] : from_f32<T>(0.0f);
     }
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (c[b] && !is_allowed(w.allowed, lo + (int)k[b])) c[b] = 0;
-      v[b] = c[b] ? x[lo + (int)k[b]] : from_f32<T>(0.0f);
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-      if (c[b]) f(lo + (int)k[b], times(t, c[b]), to_f32(v[b]));
+    for (int b = 0; b < 8; ++b)
+      if (c[b]) f(lo + (int)k0 + b, times(t, c[b]), to_f32(v[b]));
   }
 }
 
-// 16 bytes of a row, moved whole; rows are read once and written once, past the caches' own order.
+// 16 bytes of a row, moved whole.  Rows are read once, past the cache; what is written stays there
+// for the edits behind.
 template <typename T>
 struct alignas(16) Vec {
   static constexpr int N = 16 / sizeof(T);
   T v[N];
   __device__ __forceinline__ void load(const T* p) { *(uint4*)v = __ldcs((const uint4*)p); }
-  __device__ __forceinline__ void store(T* p) const { __stcs((uint4*)p, *(const uint4*)v); }
+  __device__ __forceinline__ void store(T* p) const { *(uint4*)p = *(const uint4*)v; }
 };
 
 // ---------------------------------------------------------------------- edit_logits
@@ -323,45 +348,136 @@ __global__ void __launch_bounds__(kStreamThreads)
   }
 }
 
-// The answers that the history and the biases touch, one CTA per slice of a row, after the stream.
-constexpr int kEditThreads = 512;
+// ---- what a short row touches: open addressing over the answers
+constexpr uint32_t kSlots = 4096, kShort = 3072;  // tokens and biases of a row at most
 
+struct Hash {
+  uint32_t *key, *cnt, *pos;  // answer + 1 (0: free); times and, highest bit, seen; place of the last bias
+  uint32_t* listed;
+  uint16_t* list;  // slots in use
+};
+
+constexpr size_t kHashBytes = kSlots * 12 + 16 + kShort * 2;
+
+__device__ __forceinline__ Hash hash_of(uint32_t* smem) {
+  Hash h;
+  h.key = smem;
+  h.cnt = smem + kSlots;
+  h.pos = smem + 2 * kSlots;
+  h.listed = smem + 3 * kSlots;
+  h.list = (uint16_t*)(h.listed + 4);
+  return h;
+}
+
+// The slot of answer j; the first to come to it lists it.
+__device__ __forceinline__ uint32_t slot_of(const Hash& h, uint32_t j) {
+  uint32_t s = j * 2654435761u >> 20;  // of 4096, by the golden ratio
+  for (;;) {
+    const uint32_t old = atomicCAS(h.key + s, 0u, j + 1u);
+    if (old == 0u) {
+      h.list[atomicAdd(h.listed, 1u)] = (uint16_t)s;
+      return s;
+    }
+    if (old == j + 1u) return s;
+    s = (s + 1) & (kSlots - 1);
+  }
+}
+
+__device__ __forceinline__ void fill(const cf_answer_rules& R, const Row& w, const Hash& h) {
+  for (uint32_t i = threadIdx.x * 4; i < 3 * kSlots; i += blockDim.x * 4) *(uint4*)(h.key + i) = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) *h.listed = 0;
+  __syncthreads();
+  const int32_t n = (int32_t)R.n;
+  walk<4>(R.tokens_dev, w.h0, w.h1, [&](int32_t j, uint32_t at) {
+    if (j >= n) return;
+    const uint32_t s = slot_of(h, (uint32_t)j);
+    if (at >= w.answered)
+      atomicAdd(h.cnt + s, 1u);
+    else
+      atomicOr(h.cnt + s, kSeen << 16);
+  });
+  walk<4>(R.bias_ids_dev, w.b0, w.b1, [&](int32_t j, uint32_t at) {
+    if (j < n) atomicMax(h.pos + slot_of(h, (uint32_t)j), at - w.b0 + 1u);
+  });
+  __syncthreads();
+}
+
+// The answers that the history and the biases touch, in the result, after the stream: what is not
+// allowed stays -inf there, the others are their logits.  `ctas` a row: a short row is the first
+// one's, the slices of a long one are dealt out.
 template <typename T>
-__global__ void __launch_bounds__(kEditThreads)
-    k_answer_edits(const cf_answer_rules R, const T* in, int64_t in_rs, T* out, int64_t out_rs, int log_s, int slices) {
+__global__ void __launch_bounds__(512)
+    k_answer_edits(const cf_answer_rules R, T* out, int64_t out_rs, int log_s, int slices, int ctas) {
   extern __shared__ __align__(16) uint32_t smem[];
-  const int64_t r = blockIdx.x / slices;
-  const int slice = (int)(blockIdx.x - r * slices);
+  const int64_t r = blockIdx.x / ctas;
+  const int cta = (int)(blockIdx.x - r * ctas);
   const Row w = load_row(R, r);
   if (w.h0 == w.h1 && w.b0 == w.b1) return;
-  const T* x = in + r * in_rs;
   T* y = out + r * out_rs;
+  if (w.h1 - w.h0 + (w.b1 - w.b0) <= kShort) {
+    if (cta != 0) return;
+    const Hash h = hash_of(smem);
+    fill(R, w, h);
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the stream is done
+    constexpr int kBatch = 4;
+    const uint32_t listed = *h.listed;
+    for (uint32_t i = threadIdx.x; i < listed; i += kBatch * blockDim.x) {
+      int j[kBatch];
+      uint32_t c[kBatch], p[kBatch];
+      float bias[kBatch];
+      T v[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const bool ok = i + b * blockDim.x < listed;
+        const uint32_t s = ok ? h.list[i + b * blockDim.x] : 0u;
+        j[b] = ok ? (int)h.key[s] - 1 : -1;
+        c[b] = h.cnt[s];
+        p[b] = h.pos[s];
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        v[b] = j[b] >= 0 ? y[j[b]] : from_f32<T>(0.0f);
+        bias[b] = j[b] >= 0 && p[b] ? R.bias_values_dev[w.b0 + p[b] - 1u] : 0.0f;
+        if (j[b] >= 0 && !is_allowed(w.allowed, j[b])) j[b] = -1;
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        if (j[b] < 0) continue;
+        float e = edit(to_f32(v[b]), c[b] != 0, c[b] & kWideTimes, w.rep, w.freq, w.pres);
+        if (p[b]) e = __fadd_rn(e, bias[b]);
+        y[j[b]] = from_f32<T>(e);
+      }
+    }
+    return;
+  }
   Tables t = tables_of(w, smem, log_s);
   const int n = (int)R.n;
-  const int end = (int)min((int64_t)n, (int64_t)(slice + 1) << log_s);
   bool waited = false;
-  uint32_t size;
-  for (int lo = slice << log_s; lo < end; lo += (int)size) {
-    size = (uint32_t)min(1 << (t.wide ? log_s - 2 : log_s), end - lo);
-    if (waited) __syncthreads();  // the tables are filled anew
-    if (!count(R, w, t, lo, size)) {
-      t.wide = true;
-      size = 0;
-      __syncthreads();
-      continue;
+  for (int slice = cta; slice < slices; slice += ctas) {
+    const int end = (int)min((int64_t)n, (int64_t)(slice + 1) << log_s);
+    uint32_t size;
+    for (int lo = slice << log_s; lo < end; lo += (int)size) {
+      size = (uint32_t)min(1 << (t.wide ? log_s - 2 : log_s), end - lo);
+      if (waited) __syncthreads();  // the tables are filled anew
+      const bool done = count(R, w, t, lo, size);
+      if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // the stream is done
+      waited = true;
+      if (!done) {
+        t.wide = true;
+        size = 0;
+        continue;
+      }
+      if (w.b1 > w.b0) {
+        for_biased(R, w, t, lo, size, [&](int j, bool seen, uint32_t times, float bias) {
+          if (is_allowed(w.allowed, j))
+            y[j] = from_f32<T>(__fadd_rn(edit(to_f32(y[j]), seen, times, w.rep, w.freq, w.pres), bias));
+        });
+        __syncthreads();  // the marks
+      }
+      for_seen(w, t, lo, size, y, [&](int j, uint32_t times, float v) {
+        y[j] = from_f32<T>(edit(v, true, times, w.rep, w.freq, w.pres));
+      });
     }
-    if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // the stream is done
-    waited = true;
-    // What is not allowed stays -inf; the other logits are as they were, also where the result
-    // takes the logits' place.
-    for_biased(R, w, t, lo, size, [&](int j, bool seen, uint32_t times, float bias) {
-      if (is_allowed(w.allowed, j))
-        y[j] = from_f32<T>(__fadd_rn(edit(to_f32(x[j]), seen, times, w.rep, w.freq, w.pres), bias));
-    });
-    if (w.b1 > w.b0) __syncthreads();  // the marks
-    for_seen(w, t, lo, size, x, [&](int j, uint32_t times, float v) {
-      y[j] = from_f32<T>(edit(v, true, times, w.rep, w.freq, w.pres));
-    });
   }
 }
 
@@ -602,13 +718,18 @@ cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, v
                   R, (const T*)in, in_rs, (T*)out, out_rs, chunks, units));
   }
   if (!has_edits(R)) return CF_OK;
-  // 32768 answers a slice (64 KB of tables, three CTAs an SM), fewer where that leaves SMs idle
-  int log_s = 15;
-  while (log_s > 11 && R.rows * ceil_div(R.n, (int64_t)1 << log_s) < 148) --log_s;
+  // Rows of up to 2048 tokens on average: one small CTA a row, which counts while the stream runs.
+  // Longer ones: 32768 answers a slice (64 KB of tables, three CTAs an SM), fewer where that leaves
+  // SMs idle.
+  const bool brief = R.n_tokens <= R.rows * 2048;
+  int log_s = brief ? 14 : 15;
+  if (!brief)
+    while (log_s > 11 && R.rows * ceil_div(R.n, (int64_t)1 << log_s) < 148) --log_s;
   while (log_s > 11 && (int64_t)1 << (log_s - 1) >= R.n) --log_s;
-  const int slices = (int)ceil_div(R.n, (int64_t)1 << log_s);
-  return launch("k_answer_edits", k_answer_edits<T>, R.rows * slices, kEditThreads, tables_bytes(log_s), 0, stream, st,
-                R, (const T*)in, in_rs, (T*)out, out_rs, log_s, slices);
+  const int slices = (int)ceil_div(R.n, (int64_t)1 << log_s), ctas = brief ? 1 : slices;
+  const size_t tables = tables_bytes(log_s), smem = tables > kHashBytes ? tables : kHashBytes;
+  return launch("k_answer_edits", k_answer_edits<T>, R.rows * ctas, 512, smem, 0, stream, st, R, (T*)out,
+                out_rs, log_s, slices, ctas);
 }
 
 }  // namespace
@@ -644,14 +765,15 @@ extern "C" cf_status cf_answer_margin(const cf_answer_rules* R, const float* l, 
   if (R->rows == 0) return CF_OK;
   CF_REQUIRE(l && u && labels && margin && rival, CF_ERR_NULL, "answer_margin: NULL argument");
   CF_REQUIRE(((uintptr_t)l | (uintptr_t)u) % 4 == 0, CF_ERR_SHAPE, "answer_margin: unaligned rows");
-  // 16384 answers a slice, fewer for a short row or few rows; a cluster of up to eight for a row
+  // 16384 answers a slice, fewer for a short row or few rows; a cluster of up to eight for a row, as far
+  // as all rows' fit the GPU at once
   int log_s = 14;
   while (log_s > 11 && ((int64_t)1 << (log_s - 1) >= R->n ||
                         (R->rows * ceil_div(R->n, (int64_t)1 << log_s) < 148 && (int64_t)8 << (log_s - 1) >= R->n)))
     --log_s;
   const int slices = (int)ceil_div(R->n, (int64_t)1 << log_s);
   int cluster = 1;
-  while (cluster < kMaxCluster && cluster < slices) cluster *= 2;
+  while (cluster < kMaxCluster && cluster < slices && R->rows * cluster * 2 <= 148 * 4) cluster *= 2;
   return launch("k_answer_margin", k_answer_margin, R->rows * cluster, kMarginThreads,
                 has_edits(*R) ? tables_bytes(log_s) : 0, cluster, false, as_stream(stream), *R, l, l_rs, u, u_rs,
                 labels, margin, rival, log_s, slices);
