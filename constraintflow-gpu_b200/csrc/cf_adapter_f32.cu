@@ -467,8 +467,8 @@ template <bool kSub, bool kShrink, int kBN>
 cf_status launch(const Problem& p, Tiling g, cudaStream_t st) {
   constexpr int smem = kStages * 2 * (kBM + kBN) * 128 + kBM * (kBN + 4) * 4 + 1024;
   auto* kern = k_adapter_f32<kSub, kShrink, kBN>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "k_adapter_f32: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  CF_TRY(allow_smem(kern, smem, allowed, "k_adapter_f32"));
   g.split = split_for(kShrink ? g.m_tiles : g.units, ceil_div(p.K, kStep));
   // one CTA an SM walks over the tiles; a cluster has one
   g.clusters = g.split > 1 ? g.units : (g.units < 148 ? g.units : 148);
@@ -488,7 +488,7 @@ cf_status launch(const Problem& p, Tiling g, cudaStream_t st) {
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = g.dependent ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, p, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, g);
   if (e != cudaSuccess) {
     set_error("k_adapter_f32: %s", cudaGetErrorString(e));
     return CF_ERR_CUDA;

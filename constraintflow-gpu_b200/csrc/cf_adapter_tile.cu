@@ -300,8 +300,8 @@ cf_status launch(const char* what, const Problem& p, const Maps& maps, const Til
                  cudaStream_t st) {
   constexpr int smem = (kBM + kBN) * 128 * kStages + 1024;
   auto* kern = k_adapter_tile<T, kSub, kShrink, kBN, kStages>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  CF_TRY(allow_smem(kern, smem, allowed, what));
   const int64_t blocks = clusters * g.split;
   CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "%s: too many tiles", what);
   cudaLaunchConfig_t cfg = {};
@@ -317,7 +317,7 @@ cf_status launch(const char* what, const Problem& p, const Maps& maps, const Til
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = g.dependent ? 2 : 1;
-  e = cudaLaunchKernelEx(&cfg, kern, p, maps, g);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, maps, g);
   if (e != cudaSuccess) {
     set_error("%s: %s", what, cudaGetErrorString(e));
     return CF_ERR_CUDA;
@@ -333,8 +333,9 @@ cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cu
   Tiling g = {};
   g.m_tiles = m_tiles;
   g.x_rows = (int)(p.T < kBM ? ceil_div(p.T, 8) * 8 : kBM);
-  // float16's range does not hold every intermediate that float32 does: row by row instead
-  g.q_tma = dtype == CF_BF16 && lowrank_tma;
+  // Row by row: requests of few rows, and float16, whose range does not hold every intermediate that
+  // float32 does.
+  g.q_tma = dtype == CF_BF16 && lowrank_tma && !row_shrink;
   g.whole = g.q_tma ? 16 : 0;
   CF_TRY(encode(&maps.x, dtype, p.x, p.K, p.T, 1, p.x_rs, p.x_rs * p.T, g.x_rows));
   if (p.R > 0 && row_shrink) {

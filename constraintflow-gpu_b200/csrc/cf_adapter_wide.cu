@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 template <typename T, bool kSub>
 cf_status launch(const Problem& p, const Maps& maps, bool q_tma, int x_rows, cudaStream_t st) {
   auto* kern = k_adapter_wide<T, kSub>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "k_adapter_wide: cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+  static std::atomic<uint64_t> allowed{0};
+  CF_TRY(allow_smem(kern, kSmem, allowed, "k_adapter_wide"));
   const int64_t m_tiles = ceil_div(p.T, kBM), units = m_tiles * ceil_div(p.N, kBN);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units < 148 ? units : 148));
@@ -299,7 +299,7 @@ cf_status launch(const Problem& p, const Maps& maps, bool q_tma, int x_rows, cud
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.R > 0 ? 1 : 0;
-  e = cudaLaunchKernelEx(&cfg, kern, p, maps, m_tiles, units, (int)(q_tma && p.R > 0),
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p, maps, m_tiles, units, (int)(q_tma && p.R > 0),
                          (uint32_t)x_rows * 128u);
   if (e != cudaSuccess) {
     set_error("k_adapter_wide: %s", cudaGetErrorString(e));
