@@ -52,13 +52,24 @@ bool aligned(const Operand& o, int64_t size) {
 // (no columns of x: nothing to adapt)
 bool has_adapters(const cf_adapter_layer& L, int64_t K) { return L.n_adapters > 0 && L.rank > 0 && K > 0; }
 
+// A few rows go over the weights on the CUDA cores.  float32, against the tiles: 8 rows of 4096 x
+// 4096 19 us and 38, 16 rows 36 and 38; 64 rows of 200 x 784 7 and 21, 128 of 512 x 512 23 both.
+// 16-bit, rows of W along the contraction: 1 row of 4096 x 4096 5.4 and 11.2, 2 rows 7.3 and 11.0, 4
+// rows 11 both; 8 rows of 512 x 512 with adapters 5.5 and 8.6.  16-bit the other way: never (1 row of
+// 4096 x 4096 15 and 11).
+bool few_rows(const cf_adapter_layer& L, bool substitute, int64_t T) {
+  const double weights = (double)L.n_out * L.n_in;
+  if (L.dtype == CF_F32) return T <= 8 || (T <= 1024 && T * weights <= 16777216.0);
+  return !substitute && (T <= 2 || (T <= 8 && weights <= 1048576.0));
+}
+
 // With few rows a request, a tile of the tensor cores would be multiplied once for each of its
 // requests: v row by row on the CUDA cores instead.
 bool rows_alone(int64_t T, int64_t n_requests) { return T < 16 * n_requests; }
 
 // The workspace's parts, from `base` on (NULL: only their sizes are asked for); returns its bytes.
 // x, M, A and B are pointed to their copies where they have one.
-size_t workspace(const cf_adapter_layer& L, int64_t T, int64_t n_requests, Operand& x, Operand& W, Operand& A,
+size_t workspace(const cf_adapter_layer& L, bool substitute, int64_t T, int64_t n_requests, Operand& x, Operand& W, Operand& A,
                  Operand& B, char* base, Problem* p, Pack* pack) {
   if (T <= 0) return 0;
   const bool adapters = has_adapters(L, x.cols);
@@ -84,7 +95,7 @@ size_t workspace(const cf_adapter_layer& L, int64_t T, int64_t n_requests, Opera
       p->tile_e = (int32_t*)tile_e, p->tile_q = (int32_t*)tile_q;
     }
   }
-  if (L.dtype == CF_F32) return at;
+  if (L.dtype == CF_F32 || few_rows(L, substitute, T)) return at;
   auto copy = [&](Operand& o, int64_t cols) {  // rows of `cols` elements, zeros behind the data's
     if (aligned(o, 2)) return;
     const int64_t rs = ceil_div(cols, 8) * 8;
@@ -120,7 +131,7 @@ extern "C" size_t cf_adapter_workspace_bytes(const cf_adapter_layer* L, int32_t 
   if (!L || T <= 0) return 0;
   Operand ox = operand_x(x, T, substitute ? L->n_out : L->n_in, x_rs), W = operand_W(*L, substitute != 0), A = operand_A(*L),
           B = operand_B(*L);
-  return workspace(*L, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
+  return workspace(*L, substitute != 0, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
 }
 
 extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substitute, int64_t T, const void* x,
@@ -142,13 +153,13 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
               (uintptr_t)L->bias_dev) % size == 0,
              CF_ERR_SHAPE, "adapter_matmul: unaligned data");
   Operand ox = operand_x(x, T, K, x_rs), W = operand_W(*L, substitute != 0), A = operand_A(*L), B = operand_B(*L);
-  const size_t need = workspace(*L, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
+  const size_t need = workspace(*L, substitute != 0, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
   CF_REQUIRE(ws_bytes >= need && (need == 0 || ws), CF_ERR_WORKSPACE, "adapter_matmul: workspace of %zu bytes, needs %zu",
              ws_bytes, need);
   CF_REQUIRE((uintptr_t)ws % 256 == 0, CF_ERR_WORKSPACE, "adapter_matmul: the workspace must be 256-byte aligned");
   Problem p = {};
   Pack pack = {};
-  workspace(*L, T, n_requests, ox, W, A, B, (char*)ws, &p, &pack);
+  workspace(*L, substitute != 0, T, n_requests, ox, W, A, B, (char*)ws, &p, &pack);
   p.T = T, p.K = K, p.N = N;
   p.R = adapters ? L->rank : 0, p.E = adapters ? L->n_adapters : 0, p.Q = n_requests;
   p.x = ox.p, p.x_rs = ox.rs, p.M = W.p, p.y = y, p.y_rs = y_rs;
@@ -172,6 +183,7 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   p.p_vec = substitute ? b_vec : a_vec;
   p.q_vec = substitute ? a_vec : b_vec;
   p.y_vec = vec(y, T > 1 ? y_rs : 0, 0);
+  if (few_rows(*L, substitute != 0, T)) return launch_gemv(p, L->dtype, substitute != 0, as_stream(stream));
   const bool rows = rows_alone(T, n_requests);
   if (L->dtype == CF_F32) return launch_f32(p, substitute != 0, rows, as_stream(stream));
   CF_TRY(launch_pack(pack, as_stream(stream)));

@@ -195,6 +195,8 @@ cf_status launch_tiles(const Problem& p, int dtype, bool substitute, bool row_sh
                        cudaStream_t st);
 // float32 data (cf_adapter_f32.cu)
 cf_status launch_f32(const Problem& p, bool substitute, bool row_shrink, cudaStream_t st);
+// a few rows, whatever the alignment, with v row by row (cf_adapter_gemv.cu); substitute: float32
+cf_status launch_gemv(const Problem& p, int dtype, bool substitute, cudaStream_t st);
 // v row by row, and the plan of the row tiles (cf_adapter_rows.cu)
 cf_status launch_row_shrink(const Problem& p, int dtype, bool substitute, int whole, cudaStream_t st);
 // the first site at which a bounded device wait gave up since the last call on this device (0: none)

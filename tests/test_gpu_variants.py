@@ -249,6 +249,22 @@ def test_adapter_few_rows_many_columns(dtype, sub):
 
 @pytest.mark.parametrize("sub", [False, True])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17])
+def test_adapter_few_rows(dtype, sub, T):
+    """A few rows of a layer wide enough that its contraction is shared, aligned and not."""
+    for K, N, R, Q in ((2048, 264, 16, T), (1027, 131, 5, 2), (72, 1000, 8, 1)):
+        t = make(T, K, N, R, 3, Q, dtype, sub, seed=T + K, style="tokens", ranks=True, bias=True)
+        compare(t, sub)
+        t["offsets"] = torch.clamp(t["offsets"] - 1, min=0)      # the last row is no request's
+        before = torch.randn(T, N, generator=gen(T)).to(dtype)
+        y, tol = oracle(t, sub, out=before)
+        got = ops().adapter_matmul(t["x"].cuda(), layer(t), t["offsets"].cuda(), t["ids"].cuda(), substitute=sub,
+                                   out=before.cuda())
+        V.check(got, y, tol)
+
+
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_a_contraction_over_nothing(dtype, sub):
     o = ops()
     n_out, n_in = (0, 24) if sub else (24, 0)
