@@ -311,6 +311,8 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
     key = (substitute, T, Q, xp % 16, rs)
     need = layer._need.get(key)
     if need is None:
+        if len(layer._need) >= 4096:
+            layer._need.clear()
         need = layer._need[key] = _lib.lib.cf_adapter_workspace_bytes(layer._ref, 1 if substitute else 0, T, xp, rs, Q)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own

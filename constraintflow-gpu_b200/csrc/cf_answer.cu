@@ -412,10 +412,13 @@ __global__ void __launch_bounds__(512)
   const int64_t r = blockIdx.x / ctas;
   const int cta = (int)(blockIdx.x - r * ctas);
   const Row w = load_row(R, r);
-  if (w.h0 == w.h1 && w.b0 == w.b1) return;
+  const bool brief = w.h1 - w.h0 + (w.b1 - w.b0) <= kShort;
+  if ((w.h0 == w.h1 && w.b0 == w.b1) || (brief && cta != 0)) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid's end must not come before the stream's
+    return;
+  }
   T* y = out + r * out_rs;
-  if (w.h1 - w.h0 + (w.b1 - w.b0) <= kShort) {
-    if (cta != 0) return;
+  if (brief) {
     const Hash h = hash_of(smem);
     fill(R, w, h);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the stream is done
@@ -749,6 +752,9 @@ extern "C" cf_status cf_edit_logits(const cf_answer_rules* R, int32_t dtype, con
              dtype);
   if (R->rows * R->n == 0) return CF_OK;
   CF_REQUIRE(in && out, CF_ERR_NULL, "edit_logits: NULL argument");
+  CF_REQUIRE((in == out && (R->rows == 1 || in_rs == out_rs)) ||
+                 !rows_overlap(in, in_rs, R->n, out, out_rs, R->n, R->rows, dtype == CF_F32 ? 4 : 2),
+             CF_ERR_SHAPE, "edit_logits: the logits and the result overlap");
   if (dtype == CF_F32) return edit_logits<float>(*R, in, in_rs, out, out_rs, as_stream(stream));
   if (dtype == CF_BF16) return edit_logits<__nv_bfloat16>(*R, in, in_rs, out, out_rs, as_stream(stream));
   return edit_logits<__half>(*R, in, in_rs, out, out_rs, as_stream(stream));

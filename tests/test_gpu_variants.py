@@ -407,6 +407,71 @@ def test_long_history_and_many_rows():
     same(got, V.rules(x, n, dtype=F32, **kw))
 
 
+def one_history(n, lens, biases, seed, tops=()):
+    """A row for each of `lens` tokens; `tops`: (row, answer, times) answered beyond the random ones."""
+    g = gen(seed)
+    rows = [torch.randint(0, n, (m,), generator=g) for m in lens]
+    for r, j, times in tops:
+        rows[r] = torch.cat([rows[r], torch.full((times,), j, dtype=torch.int64)])
+    count = torch.tensor([0] + [len(r) for r in rows])
+    R = len(rows)
+    ids = [torch.randint(0, n, (b,), generator=g) for b in biases]
+    return dict(tokens=torch.cat(rows).to(torch.int32), token_offsets=count.cumsum(0),
+                repetition=torch.rand(R, generator=g) + 0.6, frequency=torch.rand(R, generator=g) * 0.01,
+                presence=torch.rand(R, generator=g), bias_ids=torch.cat(ids).to(torch.int32),
+                bias_values=torch.randn(sum(biases), generator=g),
+                bias_offsets=torch.tensor([0] + list(biases)).cumsum(0))
+
+
+HISTORIES = [
+    # at the most that a row's own small table holds, and one more; repeated and distinct answers
+    (5000, [3072, 3073, 3000, 3000, 0, 0], [0, 0, 72, 73, 3072, 3073], ()),
+    (3072, [2048, 2049, 1, 0], [1024, 1024, 0, 1], ()),
+    # more biases than are compared one by one; one answer more often than 15 bits count
+    (9001, [10, 4000, 5000], [1025, 1024, 1500], ()),
+    (40000, [100, 5000, 0], [3, 2, 0], ((0, 77, 32767), (1, 39999, 32768), (2, 5, 70000))),
+    (70001, [4096, 4097], [0, 9], ((0, 0, 40000), (1, 1, 32769), (1, 70000, 32769))),
+]
+
+
+@pytest.mark.parametrize("case", range(len(HISTORIES)))
+def test_histories_at_the_tables_limits(case):
+    n, lens, biases, tops = HISTORIES[case]
+    rows = len(lens)
+    kw = one_history(n, lens, biases, case, tops)
+    x = torch.randn(rows, n, generator=gen(case)) * 3
+    rules = ops().AnswerRules(rows, n, **on_gpu(kw))
+    same(ops().edit_logits(x.cuda(), rules), V.rules(x, n, dtype=F32, **kw))
+    labels = kw["tokens"][kw["token_offsets"][:-1].clamp(max=len(kw["tokens"]) - 1)].long()
+    m, j = V.margin(x - 0.5, x + 0.5, labels, n, **kw)
+    gm, gj = ops().answer_margin((x - 0.5).cuda(), (x + 0.5).cuda(), labels.cuda(), rules)
+    same(gm, m)
+    assert torch.equal(gj.cpu(), j)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lens", [[0] * 64, [3] + [0] * 63, [9000] + [0] * 63], ids=["none", "one", "long"])
+def test_the_result_may_be_used_at_once(dtype, lens):
+    """Rows without a history end at once; what follows on the stream still finds the whole result,
+    and nothing is written after it."""
+    n = 100003
+    kw = one_history(n, lens, [0] * 64, 3)
+    x = torch.randn(64, n, generator=gen(1)).to(dtype)
+    want = V.rules(x[:1].float(), n, dtype=F32, tokens=kw["tokens"], token_offsets=kw["token_offsets"][:2],
+                   **{k: kw[k][:1] for k in ("repetition", "frequency", "presence")}).to(dtype)
+    xd, rules, out = x.cuda(), ops().AnswerRules(64, n, **on_gpu(kw)), torch.empty(64, n, dtype=dtype, device="cuda")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            ops().edit_logits(xd, rules, out=out)
+            got = out.clone()
+            out.zero_()
+            assert torch.equal(got[1:], xd[1:])
+            same(got[:1].float(), want.float())
+            assert not out.any()
+
+
 def test_offsets_are_held_within_their_lists():
     n = 50
     kw = dict(tokens=torch.arange(10, dtype=torch.int32), token_offsets=torch.tensor([-5, 4, 2, 1 << 40]),
@@ -531,6 +596,41 @@ def test_adapters_then_rules():
     assert torch.equal(rival.cpu(), wj)
     ok = (v.gather(1, best[:, None])[:, 0] > -math.inf).cpu()
     assert (m.cpu()[ok] >= 0).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_beside_their_results(dtype):
+    """x and y as columns of one buffer, logits and result too."""
+    t = make(37, 40, 56, 8, 3, 4, dtype, False, seed=51)
+    buf = torch.full((37, 120), 7.0, dtype=dtype, device="cuda")
+    buf[:, 8:48] = t["x"].cuda()
+    out = buf[:, 48:104]
+    out.zero_()
+    ops().adapter_matmul(buf[:, 8:48], layer(t), t["offsets"].cuda(), t["ids"].cuda(), out=out)
+    V.check(out, *oracle(t, False))
+    assert (buf[:, :8] == 7).all() and (buf[:, 104:] == 7).all()
+    kw = make_rules(37, 50, seed=52, hist=9, biases=3, masks=2)
+    x = torch.randn(37, 50, generator=gen(2)).to(dtype)
+    buf[:, 1:51] = x.cuda()
+    ops().edit_logits(buf[:, 1:51], ops().AnswerRules(37, 50, **on_gpu(kw)), out=buf[:, 51:101])
+    same(buf[:, 51:101].float(), V.rules(x.float(), 50, dtype=F32, **kw).to(dtype).float())
+    assert (buf[:, :1] == 7).all() and torch.equal(buf[:, 1:51].cpu(), x)
+
+
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T,Q", [(3, 2), (40, 2), (300, 200)])
+def test_broadcast_operands(dtype, sub, T, Q):
+    """One row of x for all rows, and one adapter's tensors under every id."""
+    t = make(T, 64, 72, 8, 3, Q, dtype, sub, seed=61)
+    t["x"] = t["x"][:1].expand(T, 64)
+    t["A"], t["B"] = t["A"][:1].expand(3, -1, -1), t["B"][:1].expand(3, -1, -1)
+    d = {k: t[k].cuda() for k in ("W", "scale", "offsets", "ids")}
+    A, B = t["A"][:1].contiguous().cuda().expand(3, -1, -1), t["B"][:1].contiguous().cuda().expand(3, -1, -1)
+    x = t["x"][:1].contiguous().cuda().expand(T, 64)
+    L = ops().AdapterLayer(d["W"], A, B, d["scale"])
+    V.check(ops().adapter_matmul(x, L, d["offsets"], d["ids"], substitute=sub), *oracle(t, sub))
+    ops().adapter_check()
 
 
 @pytest.mark.parametrize("sub", [False, True])

@@ -85,6 +85,27 @@ def test_edit_and_margin_refusals():
     assert e(ctypes.byref(c_rules(n=0)), _lib.CF_F32, None, 0, None, 0, None) == _lib.CF_OK
 
 
+def test_overlapping_rows_are_refused():
+    S = _lib.CF_ERR_SHAPE
+    # y within x, x within y, one element of both, for rows at one stride and at two
+    for x, x_rs, y, y_rs in ((256, 16, 256, 32), (256, 16, 300, 32), (512, 16, 256, 32), (256, 48, 258, 48),
+                             (256, 48, 256 + 30, 48), (256, 0, 286, 32), (256, 47, 256 + 32, 47)):
+        assert call(c_layer(), x=x, x_rs=x_rs, y=y, y_rs=y_rs) == S, (x, x_rs, y, y_rs)
+    e, ref = _lib.lib.cf_edit_logits, ctypes.byref(c_rules())
+    for x, x_rs, y, y_rs in ((256, 10, 260, 10), (300, 10, 256, 10), (256, 0, 256, 10), (256, 12, 256, 10),
+                             (256, 19, 296, 19)):
+        assert e(ref, _lib.CF_F32, x, x_rs, y, y_rs, None) == S, (x, x_rs, y, y_rs)
+    assert b"overlap" in _lib.lib.cf_last_error()
+
+
+def test_rules_fault_injection(monkeypatch):
+    ref = ctypes.byref(c_rules())
+    monkeypatch.setenv("CF_FAULT", "edit_logits")
+    assert _lib.lib.cf_edit_logits(ref, _lib.CF_F32, 256, 10, 4096, 10, None) == _lib.CF_ERR_INJECTED
+    monkeypatch.setenv("CF_FAULT", "answer_margin")
+    assert _lib.lib.cf_answer_margin(ref, 256, 10, 256, 10, 256, 256, 256, None) == _lib.CF_ERR_INJECTED
+
+
 def test_cpu_tensors_are_refused():
     W, A, B = torch.zeros(4, 4), torch.zeros(1, 2, 4), torch.zeros(1, 4, 2)
     with pytest.raises(RuntimeError, match="CUDA"):
