@@ -1,7 +1,6 @@
 // What the tensor-core kernels of the adapter product share: operand images, stores, the
 // row-by-row low-rank part.
 #pragma once
-#include <atomic>
 
 #include "cf_adapter.cuh"
 #include "cf_tc.cuh"
@@ -209,20 +208,6 @@ __device__ __forceinline__ void add_lowrank16(const Problem& p, int64_t t, int e
         if (n + c < p.N) a[c] = fmaf(w, to_f32(Q[(n + c) * p.q_ns + r]), a[c]);
     }
   }
-}
-
-// Allow `bytes` of dynamic shared memory to a kernel, once a device (`done`: one word a kernel).
-template <typename F>
-cf_status allow_smem(F* kern, int bytes, std::atomic<uint64_t>& done, const char* what) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
-  if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
-  }
-  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
-  return CF_OK;
 }
 
 // Read and clear a kernel file's error word.

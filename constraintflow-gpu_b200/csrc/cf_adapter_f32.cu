@@ -242,32 +242,64 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       ++it;
       return true;
     };
+    // A tile's steps: the contraction's, then those of its requests' low-rank parts, the next one's
+    // loads in flight while a step's are split and stored.
+    int k = 0;
+    uint32_t todo = 0;  // of the 32 requests from `from` on, those that have an adapter and rows here
+    int from = 0, e = kNone, r = 0, r0 = 0;
+    bool begun = false, past = true;
+    auto look = [&] {
+      const Reach at = reach(p, w.m, from);
+      todo = __ballot_sync(0xffffffffu, at.r > 0);
+      past = __any_sync(0xffffffffu, at.past);
+    };
+    auto next = [&](auto vec, Chunks<kBN>& d) -> bool {
+      if (k < ke) {
+        fetch(vec, d, w, k++);
+        return true;
+      }
+      if (!lowrank) return false;
+      if (!begun) {
+        begun = true;
+        if (!waited) dependency_wait();
+        waited = true;
+        from = p.tile_q[w.m];
+        r = 0;
+        look();
+      }
+      r0 += kStep;
+      if (r0 >= r) {
+        while (todo == 0) {
+          if (past) return false;
+          from += 32;
+          look();
+        }
+        const int i = __ffs(todo) - 1;
+        todo &= todo - 1;
+        e = adapter_of(p, from + i);
+        r = rank_of(p, e);
+        r0 = 0;
+      }
+      // rows of v are 16-byte aligned and zero from the rank to the next multiple of 4
+      fetch_x(std::true_type{}, d.x, p.v, p.v_rs, w.t0, r0, r);
+      fetch_b(std::false_type{}, d.b, (const float*)p.Qm + e * p.q_es + w.n0 * p.q_ns, p.q_rs, p.q_ns,
+              (int)min(p.N - w.n0, (int64_t)kBN), r0, r);
+      return true;
+    };
     auto tiles = [&](auto vec) {
       for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
         if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
+        k = kb;
+        begun = false;
         Chunks<kBN> one, two;
-        if (kb < ke) fetch(vec, one, w, kb);
-        for (int k = kb; k < ke && ok; k += 2) {
-          if (k + 1 < ke) fetch(vec, two, w, k + 1);
+        bool more = next(vec, one);
+        while (more) {
+          more = next(vec, two);
           ok = store(one);
-          if (!ok || k + 1 >= ke) break;
-          if (k + 2 < ke) fetch(vec, one, w, k + 2);
+          if (!ok || !more) break;
+          more = next(vec, one);
           ok = store(two);
-        }
-        if (lowrank && ok) {
-          if (!waited) dependency_wait();
-          waited = true;
-          const int from = p.tile_q[w.m];
-          ok = for_requests(p, w.m, from, reach(p, w.m, from), [&](int e, int r, int, int) {
-            for (int r0 = 0; r0 < r; r0 += kStep) {
-              // rows of v are 16-byte aligned and zero from the rank to the next multiple of 4
-              fetch_x(std::true_type{}, one.x, p.v, p.v_rs, w.t0, r0, r);
-              fetch_b(std::false_type{}, one.b, (const float*)p.Qm + e * p.q_es + w.n0 * p.q_ns, p.q_rs, p.q_ns,
-                      (int)min(p.N - w.n0, (int64_t)kBN), r0, r);
-              if (!store(one)) return false;
-            }
-            return true;
-          });
+          if (!ok) break;
         }
       }
     };

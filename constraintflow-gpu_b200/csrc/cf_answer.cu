@@ -118,6 +118,8 @@ struct Tables {
   bool wide, listing;
 };
 
+constexpr int kMostSmem = (2 << 15) + (1 << 12) + 16 + kList * 2 + kMaxBiases * 4;  // of slices of 32768
+
 size_t tables_bytes(int log_s) {
   return ((size_t)2 << log_s) + ((size_t)1 << (log_s - 3)) + 16 + kList * 2 + kMaxBiases * 4;
 }
@@ -647,14 +649,12 @@ bool has_edits(const cf_answer_rules& R) {
   return (R.tokens_dev && R.n_tokens > 0) || (R.bias_ids_dev && R.n_biases > 0);
 }
 
+// `allowed`: the devices on which the kernel may have kMostSmem bytes (nullptr: it needs no more than 48 KB)
 template <typename F, typename... Args>
-cf_status launch(const char* what, F* kern, int64_t blocks, int threads, size_t smem, int cluster, bool dependent,
-                 cudaStream_t st, Args... args) {
+cf_status launch(const char* what, F* kern, std::atomic<uint64_t>* allowed, int64_t blocks, int threads, size_t smem,
+                 int cluster, bool dependent, cudaStream_t st, Args... args) {
   CF_REQUIRE(blocks <= 0x7fffffff, CF_ERR_SHAPE, "%s: too many rows", what);
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
-  }
+  if (smem > 48 * 1024) CF_TRY(allow_smem(kern, kMostSmem, *allowed, what));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)threads);
@@ -717,7 +717,7 @@ cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, v
   if (stream) {
     const int chunks = (int)ceil_div(R.n + V - 1, kChunk);
     const int64_t units = R.rows * chunks, most = 148 * 4;  // four CTAs an SM
-    CF_TRY(launch("k_answer_stream", k_answer_stream<T>, units < most ? units : most, kStreamThreads, 0, 0, false, st,
+    CF_TRY(launch("k_answer_stream", k_answer_stream<T>, nullptr, units < most ? units : most, kStreamThreads, 0, 0, false, st,
                   R, (const T*)in, in_rs, (T*)out, out_rs, chunks, units));
   }
   if (!has_edits(R)) return CF_OK;
@@ -731,7 +731,8 @@ cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, v
   while (log_s > 11 && (int64_t)1 << (log_s - 1) >= R.n) --log_s;
   const int slices = (int)ceil_div(R.n, (int64_t)1 << log_s), ctas = brief ? 1 : slices;
   const size_t tables = tables_bytes(log_s), smem = tables > kHashBytes ? tables : kHashBytes;
-  return launch("k_answer_edits", k_answer_edits<T>, R.rows * ctas, 512, smem, 0, stream, st, R, (T*)out,
+  static std::atomic<uint64_t> allowed{0};
+  return launch("k_answer_edits", k_answer_edits<T>, &allowed, R.rows * ctas, 512, smem, 0, stream, st, R, (T*)out,
                 out_rs, log_s, slices, ctas);
 }
 
@@ -780,7 +781,8 @@ extern "C" cf_status cf_answer_margin(const cf_answer_rules* R, const float* l, 
   const int slices = (int)ceil_div(R->n, (int64_t)1 << log_s);
   int cluster = 1;
   while (cluster < kMaxCluster && cluster < slices && R->rows * cluster * 2 <= 148 * 4) cluster *= 2;
-  return launch("k_answer_margin", k_answer_margin, R->rows * cluster, kMarginThreads,
+  static std::atomic<uint64_t> allowed{0};
+  return launch("k_answer_margin", k_answer_margin, &allowed, R->rows * cluster, kMarginThreads,
                 has_edits(*R) ? tables_bytes(log_s) : 0, cluster, false, as_stream(stream), *R, l, l_rs, u, u_rs,
                 labels, margin, rival, log_s, slices);
 }

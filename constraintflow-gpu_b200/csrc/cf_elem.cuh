@@ -1,9 +1,13 @@
 // Element types of the operators that take float32, bfloat16 or float16 data: loads to
-// float32, stores rounded once to nearest even.
+// float32, stores rounded once to nearest even; and what their entry points share.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
+
+#include <atomic>
+
+#include "cf_common.cuh"
 
 namespace cf {
 
@@ -24,6 +28,20 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) {
   return __float2half_rn(x);
+}
+
+// Allow `bytes` of dynamic shared memory to a kernel, once a device (`done`: one word a kernel).
+template <typename F>
+cf_status allow_smem(F* kern, int bytes, std::atomic<uint64_t>& done, const char* what) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (e == cudaSuccess && !(done.load(std::memory_order_relaxed) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  }
+  CF_REQUIRE(e == cudaSuccess, CF_ERR_CUDA, "%s: cudaFuncSetAttribute: %s", what, cudaGetErrorString(e));
+  return CF_OK;
 }
 
 // Whether rows of a (at a_rs elements) and rows of b share memory: their ranges do, unless the rows
