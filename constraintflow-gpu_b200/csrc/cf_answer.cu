@@ -166,6 +166,18 @@ __device__ __forceinline__ bool count(const cf_answer_rules& R, const Row& w, co
   if (!t.wide)
     for (uint32_t i = w.b0 + threadIdx.x; i < w.b1; i += blockDim.x) t.ids[i - w.b0] = R.bias_ids_dev[i];
   __syncthreads();
+  if (!t.wide && !t.listing && w.h1 - min(w.h1, w.answered) <= kTimes) {  // nothing to be told by the old count
+    walk<8>(R.tokens_dev, w.h0, w.h1, [&](int32_t j, uint32_t h) {
+      const uint32_t k = (uint32_t)(j - lo), sh = (k & 1) * 16;
+      if (k >= size) return;
+      if (h >= w.answered)
+        atomicAdd(t.words + (k >> 1), 1u << sh);
+      else
+        atomicOr(t.words + (k >> 1), kSeen << sh);
+    });
+    __syncthreads();
+    return true;
+  }
   walk<8>(R.tokens_dev, w.h0, w.h1, [&](int32_t j, uint32_t h) {
     const uint32_t k = (uint32_t)(j - lo);
     if (k >= size) return;
@@ -275,6 +287,77 @@ __device__ __forceinline__ void for_seen(const Row& w, const Tables& t, int lo, 
   }
 }
 
+// What a short row touches: open addressing over the answers.
+// kShort tokens and biases of a row at most, kMarginShort for its margin (whose CTAs, four an SM, all run at
+// once, and read through what the tables leave of the L1 cache).
+constexpr uint32_t kSlots = 4096, kShort = 3072, kMarginSlots = 2048, kMarginShort = 1536;
+
+struct Hash {
+  int log_n;  // 1 << log_n slots, twice a row's tokens and biases where there are that many
+  uint32_t *key, *cnt, *pos;  // answer + 1 (0: free); times and, highest bit, seen; place of the last bias
+  uint32_t* listed;
+  uint16_t* list;  // slots in use
+};
+
+constexpr size_t hash_bytes(uint32_t slots, uint32_t most) { return slots * 12 + 16 + most * 2; }
+
+template <uint32_t kMost>
+__device__ __forceinline__ bool is_short(const Row& w) {
+  return w.h1 - w.h0 + (w.b1 - w.b0) <= kMost;
+}
+
+__device__ __forceinline__ Hash hash_of(const Row& w, uint32_t* smem, uint32_t slots) {
+  Hash h;
+  h.log_n = min(max(33 - __clz((int)(w.h1 - w.h0 + (w.b1 - w.b0))), 6), 31 - __clz((int)slots));
+  h.key = smem;
+  h.cnt = smem + (1u << h.log_n);
+  h.pos = smem + (2u << h.log_n);
+  h.listed = smem + (3u << h.log_n);
+  h.list = (uint16_t*)(h.listed + 4);
+  return h;
+}
+
+// The slot of answer j; the first to come to it lists it.
+__device__ __forceinline__ uint32_t slot_of(const Hash& h, uint32_t j) {
+  uint32_t s = j * 2654435761u >> (32 - h.log_n);  // by the golden ratio
+  for (;;) {
+    const uint32_t old = atomicCAS(h.key + s, 0u, j + 1u);
+    if (old == 0u) {
+      h.list[atomicAdd(h.listed, 1u)] = (uint16_t)s;
+      return s;
+    }
+    if (old == j + 1u) return s;
+    s = (s + 1) & ((1u << h.log_n) - 1);
+  }
+}
+
+// Whether the table holds answer j.
+__device__ __forceinline__ bool holds(const Hash& h, uint32_t j) {
+  for (uint32_t s = j * 2654435761u >> (32 - h.log_n);; s = (s + 1) & ((1u << h.log_n) - 1)) {
+    const uint32_t key = h.key[s];
+    if (key == 0u || key == j + 1u) return key != 0u;
+  }
+}
+
+__device__ __forceinline__ void fill(const cf_answer_rules& R, const Row& w, const Hash& h) {
+  for (uint32_t i = threadIdx.x * 4; i < 3u << h.log_n; i += blockDim.x * 4) *(uint4*)(h.key + i) = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x == 0) *h.listed = 0;
+  __syncthreads();
+  const int32_t n = (int32_t)R.n;
+  walk<4>(R.tokens_dev, w.h0, w.h1, [&](int32_t j, uint32_t at) {
+    if (j >= n) return;
+    const uint32_t s = slot_of(h, (uint32_t)j);
+    if (at >= w.answered)
+      atomicAdd(h.cnt + s, 1u);
+    else
+      atomicOr(h.cnt + s, kSeen << 16);
+  });
+  walk<4>(R.bias_ids_dev, w.b0, w.b1, [&](int32_t j, uint32_t at) {
+    if (j < n) atomicMax(h.pos + slot_of(h, (uint32_t)j), at - w.b0 + 1u);
+  });
+  __syncthreads();
+}
+
 // 16 bytes of a row, moved whole.  Rows are read once, past the cache; what is written stays there
 // for the edits behind.
 template <typename T>
@@ -350,78 +433,24 @@ __global__ void __launch_bounds__(kStreamThreads)
   }
 }
 
-// ---- what a short row touches: open addressing over the answers
-constexpr uint32_t kSlots = 4096, kShort = 3072;  // tokens and biases of a row at most
-
-struct Hash {
-  uint32_t *key, *cnt, *pos;  // answer + 1 (0: free); times and, highest bit, seen; place of the last bias
-  uint32_t* listed;
-  uint16_t* list;  // slots in use
-};
-
-constexpr size_t kHashBytes = kSlots * 12 + 16 + kShort * 2;
-
-__device__ __forceinline__ Hash hash_of(uint32_t* smem) {
-  Hash h;
-  h.key = smem;
-  h.cnt = smem + kSlots;
-  h.pos = smem + 2 * kSlots;
-  h.listed = smem + 3 * kSlots;
-  h.list = (uint16_t*)(h.listed + 4);
-  return h;
-}
-
-// The slot of answer j; the first to come to it lists it.
-__device__ __forceinline__ uint32_t slot_of(const Hash& h, uint32_t j) {
-  uint32_t s = j * 2654435761u >> 20;  // of 4096, by the golden ratio
-  for (;;) {
-    const uint32_t old = atomicCAS(h.key + s, 0u, j + 1u);
-    if (old == 0u) {
-      h.list[atomicAdd(h.listed, 1u)] = (uint16_t)s;
-      return s;
-    }
-    if (old == j + 1u) return s;
-    s = (s + 1) & (kSlots - 1);
-  }
-}
-
-__device__ __forceinline__ void fill(const cf_answer_rules& R, const Row& w, const Hash& h) {
-  for (uint32_t i = threadIdx.x * 4; i < 3 * kSlots; i += blockDim.x * 4) *(uint4*)(h.key + i) = make_uint4(0, 0, 0, 0);
-  if (threadIdx.x == 0) *h.listed = 0;
-  __syncthreads();
-  const int32_t n = (int32_t)R.n;
-  walk<4>(R.tokens_dev, w.h0, w.h1, [&](int32_t j, uint32_t at) {
-    if (j >= n) return;
-    const uint32_t s = slot_of(h, (uint32_t)j);
-    if (at >= w.answered)
-      atomicAdd(h.cnt + s, 1u);
-    else
-      atomicOr(h.cnt + s, kSeen << 16);
-  });
-  walk<4>(R.bias_ids_dev, w.b0, w.b1, [&](int32_t j, uint32_t at) {
-    if (j < n) atomicMax(h.pos + slot_of(h, (uint32_t)j), at - w.b0 + 1u);
-  });
-  __syncthreads();
-}
-
 // The answers that the history and the biases touch, in the result, after the stream: what is not
 // allowed stays -inf there, the others are their logits.  `ctas` a row: a short row is the first
 // one's, the slices of a long one are dealt out.
-template <typename T>
-__global__ void __launch_bounds__(512)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads)
     k_answer_edits(const cf_answer_rules R, T* out, int64_t out_rs, int log_s, int slices, int ctas) {
   extern __shared__ __align__(16) uint32_t smem[];
   const int64_t r = blockIdx.x / ctas;
   const int cta = (int)(blockIdx.x - r * ctas);
   const Row w = load_row(R, r);
-  const bool brief = w.h1 - w.h0 + (w.b1 - w.b0) <= kShort;
+  const bool brief = is_short<kShort>(w);
   if ((w.h0 == w.h1 && w.b0 == w.b1) || (brief && cta != 0)) {
     asm volatile("griddepcontrol.wait;" ::: "memory");  // this grid's end must not come before the stream's
     return;
   }
   T* y = out + r * out_rs;
   if (brief) {
-    const Hash h = hash_of(smem);
+    const Hash h = hash_of(w, smem, kSlots);
     fill(R, w, h);
     asm volatile("griddepcontrol.wait;" ::: "memory");  // the stream is done
     constexpr int kBatch = 4;
@@ -493,8 +522,10 @@ struct Best {
 };
 
 // the larger value; the lower answer on equal ones
+__device__ __forceinline__ bool beats(float v, int32_t j, const Best& a) { return v > a.v || (v == a.v && j < a.j); }
+
 __device__ __forceinline__ void take(Best& a, float v, int32_t j) {
-  if (v > a.v || (v == a.v && j < a.j)) {
+  if (beats(v, j, a)) {
     a.v = v;
     a.j = j;
   }
@@ -503,6 +534,13 @@ __device__ __forceinline__ void take(Best& a, float v, int32_t j) {
 constexpr int32_t kNone = INT32_MAX;
 constexpr int kMarginThreads = 256, kMaxCluster = 8;
 
+// floats as integers of the same order, and back
+__device__ __forceinline__ int to_ordered(float v) {
+  const int i = __float_as_int(v);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float from_ordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+
 // the larger, NaN if one is
 __device__ __forceinline__ float max_nan(float a, float b) {
   float m;
@@ -510,9 +548,10 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return m;
 }
 
-// One cluster per row, a slice a CTA: the label's edited lower bound less the best edited upper
-// bound among the other answers.  On the way over the bounds a vector is looked into only where it
-// holds something above the best so far; what is touched is left to its own pass.
+// One cluster per row: the label's edited lower bound less the best edited upper bound among the
+// other answers.  Each CTA has a share of the answers (of a row with a long history, slices); what
+// is touched has its own pass, and on the way over the bounds a vector is looked into only where it
+// holds something above the best so far.
 __global__ void __launch_bounds__(kMarginThreads, 4)
     k_answer_margin(const cf_answer_rules R, const float* __restrict__ l, int64_t l_rs, const float* __restrict__ u,
                     int64_t u_rs, const int64_t* __restrict__ labels, float* margin, int32_t* rival, int log_s,
@@ -520,10 +559,13 @@ __global__ void __launch_bounds__(kMarginThreads, 4)
   extern __shared__ __align__(16) uint32_t smem[];
   __shared__ Best part_best[kMarginThreads / 32];
   __shared__ Best joined[kMaxCluster];
+  __shared__ float joined_l[kMaxCluster];
   __shared__ float label_l;
+  __shared__ int heard;  // the best of the CTA's warps, as far as told
   constexpr int V = 4, kVpt = 4, kChunk = kMarginThreads * V * kVpt;
   cg::cluster_group cl = cg::this_cluster();
-  const int nc = (int)cl.num_blocks(), n = (int)R.n;
+  const int nc = (int)cl.num_blocks(), rank = (int)cl.block_rank(), n = (int)R.n;
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // this CTA runs; awaited at the end
   const int64_t r = blockIdx.x / nc;
   const float* x = u + r * u_rs;
   const int mis = (int)(((uintptr_t)x & 15) / 4);
@@ -543,30 +585,91 @@ __global__ void __launch_bounds__(kMarginThreads, 4)
 #pragma unroll
     for (int i = 0; i < kVpt; ++i) load(i, j0, end);
   };
-  // a slice's answers [lo, end), the first vector's place
+  // of answers [lo, end), the first vector's place
   auto first = [&](int lo) { return ((lo + mis) & ~3) - mis; };
-  const int slice0 = (int)cl.block_rank();
-  if (slice0 < slices) load_all(first(slice0 << log_s), (int)min((int64_t)n, (int64_t)(slice0 + 1) << log_s));
   const Row w = load_row(R, r);
+  const bool touch = w.h1 > w.h0 || w.b1 > w.b0, brief = is_short<kMarginShort>(w);
+  // this CTA's share of a row without a long history
+  const int share = (int)(((n + nc - 1) / nc + 3) & ~3), lo0 = min(rank * share, n), end0 = min(lo0 + share, n);
+  if (brief && lo0 < end0) load_all(first(lo0), end0);
   const int label = labels[r] >= 0 && labels[r] < n ? (int)labels[r] : INT32_MIN;  // or no answer
-  Tables tab = tables_of(w, smem, log_s);
-  const bool touch = w.h1 > w.h0 || w.b1 > w.b0;
-  if (threadIdx.x == 0) label_l = -INFINITY;
-  cl.sync();  // the label's bound is written to the first CTA below
+  const float label_x = label >= 0 ? l[r * l_rs + label] : 0.0f;
+  if (threadIdx.x == 0) {
+    label_l = -INFINITY;
+    heard = to_ordered(-INFINITY);
+  }
+  __syncthreads();
   Best best{-INFINITY, kNone};
   // the edited bound v of allowed answer j
   auto bound = [&](int j, float v) { take(best, v != v ? INFINITY : v, j); };
-  auto own = [&](float v) {  // a bound that is no number bounds nothing
-    *cl.map_shared_rank(&label_l, 0) = v != v ? -INFINITY : v;
+  auto own = [&](float v) { label_l = v != v ? -INFINITY : v; };  // a bound that is no number bounds nothing
+  // the bounds of answers [lo, stop) that are not touched; their first chunk is loaded
+  auto pass = [&](int lo, int stop, auto&& touched) {
+    if (lo >= stop) return;
+    if (label >= lo && label < stop && threadIdx.x == 0 && is_allowed(w.allowed, label) && !touched(label)) own(label_x);
+    __syncwarp();
+    float floor = best.v;  // what the warp, and as far as it has heard the CTA, has found
+    for (int j0 = first(lo); j0 < stop; j0 += kChunk) {
+      floor = fmaxf(floor, from_ordered(*(volatile int*)&heard));
+#pragma unroll
+      for (int i = 0; i < kVpt; ++i) {
+        const int j = j0 + (i * kMarginThreads + (int)threadIdx.x) * V;
+        const Vec<float> a = t[i];
+        load(i, j0 + kChunk, stop);
+        const float top = max_nan(max_nan(a.v[0], a.v[1]), max_nan(a.v[2], a.v[3]));
+        const bool look = j < stop && !(top < floor);
+        if (__any_sync(0xffffffffu, look)) {
+          if (look) {
+            const uint32_t bits = open_bits<V>(w.allowed, j, n);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              const float v = a.v[e] != a.v[e] ? INFINITY : a.v[e];
+              if (v >= floor && beats(v, j + e, best) && (bits >> e & 1u) && j + e >= lo && j + e < stop &&
+                  j + e != label && !touched(j + e))
+                best = {v, j + e};
+            }
+          }
+          float top_found = best.v;
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1)
+            top_found = fmaxf(top_found, __shfl_xor_sync(0xffffffffu, top_found, off));
+          if (top_found > floor) {
+            floor = top_found;
+            if ((threadIdx.x & 31) == 0) atomicMax(&heard, to_ordered(floor));
+          }
+        }
+      }
+    }
   };
-  bool loaded = true, counted = false;
-  for (int slice = slice0; slice < slices; slice += nc) {
-    const int end = (int)min((int64_t)n, (int64_t)(slice + 1) << log_s);
-    uint32_t size;
-    for (int lo = slice << log_s; lo < end; lo += (int)size) {
-      const int stop = min(lo + (1 << (tab.wide ? log_s - 2 : log_s)), end);
-      size = (uint32_t)(stop - lo);
-      if (touch) {
+  if (!touch) {
+    pass(lo0, end0, [](int) { return false; });
+  } else if (brief) {
+    const Hash h = hash_of(w, smem, kMarginSlots);
+    fill(R, w, h);
+    const uint32_t listed = *h.listed;
+    for (uint32_t i = threadIdx.x; i < listed; i += kMarginThreads) {
+      const uint32_t s = h.list[i], c = h.cnt[s], at = h.pos[s];
+      const int j = (int)h.key[s] - 1;
+      if (j < lo0 || j >= end0 || !is_allowed(w.allowed, j)) continue;
+      float v = edit(j == label ? label_x : x[j], c != 0, c & kWideTimes, w.rep, w.freq, w.pres);
+      if (at) v = __fadd_rn(v, R.bias_values_dev[w.b0 + at - 1u]);
+      if (j == label)
+        own(v);
+      else
+        bound(j, v);
+    }
+    __syncwarp();
+    pass(lo0, end0, [&](int j) { return holds(h, (uint32_t)j); });
+  } else {
+    Tables tab = tables_of(w, smem, log_s);
+    bool counted = false;
+    for (int slice = rank; slice < slices; slice += nc) {
+      const int end = (int)min((int64_t)n, (int64_t)(slice + 1) << log_s);
+      uint32_t size;
+      for (int lo = slice << log_s; lo < end; lo += (int)size) {
+        const int stop = min(lo + (1 << (tab.wide ? log_s - 2 : log_s)), end);
+        size = (uint32_t)(stop - lo);
+        load_all(first(lo), stop);
         if (counted) __syncthreads();  // the tables are filled anew
         counted = true;
         if (!count(R, w, tab, lo, size)) {
@@ -576,49 +679,25 @@ __global__ void __launch_bounds__(kMarginThreads, 4)
         }
         for_biased(R, w, tab, lo, size, [&](int j, bool seen, uint32_t times, float bias) {
           if (!is_allowed(w.allowed, j)) return;
-          if (j == label)
-            own(__fadd_rn(edit(l[r * l_rs + j], seen, times, w.rep, w.freq, w.pres), bias));
-          else
-            bound(j, __fadd_rn(edit(x[j], seen, times, w.rep, w.freq, w.pres), bias));
-        });
-        if (w.b1 > w.b0) __syncthreads();  // the marks
-        for_seen(w, tab, lo, size, x, [&](int j, uint32_t times, float v) {
-          v = edit(j == label ? l[r * l_rs + j] : v, true, times, w.rep, w.freq, w.pres);
+          const float v = __fadd_rn(edit(j == label ? label_x : x[j], seen, times, w.rep, w.freq, w.pres), bias);
           if (j == label)
             own(v);
           else
             bound(j, v);
         });
-      }
-      auto touched = [&](int j) {
-        const uint32_t k = (uint32_t)(j - lo);
-        return touch && (entry(tab, k) != 0 || is_biased(w, tab, k));
-      };
-      if (label >= lo && label < stop && threadIdx.x == 0 && is_allowed(w.allowed, label) && !touched(label))
-        own(l[r * l_rs + label]);
-      __syncwarp();
-      for (int j0 = first(lo); j0 < stop; j0 += kChunk) {
-        if (!loaded) load_all(j0, stop);
-        loaded = j0 + kChunk < stop;  // by the end of this chunk
-        float floor = best.v;  // the warp's best
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) floor = fmaxf(floor, __shfl_xor_sync(0xffffffffu, floor, off));
-#pragma unroll
-        for (int i = 0; i < kVpt; ++i) {
-          const int j = j0 + (i * kMarginThreads + (int)threadIdx.x) * V;
-          if (j >= stop) break;
-          const Vec<float> a = t[i];
-          load(i, j0 + kChunk, stop);
-          const float top = max_nan(max_nan(a.v[0], a.v[1]), max_nan(a.v[2], a.v[3]));
-          if (top < floor) continue;
-          const uint32_t bits = open_bits<V>(w.allowed, j, n);
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float v = a.v[e] != a.v[e] ? INFINITY : a.v[e];
-            if (v >= floor && (bits >> e & 1u) && j + e >= lo && j + e < stop && j + e != label && !touched(j + e))
-              take(best, v, j + e);
-          }
-        }
+        if (w.b1 > w.b0) __syncthreads();  // the marks
+        for_seen(w, tab, lo, size, x, [&](int j, uint32_t times, float v) {
+          v = edit(j == label ? label_x : v, true, times, w.rep, w.freq, w.pres);
+          if (j == label)
+            own(v);
+          else
+            bound(j, v);
+        });
+        __syncwarp();
+        pass(lo, stop, [&](int j) {
+          const uint32_t k = (uint32_t)(j - lo);
+          return entry(tab, k) != 0 || is_biased(w, tab, k);
+        });
       }
     }
   }
@@ -630,21 +709,32 @@ __global__ void __launch_bounds__(kMarginThreads, 4)
   }
   if ((threadIdx.x & 31) == 0) part_best[threadIdx.x >> 5] = best;
   __syncthreads();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // all of the cluster's CTAs run
   if (threadIdx.x == 0) {
     for (int i = 1; i < kMarginThreads / 32; ++i) take(best, part_best[i].v, part_best[i].j);
-    cl.map_shared_rank(joined, 0)[cl.block_rank()] = best;
+    cl.map_shared_rank(joined, 0)[rank] = best;
+    cl.map_shared_rank(joined_l, 0)[rank] = label_l;
   }
   cl.sync();
-  if (cl.block_rank() == 0 && threadIdx.x == 0) {
-    for (int i = 0; i < nc; ++i) take(best, joined[i].v, joined[i].j);
+  if (rank == 0 && threadIdx.x == 0) {
+    float mine = label_l;  // one CTA has the label, the others' is -inf
+    for (int i = 0; i < nc; ++i) {
+      take(best, joined[i].v, joined[i].j);
+      mine = fmaxf(mine, joined_l[i]);
+    }
     const bool any = best.v > -INFINITY;
-    const float m = label_l - best.v;
+    const float m = mine - best.v;
     margin[r] = m != m ? -INFINITY : m;  // an infinite bound less itself says nothing
     rival[r] = any ? best.j : -1;
   }
 }
 
 // ------------------------------------------------------------------------------ host
+size_t smem_bytes(int log_s, size_t hash) {
+  const size_t tables = tables_bytes(log_s);
+  return tables > hash ? tables : hash;
+}
+
 bool has_edits(const cf_answer_rules& R) {
   return (R.tokens_dev && R.n_tokens > 0) || (R.bias_ids_dev && R.n_biases > 0);
 }
@@ -730,10 +820,13 @@ cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, v
     while (log_s > 11 && R.rows * ceil_div(R.n, (int64_t)1 << log_s) < 148) --log_s;
   while (log_s > 11 && (int64_t)1 << (log_s - 1) >= R.n) --log_s;
   const int slices = (int)ceil_div(R.n, (int64_t)1 << log_s), ctas = brief ? 1 : slices;
-  const size_t tables = tables_bytes(log_s), smem = tables > kHashBytes ? tables : kHashBytes;
-  static std::atomic<uint64_t> allowed{0};
-  return launch("k_answer_edits", k_answer_edits<T>, &allowed, R.rows * ctas, 512, smem, 0, stream, st, R, (T*)out,
-                out_rs, log_s, slices, ctas);
+  const size_t smem = smem_bytes(log_s, hash_bytes(kSlots, kShort));
+  static std::atomic<uint64_t> allowed[2];
+  if (brief)
+    return launch("k_answer_edits", k_answer_edits<T, 512>, &allowed[0], R.rows * ctas, 512, smem, 0, stream, st, R,
+                  (T*)out, out_rs, log_s, slices, ctas);
+  return launch("k_answer_edits", k_answer_edits<T, 1024>, &allowed[1], R.rows * ctas, 1024, smem, 0, stream, st, R,
+                (T*)out, out_rs, log_s, slices, ctas);
 }
 
 }  // namespace
@@ -772,9 +865,9 @@ extern "C" cf_status cf_answer_margin(const cf_answer_rules* R, const float* l, 
   if (R->rows == 0) return CF_OK;
   CF_REQUIRE(l && u && labels && margin && rival, CF_ERR_NULL, "answer_margin: NULL argument");
   CF_REQUIRE(((uintptr_t)l | (uintptr_t)u) % 4 == 0, CF_ERR_SHAPE, "answer_margin: unaligned rows");
-  // 16384 answers a slice, fewer for a short row or few rows; a cluster of up to eight for a row, as far
-  // as all rows' fit the GPU at once
-  int log_s = 14;
+  // 8192 answers a slice, 16384 where rows are long on average, fewer for few answers or few rows; a cluster of up
+  // to eight for a row, as far as all rows' fit the GPU at once
+  int log_s = R->n_tokens > R->rows * kMarginShort ? 14 : 13;
   while (log_s > 11 && ((int64_t)1 << (log_s - 1) >= R->n ||
                         (R->rows * ceil_div(R->n, (int64_t)1 << log_s) < 148 && (int64_t)8 << (log_s - 1) >= R->n)))
     --log_s;
@@ -783,6 +876,6 @@ extern "C" cf_status cf_answer_margin(const cf_answer_rules* R, const float* l, 
   while (cluster < kMaxCluster && cluster < slices && R->rows * cluster * 2 <= 148 * 4) cluster *= 2;
   static std::atomic<uint64_t> allowed{0};
   return launch("k_answer_margin", k_answer_margin, &allowed, R->rows * cluster, kMarginThreads,
-                has_edits(*R) ? tables_bytes(log_s) : 0, cluster, false, as_stream(stream), *R, l, l_rs, u, u_rs,
+                has_edits(*R) ? smem_bytes(log_s, hash_bytes(kMarginSlots, kMarginShort)) : 0, cluster, false, as_stream(stream), *R, l, l_rs, u, u_rs,
                 labels, margin, rival, log_s, slices);
 }
