@@ -234,7 +234,7 @@ def _plain(t, dtype, gpu, shape):
 def _launch(gpu, fn, *args):
     """fn(*args, stream): a libcfgpu call on the current stream of that GPU, made the current device
     where it is not."""
-    if gpu == torch.cuda.current_device():
+    if gpu == torch._C._cuda_getDevice():
         return fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
     with torch.cuda.device(gpu):
         return fn(*args, torch._C._cuda_getCurrentRawStream(gpu))
@@ -297,8 +297,10 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
     if x.dim() == 2 and x.stride(1) != 1:
         x = x.contiguous()
     T, Q = x.shape[0], ids.shape[0]
+    rs, out_rs = K, N
     if not _plain(x, dt, gpu, (T, K)):
         _expect("x", x, dt, (None, K), dev, strided=True)
+        rs = _row_stride(x)
     if not _plain(offsets, torch.int64, gpu, (Q + 1,)):
         _expect("offsets", offsets, torch.int64, (Q + 1,), dev)
     if not _plain(ids, torch.int32, gpu, (Q,)):
@@ -307,7 +309,8 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
         out = torch.zeros(T, N, dtype=dt, device=dev)
     elif not _plain(out, dt, gpu, (T, N)):
         _expect("out", out, dt, (T, N), dev, strided=True)
-    xp, rs = x.data_ptr(), _row_stride(x)
+        out_rs = _row_stride(out)
+    xp = x.data_ptr()
     key = (substitute, T, Q, xp % 16, rs)
     need = layer._need.get(key)
     if need is None:
@@ -317,7 +320,7 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
     st = _launch(gpu, _lib.lib.cf_adapter_matmul, layer._ref, 1 if substitute else 0, T, xp, rs, Q,
-                 offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), _row_stride(out), ws.data_ptr(), need)
+                 offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), out_rs, ws.data_ptr(), need)
     if st:
         _lib.check(st, "cf_adapter_matmul")
     return out
@@ -350,6 +353,7 @@ class AnswerRules:
     def __init__(self, rows, n, tokens=None, token_offsets=None, prompt_len=None, repetition=None, frequency=None,
                  presence=None, bias_ids=None, bias_values=None, bias_offsets=None, allowed=None, allowed_row=None):
         self.rows, self.n = int(rows), int(n)
+        self.shape = (self.rows, self.n)
         given = dict(tokens=tokens, token_offsets=token_offsets, prompt_len=prompt_len, repetition=repetition,
                      frequency=frequency, presence=presence, bias_ids=bias_ids, bias_values=bias_values,
                      bias_offsets=bias_offsets, allowed=allowed, allowed_row=allowed_row)
@@ -383,14 +387,16 @@ class AnswerRules:
 
 
 def _rules_rows(name, t, rules, dtype, gpu):
-    """t as rows for the rules: [rows, n] of `dtype` on `gpu`, its last dimension contiguous."""
+    """(t, its row stride) as rows for the rules: [rows, n] of `dtype` on `gpu`, its last dimension
+    contiguous."""
     if rules.device is not None and gpu != rules.device.index:
         raise Exception(f"SHAPE MISMATCH: {name} is on GPU {gpu}, the rules are on {rules.device}")
+    if _plain(t, dtype, gpu, rules.shape):
+        return t, rules.n
     if t.dim() == 2 and t.stride(1) != 1:
         t = t.contiguous()
-    if not _plain(t, dtype, gpu, (rules.rows, rules.n)):
-        _expect(name, t, dtype, (rules.rows, rules.n), torch.device("cuda", gpu), strided=True)
-    return t
+    _expect(name, t, dtype, rules.shape, torch.device("cuda", gpu), strided=True)
+    return t, _row_stride(t)
 
 
 def edit_logits(logits, rules, out=None):
@@ -400,14 +406,15 @@ def edit_logits(logits, rules, out=None):
     if dt not in _DTYPES:
         raise NotImplementedError(f"logits of {dt} (float32, bfloat16 and float16 are supported)")
     gpu = _cuda("logits", logits).index
-    x = _rules_rows("logits", logits, rules, dt, gpu)
+    x, rs = _rules_rows("logits", logits, rules, dt, gpu)
+    out_rs = rules.n
     if out is None:
         out = torch.empty(rules.rows, rules.n, dtype=dt, device=x.device)
-    elif not _plain(out, dt, gpu, (rules.rows, rules.n)):
-        _expect("out", out, dt, (rules.rows, rules.n), x.device, strided=True)
+    elif not _plain(out, dt, gpu, rules.shape):
+        _expect("out", out, dt, rules.shape, x.device, strided=True)
+        out_rs = _row_stride(out)
     LAUNCHES[0] += rules.launches
-    st = _launch(gpu, _lib.lib.cf_edit_logits, rules._ref, _DTYPES[dt], x.data_ptr(), _row_stride(x), out.data_ptr(),
-                 _row_stride(out))
+    st = _launch(gpu, _lib.lib.cf_edit_logits, rules._ref, _DTYPES[dt], x.data_ptr(), rs, out.data_ptr(), out_rs)
     if st:
         _lib.check(st, "cf_edit_logits")
     return out
@@ -421,14 +428,13 @@ def answer_margin(l, u, labels, rules):
     A label that is not allowed has margin -inf; a bound that is NaN bounds nothing."""
     dev = _cuda("l", l)
     gpu = dev.index
-    l = _rules_rows("l", l, rules, torch.float32, gpu)
-    u = _rules_rows("u", u, rules, torch.float32, gpu)
+    l, l_rs = _rules_rows("l", l, rules, torch.float32, gpu)
+    u, u_rs = _rules_rows("u", u, rules, torch.float32, gpu)
     if not _plain(labels, torch.int64, gpu, (rules.rows,)):
         _expect("labels", labels, torch.int64, (rules.rows,), dev)
-    margin = torch.empty(rules.rows, dtype=torch.float32, device=dev)
-    rival = torch.empty(rules.rows, dtype=torch.int32, device=dev)
+    margin, rival = l.new_empty(rules.rows), l.new_empty(rules.rows, dtype=torch.int32)
     LAUNCHES[0] += 1
-    st = _launch(gpu, _lib.lib.cf_answer_margin, rules._ref, l.data_ptr(), _row_stride(l), u.data_ptr(), _row_stride(u),
+    st = _launch(gpu, _lib.lib.cf_answer_margin, rules._ref, l.data_ptr(), l_rs, u.data_ptr(), u_rs,
                  labels.data_ptr(), margin.data_ptr(), rival.data_ptr())
     if st:
         _lib.check(st, "cf_answer_margin")
