@@ -598,6 +598,38 @@ def test_adapters_then_rules():
     assert (m.cpu()[ok] >= 0).all()
 
 
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("rows", [256, 1000, 1024, 1100, 1281])
+def test_requests_at_the_tiles_bounds(sub, rows):
+    """Requests that begin and end at, before and behind the bounds of row tiles; ranks that go row by
+    row beside those that do not; NaN stays with its request."""
+    K, N, R = 136, 5000, 48
+    cuts = [c for c in (0, 128, 200, 256, 300, 512, 640, 700, 704, 768, 900, 1024, 1050, 1152, 1200) if c < rows] + [rows]
+    t = make(rows, K, N, R, 7, len(cuts) - 1, BF16, sub, seed=71)
+    t["offsets"] = torch.tensor(cuts)
+    t["ids"] = torch.tensor([0, 1, 1, 2, 2, -1, 3, 4, 3, 5, 5, 3, 0, 4, 4, 4][:len(cuts) - 1], dtype=torch.int32)
+    t["ranks"] = torch.tensor([48, 32, 16, 48, 5, 0, 48], dtype=torch.int32)
+    compare(t, sub)
+    want, tol = oracle(t, sub)
+    for e in (0, 2, 3):
+        u = dict(t, A=t["A"].clone(), B=t["B"].clone())
+        u["A"][e] = math.nan
+        u["B"][e, 3] = math.inf
+        got = ops().adapter_matmul(u["x"].cuda(), layer(u), u["offsets"].cuda(), u["ids"].cuda(), substitute=sub)
+        for q, i in enumerate(t["ids"].tolist()):
+            if i != e:
+                V.check(got[cuts[q]:cuts[q + 1]], want[cuts[q]:cuts[q + 1]], tol[cuts[q]:cuts[q + 1]], f"{e} {q}")
+            else:
+                assert got[cuts[q]:cuts[q + 1]].isnan().all()
+    # the first and last rows are no request's
+    t["offsets"] = torch.tensor([c + 1 for c in cuts[:-1]] + [rows - 2])
+    before = torch.randn(rows, N, generator=gen(3)).to(BF16)
+    y, tol = oracle(t, sub, out=before)
+    V.check(ops().adapter_matmul(t["x"].cuda(), layer(t), t["offsets"].cuda(), t["ids"].cuda(), substitute=sub,
+                                 out=before.cuda()), y, tol)
+    ops().adapter_check()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_rows_beside_their_results(dtype):
     """x and y as columns of one buffer, logits and result too."""
