@@ -1,6 +1,6 @@
 // The adapter product for a few rows, on the CUDA cores: the weights are read once, at the memory's
 // rate, and a tile of the tensor cores would be filled by few rows (one row of 4096 x 4096
-// float32: the tiles took 38 us).
+// float32: the tiles took 38 us, this 8; bfloat16 11 and 5.4, from the L2 cache; memory gives 33 MB in 5.2).
 //
 //   project:    M = W^T, rows of k.  A CTA has four columns; its eight warps share the contraction.
 //   substitute: M = W, rows of n, float32.  A CTA has 32 columns, eight lanes of 16 bytes a row of W;

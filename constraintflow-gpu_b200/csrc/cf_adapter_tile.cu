@@ -13,6 +13,9 @@
 // Operands in shared memory are 128-byte-swizzled images, 128 bytes of the contraction a row:
 // loaded by tensor maps; M and Q_e with n contiguous (substitution) stay as they lie, as MN-major
 // images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
+//
+// 64 rows of 4096 x 4096, each with its own adapter of rank 16: 18.5 us, 47 MB at 2.5 TB/s: a chain of
+// launch, v, weights, sums and the rows' own adapters, each part waiting for the one before.
 #include <cooperative_groups.h>
 
 #include "cf_adapter_tma.cuh"

@@ -15,11 +15,15 @@
 // What the history and the biases touch is little and is put right from their side, in the result
 // that the stream has left in the cache.  For 256 x 131072 bfloat16 and 1024 tokens a row: a lookup
 // for every answer on the way 228 us (some lane of nearly every warp edits), edits of each slice in
-// shared memory on its way 50, the stream 22 and behind it the edits.
+// shared memory on its way 50, the stream 22 (134 MB: 0.94 of a copy's rate) and behind it the edits
+// 12: random reads and writes of single answers, each waiting on the last for its address.
 //
 // Short histories go into a hash table of the answers they touch, one CTA a row, whatever the row's
 // length.  Long ones are counted slice by slice in tables of all answers: 16 bits an answer, seen
-// and 15 bits of times, and a bit for its having a bias.
+// and 15 bits of times, and a bit for its having a bias; what bounds them is the walk over the history, once a
+// slice, and its atomics on the answers that come again and again (33 rows of 100003, up to 32768
+// tokens, the first slice 0.55 of them: 35 us, 6 of them the stream; smaller slices walk more
+// often: 45 us in twice as many).
 // Which of the (few) biases of one answer is the last is found by comparing them.  A row with more
 // than kMaxBiases biases, or one answer more than kTimes times, is done in quarters of a
 // slice, with 32 bits for the times and 32 for the place of the last bias.  Counts are integers
@@ -551,7 +555,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // One cluster per row: the label's edited lower bound less the best edited upper bound among the
 // other answers.  Each CTA has a share of the answers (of a row with a long history, slices); what
 // is touched has its own pass, and on the way over the bounds a vector is looked into only where it
-// holds something above the best so far.
+// holds something above the best that the CTA's warps have told one another of.  128 rows of 131072, 67 MB:
+// 14 us without edits (from the L2 cache; 21 when each warp only knew its own best), 25 with up to 1024
+// tokens a row: the table has to be there before the first bound can be passed over.
 __global__ void __launch_bounds__(kMarginThreads, 4)
     k_answer_margin(const cf_answer_rules R, const float* __restrict__ l, int64_t l_rs, const float* __restrict__ u,
                     int64_t u_rs, const int64_t* __restrict__ labels, float* margin, int32_t* rival, int log_s,
@@ -822,7 +828,9 @@ cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, v
   const int slices = (int)ceil_div(R.n, (int64_t)1 << log_s), ctas = brief ? 1 : slices;
   const size_t smem = smem_bytes(log_s, hash_bytes(kSlots, kShort));
   static std::atomic<uint64_t> allowed[2];
-  if (brief)
+  // More short rows than SMs: two CTAs of 512 an SM (256 rows of 131072 bfloat16, up to 2048 tokens: 34.3 us, 36.7 with
+  // 1024); else 1024 (64 rows, up to 1000 tokens: 12.4 us, 13.6 with 512).
+  if (brief && R.rows > 148)
     return launch("k_answer_edits", k_answer_edits<T, 512>, &allowed[0], R.rows * ctas, 512, smem, 0, stream, st, R,
                   (T*)out, out_rs, log_s, slices, ctas);
   return launch("k_answer_edits", k_answer_edits<T, 1024>, &allowed[1], R.rows * ctas, 1024, smem, 0, stream, st, R,
