@@ -294,7 +294,7 @@ __device__ __forceinline__ void for_seen(const Row& w, const Tables& t, int lo, 
 // What a short row touches: open addressing over the answers.
 // kShort tokens and biases of a row at most, kMarginShort for its margin (whose CTAs, four an SM, all run at
 // once, and read through what the tables leave of the L1 cache).
-constexpr uint32_t kSlots = 4096, kShort = 3072, kMarginSlots = 2048, kMarginShort = 1536;
+constexpr uint32_t kSlots = 4096, kShort = 2800, kMarginSlots = 2048, kMarginShort = 1536;
 
 struct Hash {
   int log_n;  // 1 << log_n slots, twice a row's tokens and biases where there are that many

@@ -425,8 +425,8 @@ def one_history(n, lens, biases, seed, tops=()):
 
 HISTORIES = [
     # at the most that a row's own small table holds, and one more; repeated and distinct answers
-    (5000, [3072, 3073, 3000, 3000, 0, 0], [0, 0, 72, 73, 3072, 3073], ()),
-    (3072, [2048, 2049, 1, 0], [1024, 1024, 0, 1], ()),
+    (5000, [2800, 2801, 2700, 2700, 0, 0], [0, 0, 100, 101, 2800, 2801], ()),
+    (2900, [1536, 1537, 1036, 1036, 1, 0, 0], [0, 0, 500, 501, 1536, 1537, 1], ()),
     # more biases than are compared one by one; one answer more often than 15 bits count
     (9001, [10, 4000, 5000], [1025, 1024, 1500], ()),
     (40000, [100, 5000, 0], [3, 2, 0], ((0, 77, 32767), (1, 39999, 32768), (2, 5, 70000))),
@@ -671,3 +671,67 @@ def test_adapter_grid_of_wide_tiles(dtype, sub):
     """Enough tiles that every SM walks over several, the last ones ragged in both directions."""
     compare(make(4000, 72, 5208, 32, 5, 9, dtype, sub, seed=31, ranks=True, bias=True), sub)
     compare(make(8000, 136, 2056, 72, 3, 60, dtype, sub, seed=32), sub)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_results_of_more_than_2_31_elements(dtype):
+    """The rows at the far end of a large result are those of a call with these rows alone."""
+    T, K, N, tail = 33001, 64, 66000, 150
+    t = make(T, K, N, 8, 3, 5, dtype, False, seed=81, style="tokens")
+    L = layer(t)
+    y = ops().adapter_matmul(t["x"].cuda(), L, t["offsets"].cuda(), t["ids"].cuda())
+    u = dict(t, x=t["x"][-tail:], offsets=(t["offsets"] - (T - tail)).clamp(min=0))
+    V.check(y[-tail:], *oracle(u, False))
+    del y
+    rows, n = 16500, 131072
+    kw = make_rules(2, n, seed=82, hist=50, biases=9, masks=1)
+    at = [0, rows - 1]                         # the rules of the first and the last row
+    for k in ("token_offsets", "bias_offsets"):
+        kw[k] = torch.cat([kw[k][:1], kw[k][1:2].expand(rows - 1), kw[k][2:]])
+    for k in ("prompt_len", "repetition", "frequency", "presence", "allowed_row"):
+        full = torch.full((rows,), -1 if k == "allowed_row" else 1, dtype=kw[k].dtype)
+        full[at] = kw[k]
+        kw[k] = full
+    x = torch.zeros(rows, n, dtype=dtype, device="cuda")
+    ends = (torch.randn(2, n, generator=gen(1)) * 3).to(dtype)
+    x[at] = ends.cuda()
+    rules = ops().AnswerRules(rows, n, **on_gpu(kw))
+    got = ops().edit_logits(x, rules)
+    small = {k: v[at] if k in ("prompt_len", "repetition", "frequency", "presence", "allowed_row") else v
+             for k, v in kw.items()}
+    for k in ("token_offsets", "bias_offsets"):
+        small[k] = torch.stack([kw[k][0], kw[k][1], kw[k][-1]])
+    same(got[at].float(), V.rules(ends.float(), n, dtype=F32, **small).to(dtype).float())
+    assert not got[1:-1].any()
+    if dtype is F32:
+        labels = torch.full((rows,), 7)
+        m, j = ops().answer_margin(x, x, labels.cuda(), rules)
+        wm, wj = V.margin(ends, ends, labels[:2], n, **small)
+        same(m[at], wm)
+        assert torch.equal(j[at].cpu(), wj)
+        assert not m[1:-1].any() and not j[1:-1].any()
+
+
+def test_rules_on_two_streams_at_once():
+    rows, n = 40, 60000
+    xs, want, rules = [], [], []
+    for i in range(2):
+        kw = make_rules(rows, n, seed=90 + i, hist=3000 * (i + 1), biases=40, masks=3)
+        x = torch.randn(rows, n, generator=gen(i)) * 3
+        labels = x.argmax(dim=1)
+        xs.append((x.cuda(), labels.cuda()))
+        rules.append(ops().AnswerRules(rows, n, **on_gpu(kw)))
+        want.append((V.rules(x, n, dtype=F32, **kw), *V.margin(x, x, labels, n, **kw)))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                x, labels = xs[i]
+                got[i] = (ops().edit_logits(x, rules[i]), *ops().answer_margin(x, x, labels, rules[i]))
+        torch.cuda.synchronize()
+        for g, w in zip(got, want):
+            same(g[0], w[0])
+            same(g[1], w[1])
+            assert torch.equal(g[2].cpu(), w[2])
