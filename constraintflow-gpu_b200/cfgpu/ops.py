@@ -291,7 +291,8 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
     offsets [n_requests + 1] int64: the rows of request q are offsets[q] .. offsets[q+1]-1;
     ids [n_requests] int32: its adapter, any value outside 0 .. n_adapters-1 none.  Both are
     read on the device, without a synchronisation.  Rows of no request are left as they were in
-    `out`, and are 0 in a new result.  `out` must not overlap x."""
+    `out`, and are 0 in a new result.  `out` must not overlap x.  What meets an infinity comes out
+    as an infinity or NaN, in rows of that request only."""
     dev, gpu, dt = layer.device, layer.gpu, layer.dtype
     K, N = (layer.n_out, layer.n_in) if substitute else (layer.n_in, layer.n_out)
     if x.dim() == 2 and x.stride(1) != 1:

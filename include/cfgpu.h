@@ -430,7 +430,9 @@ typedef struct cf_adapter_layer {
  * of no request (before offsets[0], from offsets[n_requests] on) are left as they were.  x and y
  * do not overlap.  A request's rows depend on its own adapter only: infinities or NaN in another
  * adapter or in rows of other requests do not reach them.  Products are accumulated in float32;
- * float32 data is multiplied as 3xTF32, as in the chained substitution.  The workspace
+ * float32 data is multiplied as 3xTF32, as in the chained substitution.  Where a row meets an
+ * infinity of its own, of W or of its adapter, or an intermediate of it overflows, the result is
+ * an infinity or NaN (a number held in two parts has no second part then).  The workspace
  * (256-byte aligned, >= cf_adapter_workspace_bytes for these arguments) belongs to the call until
  * it has run; 16-bit operands whose rows are not 16-byte aligned are copied into it. */
 size_t cf_adapter_workspace_bytes(const cf_adapter_layer* layer, int32_t substitute, int64_t T,

@@ -673,6 +673,20 @@ def test_adapter_grid_of_wide_tiles(dtype, sub):
     compare(make(8000, 136, 2056, 72, 3, 60, dtype, sub, seed=32), sub)
 
 
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("T,N", [(4, 96), (300, 96), (300, 9000)])
+def test_an_infinity_stays_with_its_row(dtype, sub, T, N):
+    t = make(T, 64, N, 8, 3, 3, dtype, sub, seed=85, style="tokens")
+    want, tol = oracle(t, sub)
+    x = t["x"].clone()
+    x[T // 2, 7] = math.inf
+    got = ops().adapter_matmul(x.cuda(), layer(t), t["offsets"].cuda(), t["ids"].cuda(), substitute=sub)
+    assert not got[T // 2].isfinite().any()
+    keep = torch.arange(T) != T // 2
+    V.check(got[keep.cuda()], want[keep], tol[keep])
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 def test_results_of_more_than_2_31_elements(dtype):
     """The rows at the far end of a large result are those of a call with these rows alone."""
