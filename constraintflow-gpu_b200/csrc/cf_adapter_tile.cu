@@ -66,6 +66,10 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
   const uint32_t sbase = smem_u32(smem);
   cg::cluster_group cl = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == kProducerWarp * 32) {
+    prefetch_map(&maps.x);
+    prefetch_map(&maps.b);
+  }
   const int split = g.split;
   const int rank = split > 1 ? (int)cl.block_rank() : 0;
   const int64_t unit = blockIdx.x / split;

@@ -15,6 +15,11 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int
       : "memory");
 }
 
+// Fetch a tensor map ahead of the first load through it.
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+
 __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(

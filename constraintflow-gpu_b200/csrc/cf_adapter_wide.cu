@@ -50,6 +50,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == kProducerWarp * 32) {
+    prefetch_map(&maps.x);
+    prefetch_map(&maps.b);
+  }
   if (warp == kMmaWarp) tmem_alloc(&bars.tmem, 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
