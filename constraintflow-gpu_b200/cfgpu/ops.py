@@ -268,6 +268,7 @@ class AdapterLayer:
         if bias is not None:
             _expect("bias", bias, dt, (self.n_out,), dev)
         self.device, self.dtype, self.gpu = dev, dt, dev.index
+        self.size = W.element_size()
         self._need = {}           # workspace bytes by sizes and alignment
         self._keep = (W, A, B, scale, ranks, bias)
 
@@ -318,7 +319,7 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
         if len(layer._need) >= 4096:
             layer._need.clear()
         need = layer._need[key] = _lib.lib.cf_adapter_workspace_bytes(layer._ref, 1 if substitute else 0, T, xp, rs, Q)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = x.new_empty(need // layer.size)
     LAUNCHES[0] += 1 + (need > 0)        # the adapters' part has a launch of its own
     st = _launch(gpu, _lib.lib.cf_adapter_matmul, layer._ref, 1 if substitute else 0, T, xp, rs, Q,
                  offsets.data_ptr(), ids.data_ptr(), out.data_ptr(), out_rs, ws.data_ptr(), need)
