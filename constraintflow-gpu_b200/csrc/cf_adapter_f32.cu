@@ -21,11 +21,10 @@
 // with few tiles the contraction is dealt out to the CTAs of a cluster instead, which sum their
 // parts in rank order.
 //
-// 4096 x 4096 x 4096, rank 64: 965 us, 142 TFLOP/s, half of the rate of 3xTF32 alone (276): a step's images
+// 4096 x 4096 x 4096, rank 64: 925 us, 149 TFLOP/s, 0.54 of the rate of 3xTF32 alone (276): a step's images
 // are written, read for three products and loaded through the same 128 bytes a cycle of the SM, about
-// as long as its MMAs take to issue.  51200 x 200 x 784 with 256 requests of rank 8: 272 us and 48 for v, of which
-// the low-rank chunks (two a tile, next to seven steps of x M) are a fifth; tensor pipe active 0.22,
-// issue slots 0.51.
+// as long as its MMAs take to issue.  A third stage takes the L1 cache that the loads go through (1104 us).
+// 51200 x 200 x 784 with 256 requests of rank 8: 244 us, substituted 302, without adapters 162 and 178.
 #include <cooperative_groups.h>
 
 #include <type_traits>
@@ -43,9 +42,13 @@ using namespace tc;
 constexpr int kDrain = 256, kLoad = 256;  // threads of the two groups
 constexpr int kMmaWarp = 16;
 constexpr int kThreads = 640;  // five warpgroups; warps 17-19 idle
-// Registers a thread: 96 at launch (640 x 96 = 61440).  The loads hold two steps of chunks and take
-// what the MMA group gives up: 128 (2 x 96 + 2 x 112 + 64) = 61440.
-constexpr int kDrainRegs = 96, kLoadRegs = 112, kMmaRegs = 64;
+// Registers a thread: 96 at launch (640 x 96 = 61440).  What the MMA group gives up goes to the drain, which
+// holds a tile's sums, 128 (2 x 112 + 2 x 96 + 64) = 61440; for v, with half a tile and less, to the loads.
+constexpr int kMmaRegs = 64;
+template <bool kShrink, int kBN>
+struct Regs {
+  static constexpr int kDrain = kShrink ? (kBN == 64 ? 96 : 104) : 112, kLoad = 208 - kDrain;
+};
 constexpr int kStep = 32;   // contraction of a stage: 128 bytes
 constexpr int kChunk = 2;   // steps of one accumulation
 constexpr int kStages = 2, kBufs = 2;
@@ -111,8 +114,6 @@ struct Bars {
   uint32_t tmem;
 };
 
-__device__ __forceinline__ void drain_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kDrain) : "memory"); }
-
 template <int kBN>
 struct Chunks {  // one step's operand chunks of a loading thread
   uint4 x[kBM * 8 / kLoad], b[kBN * 8 / kLoad];
@@ -125,10 +126,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
   extern __shared__ uint8_t smem_raw[];
   __shared__ Bars bars;
   __shared__ int row_e[kShrink ? 1 : kBM];  // each row's adapter, kMixed for a row of no request
-  __shared__ int gave_up;                   // a draining warp's wait did: all of them stop at the same tile
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const uint32_t sbase = smem_u32(smem);
-  float* part = (float*)(smem + kStages * kStageBytes);  // the tile, [kBM][kLd]
+  float* part = (float*)smem;  // a cluster's tile, [kBM][kLd], where its operands were
+  static_assert(kBM * kLd * 4 <= kStages * kStageBytes, "the tile is staged where the operands were");
   cg::cluster_group cl = cg::this_cluster();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = g.split, rank = split > 1 ? (int)cl.block_rank() : 0;
@@ -153,7 +154,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     }
     mbar_init(&bars.done, 1);
     fence_mbar_init();
-    gave_up = 0;
   }
   tc_fence_before();
   __syncthreads();
@@ -166,15 +166,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
   const bool lowrank = !kShrink && p.R > 0 && !g.rowwise && rank == 0;
   Tile w = {};
   // v up to the adapter's rank, and zeros up to the next multiple of 4
-  auto put_v = [&](int64_t t, int r, float v) {
-    if (r < (w.e_rank + 3) / 4 * 4) store_v(p, t, r, r < w.e_rank ? v : 0.0f);
+  auto put_v4 = [&](int64_t t, int r, float scale, float a, float b, float c, float d) {
+    if (r >= w.e_rank) return;
+    *(float4*)(p.v + t * p.v_rs + r) = make_float4(scale * a, r + 1 < w.e_rank ? scale * b : 0.0f,
+                                                   r + 2 < w.e_rank ? scale * c : 0.0f, r + 3 < w.e_rank ? scale * d : 0.0f);
   };
   bool waited = !g.dependent;
   bool ok = true;
 
   if (warp >= 8 && warp < kMmaWarp) {
     // ---------------------------------------------------------------- loads
-    more_registers<kLoadRegs>();
+    more_registers<Regs<kShrink, kBN>::kLoad>();
     const int tid = threadIdx.x - kDrain, chunk = tid & 7, prow = tid >> 3;
     int it = 0;
     // four elements of a row with contiguous k from k on, of n_kk; vec: 16-byte aligned, n_kk a
@@ -363,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     }
   } else {
     // ---------------------------------------------------------------- chunks, tiles
-    more_registers<kDrainRegs>();  // the compiler allots by it
+    more_registers<Regs<kShrink, kBN>::kDrain>();  // the compiler allots by it
     const int row = (warp & 3) * 32 + lane, c0 = (warp >> 2) * (kBN / 2);
     const uint32_t src = tmem + ((uint32_t)((warp & 3) * 32) << 16) + c0;
     int ch = 0;
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
       const int rows = (int)min((int64_t)kBM, p.T - w.t0);
       if constexpr (!kShrink) {
-        if (threadIdx.x < rows) {
+        if (split > 1 && threadIdx.x < rows) {
           const int64_t t = w.t0 + (int)threadIdx.x;
           row_e[threadIdx.x] = !is_owned(p, t) ? kMixed : g.rowwise ? adapter_of(p, request_of(p, t)) : kNone;
         }
@@ -411,42 +413,52 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
           return true;
         });
       }
+      if (split > 1) {  // one tile: the cluster's parts are summed below
+        if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < kBN / 2; i += 4)
-        *(float4*)(part + row * kLd + c0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
-      if (split > 1) break;  // one tile: the cluster's parts are summed below
-      if (!ok) *(volatile int*)&gave_up = 1;
-      drain_sync();
-      ok = *(volatile int*)&gave_up == 0;
+        for (int i = 0; i < kBN / 2; i += 4)
+          *(float4*)(part + row * kLd + c0 + i) = make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+        break;
+      }
+      if (!ok) break;
       if constexpr (kShrink) {
-        const int a = w.row0, b = w.row1, quads = w.cols / 4;
-        const float scale = p.scale[w.e];
-        for (int i = threadIdx.x; i < (b - a) * quads; i += kDrain) {
-          const int r = a + i / quads, c = i % quads * 4;
+        if (row >= w.row0 && row < w.row1) {
+          const float scale = p.scale[w.e];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            put_v(w.t0 + r, w.r0 + c + j, scale * part[r * kLd + c + j]);
+          for (int i = 0; i < kBN / 2; i += 4) put_v4(w.t0 + row, w.r0 + c0 + i, scale, acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
         }
       } else {
-        const int64_t n = w.n0 + lane * 4;
-        float bias[4] = {};
-        if (p.bias)
+        // The warp's rows, 32 columns at a time: turned in its own shared memory, written four rows of 128
+        // bytes a turn.
+        const int64_t t = w.t0 + row;
+        const int mine = row >= rows || !is_owned(p, t) ? kMixed : g.rowwise ? adapter_of(p, request_of(p, t)) : kNone;
+        float* turn = (float*)(smem + kStages * kStageBytes) + warp * 1024;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (n + i < p.N) bias[i] = ((const float*)p.bias)[n + i];
-        if (n < p.N) {
+        for (int c = 0; c < kBN / 2; c += 32) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            *(float4*)(turn + lane * 32 + ((i ^ (lane & 7)) << 2)) =
+                make_float4(acc[c + 4 * i], acc[c + 4 * i + 1], acc[c + 4 * i + 2], acc[c + 4 * i + 3]);
+          __syncwarp();
+          const int64_t n = w.n0 + c0 + c + (lane & 7) * 4;
+          float bias[4] = {};
+          if (p.bias)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n + i < p.N) bias[i] = ((const float*)p.bias)[n + i];
 #pragma unroll 1
-          for (int r = warp; r < rows; r += 8) {
-            const int re = row_e[r];
-            if (re == kMixed) continue;
-            const float4 s = *(const float4*)(part + r * kLd + lane * 4);
-            float a[4] = {s.x + bias[0], s.y + bias[1], s.z + bias[2], s.w + bias[3]};
-            if (g.rowwise) add_lowrank<float, kSub>(p, w.t0 + r, re, rank_of(p, re), n, a);
-            store4<float>(p, w.t0 + r, n, a);
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3), re = __shfl_sync(0xffffffffu, mine, r);
+            if (re == kMixed || n >= p.N) continue;
+            const float4 d = *(const float4*)(turn + r * 32 + (((lane & 7) ^ (r & 7)) << 2));
+            float a[4] = {d.x + bias[0], d.y + bias[1], d.z + bias[2], d.w + bias[3]};
+            const int64_t tr = w.t0 + (warp & 3) * 32 + r;
+            if (g.rowwise) add_lowrank<float, kSub>(p, tr, re, rank_of(p, re), n, a);
+            store4<float>(p, tr, n, a);
           }
         }
       }
-      drain_sync();  // before the next tile is staged
     }
   }
   __syncwarp();
@@ -475,9 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       for (int i = rank * kDrain + threadIdx.x; i < (b - a) * quads; i += split * kDrain) {
         const int r = a + i / quads, c = i % quads * 4;
         const float4 s = sum4(r, c);
-        const float v[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) put_v(w.t0 + r, w.r0 + c + j, scale * v[j]);
+        put_v4(w.t0 + r, w.r0 + c, scale, s.x, s.y, s.z, s.w);
       }
     } else {
       const int rows = (int)min((int64_t)kBM, p.T - w.t0);
@@ -503,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
 
 template <bool kSub, bool kShrink, int kBN>
 cf_status launch(const Problem& p, Tiling g, cudaStream_t st) {
-  constexpr int smem = kStages * 2 * (kBM + kBN) * 128 + kBM * (kBN + 4) * 4 + 1024;
+  constexpr int smem = kStages * 2 * (kBM + kBN) * 128 + (kShrink ? 0 : kDrain / 32 * 4096) + 1024;
   auto* kern = k_adapter_f32<kSub, kShrink, kBN>;
   static std::atomic<uint64_t> allowed{0};
   CF_TRY(allow_smem(kern, smem, allowed, "k_adapter_f32"));
