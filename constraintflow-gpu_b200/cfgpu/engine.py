@@ -8,6 +8,7 @@ CROWN's all-crossing branch) run the general traversal of cfgpu.general over lib
 block kernels.  Torch only provides device memory and the stream handle.
 """
 import ctypes
+import math
 
 import torch
 
@@ -338,10 +339,12 @@ class DeepPolyEngine:
     def answer(self, l0, u0, labels, rules, adapter_ids=None):
         """Whether each region's answer under `rules` (ops.AnswerRules over the network's last
         layer) is its label: (margin [B] float32, rival [B] int32), margin > 0 certifies it
-        (ops.answer_margin).  Without a repetition factor the rules add a constant to each
-        logit, and the margin is taken from the property rows' bounds of y[label] - y[j]; with
-        one, from the bounds of the logits themselves.  labels [B] int64 device tensor of
-        answers in 0 .. n_last-1."""
+        (ops.answer_margin): ops.edit_logits of any float32 logits within the bounds then leaves
+        the label above every other answer.  Without a repetition factor the rules add constants
+        to a logit, and the margin is taken from the property rows' bounds of y[label] - y[j], less
+        what the additions to logits of that size may round by; with one, from the bounds of the
+        logits themselves.  labels [B] int64 device tensor of answers in 0 .. n_last-1.  The property
+        rows take B (n_last - 1) n_last floats."""
         from . import ops
         B, n = int(l0.shape[0]), self.n_last
         if (rules.rows, rules.n) != (B, n) or self.n_spec != n - 1:
@@ -353,16 +356,30 @@ class DeepPolyEngine:
         W = torch.empty(B, n - 1, n, dtype=torch.float32, device=self.device)
         stream = torch.cuda.current_stream(self.device).cuda_stream
         check(lib.cf_spec_matrix(B, n, labels.data_ptr(), W.data_ptr(), stream), "cf_spec_matrix")
-        if rules.c.repetition_dev:
-            _, _, sl, su = self.run(l0, u0, W, want_state=True, adapter_ids=adapter_ids)
+        edits = rules.launches > 1
+        if not edits:
+            lb, _ = self.run(l0, u0, W, adapter_ids=adapter_ids)
+        else:
+            lb, _, sl, su = self.run(l0, u0, W, want_state=True, adapter_ids=adapter_ids)
             at = self.N - self.n_spec - n
-            return ops.answer_margin(sl[:, at:at + n], su[:, at:at + n], labels, rules)
-        lb, _ = self.run(l0, u0, W, adapter_ids=adapter_ids)
+            l, u = sl[:, at:at + n], su[:, at:at + n]
+            if rules.c.repetition_dev:
+                return ops.answer_margin(l, u, labels, rules)
         # y[j] - y[label] <= -lb: upper bounds of the other answers relative to the label's 0
         row = torch.arange(n - 1, device=self.device)
         col = row + (row >= labels[:, None])
+        low = lb.float()
+        low = torch.where(low > lb, torch.nextafter(low, low.new_full((), -math.inf)), low)
         lo = torch.zeros(B, n, dtype=torch.float32, device=self.device)
-        up = torch.zeros_like(lo).scatter_(1, col, ops.unary("neg", lb.float(), torch.float32))
+        up = torch.zeros_like(lo).scatter_(1, col, ops.unary("neg", low, torch.float32))
+        if edits:
+            # Up to three additions round the edited logit, each by 2^-24 of at most |logit| + constants;
+            # the same three, and the sum below, the edited difference: 8 * 2^-24 of all of them for both.
+            # An infinite constant makes the logit infinite and rounds nothing.
+            K = rules.constants(self.device)
+            far = torch.maximum(l.abs(), u.abs()) + up.abs() + 4.0 * K
+            slack = torch.where((K > 0) & (K < math.inf), 2.0**-21 * far, torch.zeros_like(K))
+            lo, up = lo - slack, up + slack
         return ops.answer_margin(lo, up, labels, rules)
 
 

@@ -387,6 +387,19 @@ class AnswerRules:
         self._ref = ctypes.byref(self.c)
         self.launches = 1 + (count["tokens"] + count["bias_ids"] > 0)   # the stream, the edits
 
+    def constants(self, device):
+        """[rows, n] float32: a quarter of the sum of the magnitudes of what the penalties and the
+        biases add to each logit, 0 where nothing is added, infinite only where a constant is."""
+        k = self._keep
+
+        def quarter(t, sign):
+            return None if t is None else torch.where(t == 0, 0.0, sign * (0.25 * t.abs() + 1e-38))
+        added = AnswerRules(self.rows, self.n, k["tokens"], k["token_offsets"], k["prompt_len"],
+                            frequency=quarter(k["frequency"], -1.0), presence=quarter(k["presence"], -1.0),
+                            bias_ids=k["bias_ids"], bias_values=quarter(k["bias_values"], 1.0),
+                            bias_offsets=k["bias_offsets"])
+        return edit_logits(torch.zeros(self.rows, self.n, dtype=torch.float32, device=device), added)
+
 
 def _rules_rows(name, t, rules, dtype, gpu):
     """(t, its row stride) as rows for the rules: [rows, n] of `dtype` on `gpu`, its last dimension

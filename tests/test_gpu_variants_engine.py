@@ -207,3 +207,72 @@ def test_refusals():
         eng.answer(*box, y.to(dev()), ops.AnswerRules(2, 10))
     with pytest.raises(Exception, match="SHAPE MISMATCH"):
         eng.answer(*box, y.int().to(dev()), ops.AnswerRules(6, 10))
+
+
+def constant_network(logits):
+    """A network whose logits are `logits`, whatever its input: bounds without any slack."""
+    from cfgpu.engine import DeepPolyEngine
+
+    class Layer:
+        kind, W, b = "linear", torch.zeros(len(logits), 4), logits
+    return DeepPolyEngine([Layer()], 4, dev(), n_spec=len(logits) - 1)
+
+
+def certified(logits, labels, **kw):
+    """(margin, the logits as edited) for len(labels) regions of the constant network."""
+    from cfgpu import ops
+    B, n = len(labels), len(logits)
+    rules = ops.AnswerRules(B, n, **{k: v.to(dev()) for k, v in kw.items()})
+    box = torch.zeros(B, 4, device=dev()), torch.ones(B, 4, device=dev())
+    margin, _ = constant_network(logits).answer(*box, labels.to(dev()), rules)
+    return margin.cpu(), ops.edit_logits(logits.expand(B, n).contiguous().to(dev()), rules).cpu()
+
+
+def test_the_margin_is_of_the_rounded_rule():
+    """16777216 + 0.5 is a tie in float32, which 0 + 0.5 against 0 is not."""
+    margin, edited = certified(torch.full((2,), 16777216.0), torch.tensor([0]),
+                               bias_ids=torch.tensor([0], dtype=torch.int32), bias_values=torch.tensor([0.5]),
+                               bias_offsets=torch.tensor([0, 1]))
+    assert edited[0, 0] == edited[0, 1] and float(margin[0]) <= 0
+
+
+@pytest.mark.parametrize("size", [2.0**25, 2.0**12, 1.0])
+def test_certified_answers_win_after_rounding(size):
+    """Logits a few float32 steps apart and edits of a few steps: a margin above 0 means that the
+    label's edited logit is above all others.  The margin is at most 4 * 2^-21 of the magnitudes
+    (two answers' allowance of 2^-21 and its rounding, twice for good measure) below the real one."""
+    g = torch.Generator()
+    g.manual_seed(7)
+    B, n = 400, 5
+    step = size * 2.0**-23
+    for turn in range(4):
+        logits = (size + step * torch.randint(-3, 4, (n,), generator=g)).float()
+        labels = torch.randint(0, n, (B,), generator=g)
+        kw = dict(tokens=torch.randint(0, n, (3 * B,), generator=g).to(torch.int32),
+                  token_offsets=torch.arange(0, 3 * B + 1, 3),
+                  prompt_len=torch.randint(0, 3, (B,), generator=g).to(torch.int32),
+                  frequency=step * torch.randn(B, generator=g), presence=step * torch.randn(B, generator=g),
+                  bias_ids=torch.randint(0, n, (2 * B,), generator=g).to(torch.int32),
+                  bias_values=(10.0**turn) * step * torch.randn(2 * B, generator=g),
+                  bias_offsets=torch.arange(0, 2 * B + 1, 2))
+        margin, edited = certified(logits, labels, **kw)
+        others = edited.scatter(1, labels[:, None], -math.inf).max(dim=1).values
+        mine = edited.gather(1, labels[:, None])[:, 0]
+        assert (mine > others)[margin > 0].all()
+        real = V.rules(logits.expand(B, n), n, **kw)
+        gap = real.gather(1, labels[:, None])[:, 0] - real.scatter(1, labels[:, None], -math.inf).max(dim=1).values
+        far = logits.abs().max().double() + 2 * (real - logits.double()).abs().max() + 40 * step * 10.0**turn
+        assert (margin.double() <= gap + 2.0**-20 * far).all() and (margin.double() >= gap - 2.0**-19 * far).all()
+
+
+def test_bans_by_infinite_biases_and_by_sets():
+    """An answer with a bias of -inf is out, one with +inf bars any certificate, sets need no
+    allowance: the margin is then the difference of the logits itself."""
+    logits = torch.tensor([3.0, 5.0, 4.0, 1.0])
+    labels = torch.tensor([0, 0, 0])
+    margin, _ = certified(logits, labels, bias_ids=torch.tensor([1, 2, 1], dtype=torch.int32),
+                          bias_values=torch.tensor([-math.inf, -math.inf, math.inf]),
+                          bias_offsets=torch.tensor([0, 2, 2, 3]))
+    assert margin.tolist() == [2.0, -2.0, -math.inf]
+    margin, _ = certified(logits, labels, allowed=V.pack(torch.tensor([[True, False, False, True]] * 3)))
+    assert margin.tolist() == [2.0] * 3
