@@ -359,6 +359,8 @@ class AnswerRules:
         given = dict(tokens=tokens, token_offsets=token_offsets, prompt_len=prompt_len, repetition=repetition,
                      frequency=frequency, presence=presence, bias_ids=bias_ids, bias_values=bias_values,
                      bias_offsets=bias_offsets, allowed=allowed, allowed_row=allowed_row)
+        if allowed is not None and allowed_row is None and allowed.shape[:1] != (self.rows,):
+            raise Exception(f"SHAPE MISMATCH: {tuple(allowed.shape)} sets for {self.rows} rows without allowed_row")
         first = next(((k, t) for k, t in given.items() if t is not None), None)
         self.device = _cuda(*first) if first else None
         i32, i64, f32 = torch.int32, torch.int64, torch.float32

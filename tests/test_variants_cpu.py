@@ -166,3 +166,10 @@ def test_oracle_rules_by_hand():
     assert V.rules(x, n, **kw).tolist() == [[1.0, -4.0 - 1.0 - 0.25, -math.inf, 6.0]]
     m, j = V.margin(x, x, torch.tensor([3]), n, **kw)
     assert m.tolist() == [5.0] and j.tolist() == [0]
+
+
+@pytest.mark.parametrize("sets", [0, 1, 3])
+def test_a_row_without_a_set_of_its_own_is_refused(sets):
+    """Without allowed_row, row r has set r: fewer sets than rows would leave rows without their mask."""
+    with pytest.raises(Exception, match="SHAPE MISMATCH"):
+        ops.AnswerRules(2, 4, allowed=torch.zeros(sets, 1, dtype=torch.int32))
