@@ -19,7 +19,7 @@ cf_status check_layer(const cf_adapter_layer* L) {
              "adapter_matmul: dtype %d", L->dtype);
   CF_REQUIRE(L->n_out >= 0 && L->n_in >= 0 && L->n_adapters >= 0 && L->rank >= 0, CF_ERR_SHAPE,
              "adapter_matmul: negative size");
-  CF_REQUIRE(L->n_out <= 0x7fffff00 && L->n_in <= 0x7fffff00, CF_ERR_SHAPE, "adapter_matmul: layer too wide");
+  CF_REQUIRE(L->n_out <= kMaxWidth && L->n_in <= kMaxWidth, CF_ERR_SHAPE, "adapter_matmul: layer too wide");
   CF_REQUIRE(L->w_rs >= L->n_in, CF_ERR_SHAPE, "adapter_matmul: rows of W overlap");
   if (L->n_adapters > 0 && L->rank > 0)
     CF_REQUIRE(L->a_rs >= L->n_in && L->b_rs >= L->rank && L->a_es >= 0 && L->b_es >= 0, CF_ERR_SHAPE,

@@ -8,6 +8,9 @@
 namespace cf {
 namespace adapter {
 
+// Widths of a layer: the kernels step an int through the contraction and the columns, at most kMaxStep
+// past their end.
+constexpr int kMaxStep = 1 << 16, kMaxWidth = 0x7fffffff - kMaxStep;
 constexpr int kBM = 128;  // rows of a tile
 // tile_e: what a tile's rows carry
 constexpr int kNone = -1;   // no adapter

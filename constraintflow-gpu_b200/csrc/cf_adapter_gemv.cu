@@ -81,7 +81,8 @@ __global__ void __launch_bounds__(kThreads) k_adapter_gemv(const Problem p, int 
         for (int c = 0; c < kCols; ++c)
           acc[r][c] = fmaf(to_f32(((const T*)&x[r])[i]), to_f32(((const T*)&m[c])[i]), acc[r][c]);
   };
-  const int step = kThreads * E;
+  constexpr int step = kThreads * E;
+  static_assert(step + E <= kMaxStep, "k stays an int");
   int k = threadIdx.x * E;
   if (p.x_vec && p.m_vec) {
 #pragma unroll 4
@@ -124,6 +125,7 @@ __global__ void __launch_bounds__(kThreads) k_adapter_gemv_sub(const Problem p, 
   const bool vec = p.m_vec && n + E <= p.N;
   float acc[kRows][E] = {};
   constexpr int kStep = kThreads / 8;  // rows of W a turn
+  static_assert(kStep * (kUnroll + 1) <= kMaxStep, "k stays an int");
   for (int k0 = kb + warp * 4 + (lane >> 3); k0 < ke; k0 += kStep * kUnroll) {
     uint4 m[kUnroll];
     float w[kUnroll][kRows];

@@ -35,6 +35,7 @@ __global__ void __launch_bounds__(kRowThreads) k_adapter_shrink_rows(const Probl
     float v = 0.0f;
     if (p.p_vec && p.R % 8 == 0 && sizeof(T) == 2) {  // eight columns a load, two threads a row
       constexpr int kBatch = 8, kRows = kRowThreads / 2;
+      static_assert((kBatch + 1) * kRows <= kMaxStep, "k stays an int");
       const int c = (threadIdx.x & 1) * 8;
       const bool in = r0 + c < p.R;
       const T* at = P + r0 + c;
@@ -86,6 +87,7 @@ __global__ void __launch_bounds__(kRowThreads) k_adapter_shrink_rows(const Probl
     int k = lane * E;
     if (p.x_vec && p.p_vec) {  // kBatch pairs of loads in flight
       constexpr int kBatch = 8;
+      static_assert((kBatch + 1) * 32 * E <= kMaxStep, "k stays an int");
       for (; k + (kBatch - 1) * 32 * E + E <= K; k += kBatch * 32 * E) {
         uint4 a[kBatch], b[kBatch];
 #pragma unroll

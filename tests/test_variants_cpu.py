@@ -173,3 +173,14 @@ def test_a_row_without_a_set_of_its_own_is_refused(sets):
     """Without allowed_row, row r has set r: fewer sets than rows would leave rows without their mask."""
     with pytest.raises(Exception, match="SHAPE MISMATCH"):
         ops.AnswerRules(2, 4, allowed=torch.zeros(sets, 1, dtype=torch.int32))
+
+
+def test_widths_that_an_int_cannot_step_past_are_refused():
+    """The kernels step an int through the contraction, up to 2^16 past its end."""
+    most = 2**31 - 2**16 - 1
+    for n in (most + 1, 2**31 - 300, 2**31 - 256, 2**31 - 255, 2**31):
+        assert call(c_layer(n_in=n, w_rs=n, a_rs=n, a_es=4 * n), x_rs=n, ws=1 << 40, wsb=1 << 50) == _lib.CF_ERR_SHAPE
+        assert call(c_layer(n_out=n, b_es=4 * n), y=1 << 50, y_rs=n, ws=1 << 40, wsb=1 << 50) == _lib.CF_ERR_SHAPE
+    # within the limits: the next check is the one that answers
+    assert call(c_layer(n_in=most, w_rs=most, a_rs=most, a_es=4 * most), x_rs=most, y=1 << 50, wsb=0) == \
+        _lib.CF_ERR_WORKSPACE
