@@ -152,6 +152,8 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   CF_REQUIRE(((uintptr_t)x | (uintptr_t)y | (uintptr_t)L->W_dev | (uintptr_t)L->A_dev | (uintptr_t)L->B_dev |
               (uintptr_t)L->bias_dev) % size == 0,
              CF_ERR_SHAPE, "adapter_matmul: unaligned data");
+  CF_REQUIRE((uintptr_t)offsets % 8 == 0 && ((uintptr_t)ids | (uintptr_t)L->scale_dev | (uintptr_t)L->ranks_dev) % 4 == 0,
+             CF_ERR_SHAPE, "adapter_matmul: unaligned offsets, ids, scales or ranks");
   CF_REQUIRE(K == 0 || !rows_overlap(x, x_rs, K, y, y_rs, N, T, size), CF_ERR_SHAPE, "adapter_matmul: x and y overlap");
   Operand ox = operand_x(x, T, K, x_rs), W = operand_W(*L, substitute != 0), A = operand_A(*L), B = operand_B(*L);
   const size_t need = workspace(*L, substitute != 0, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);

@@ -800,6 +800,11 @@ cf_status check_rules(const cf_answer_rules* R, const char* what) {
   } else {
     CF_REQUIRE(!R->allowed_row_dev, CF_ERR_NULL, "%s: mask rows without masks", what);
   }
+  CF_REQUIRE(((uintptr_t)R->token_offsets_dev | (uintptr_t)R->bias_offsets_dev) % 8 == 0 &&
+                 ((uintptr_t)R->tokens_dev | (uintptr_t)R->prompt_len_dev | (uintptr_t)R->repetition_dev |
+                  (uintptr_t)R->frequency_dev | (uintptr_t)R->presence_dev | (uintptr_t)R->bias_ids_dev |
+                  (uintptr_t)R->bias_values_dev | (uintptr_t)R->allowed_dev | (uintptr_t)R->allowed_row_dev) % 4 == 0,
+             CF_ERR_SHAPE, "%s: unaligned rules", what);
   return CF_OK;
 }
 
@@ -873,6 +878,8 @@ extern "C" cf_status cf_answer_margin(const cf_answer_rules* R, const float* l, 
   if (R->rows == 0) return CF_OK;
   CF_REQUIRE(l && u && labels && margin && rival, CF_ERR_NULL, "answer_margin: NULL argument");
   CF_REQUIRE(((uintptr_t)l | (uintptr_t)u) % 4 == 0, CF_ERR_SHAPE, "answer_margin: unaligned rows");
+  CF_REQUIRE((uintptr_t)labels % 8 == 0 && ((uintptr_t)margin | (uintptr_t)rival) % 4 == 0, CF_ERR_SHAPE,
+             "answer_margin: unaligned labels or results");
   // 8192 answers a slice, 16384 where rows are long on average, fewer for few answers or few rows; a cluster of up
   // to eight for a row, as far as all rows' fit the GPU at once
   int log_s = R->n_tokens > R->rows * kMarginShort ? 14 : 13;

@@ -395,7 +395,7 @@ cf_status cf_conv_transpose(const cf_conv_geom* g, int64_t nb, int64_t per_b, co
  * No counterpart in the reference, whose regions share one network and one decision rule.
  * Requests (regions under certification, sequences being answered) may each carry a
  * low-rank adapter beside a layer's shared weights, and a rule by which their answer is
- * taken from the logits.
+ * taken from the logits.  Pointers are aligned to their elements; others are refused.
  *
  * An affine layer with adapters: W [n_out, n_in], bias [n_out] or NULL, and for adapter e
  * A_e [rank, n_in], B_e [n_out, rank] and scale_e, standing for W + scale_e B_e A_e.  Rows of

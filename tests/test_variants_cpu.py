@@ -184,3 +184,25 @@ def test_widths_that_an_int_cannot_step_past_are_refused():
     # within the limits: the next check is the one that answers
     assert call(c_layer(n_in=most, w_rs=most, a_rs=most, a_es=4 * most), x_rs=most, y=1 << 50, wsb=0) == \
         _lib.CF_ERR_WORKSPACE
+
+
+def test_unaligned_lists_are_refused():
+    """A misaligned address would end the context."""
+    S = _lib.CF_ERR_SHAPE
+    for at in (257, 258, 260):
+        assert call(c_layer(), off=at) == S
+    for at in (257, 258):
+        assert call(c_layer(), ids=at) == S
+        assert call(c_layer(scale_dev=at)) == S
+        assert call(c_layer(ranks_dev=at)) == S
+    full = dict(tokens_dev=256, token_offsets_dev=256, prompt_len_dev=256, repetition_dev=256, frequency_dev=256,
+                presence_dev=256, bias_ids_dev=256, bias_values_dev=256, bias_offsets_dev=256, allowed_dev=256,
+                allowed_row_dev=256, n_tokens=4, n_biases=4, n_masks=1, allowed_words=1)
+    for k in full:
+        if k.endswith("_dev"):
+            R = ctypes.byref(c_rules(**{**full, k: 260 if k.endswith("offsets_dev") else 258}))
+            assert _lib.lib.cf_edit_logits(R, _lib.CF_F32, 256, 10, 4096, 10, None) == S, k
+            assert _lib.lib.cf_answer_margin(R, 256, 10, 256, 10, 256, 256, 256, None) == S, k
+    R = ctypes.byref(c_rules())
+    for labels, margin, rival in ((260, 256, 256), (256, 258, 256), (256, 256, 257)):
+        assert _lib.lib.cf_answer_margin(R, 256, 10, 256, 10, labels, margin, rival, None) == S
