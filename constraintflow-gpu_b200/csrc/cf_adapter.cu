@@ -157,6 +157,9 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   CF_REQUIRE(K == 0 || !rows_overlap(x, x_rs, K, y, y_rs, N, T, size), CF_ERR_SHAPE, "adapter_matmul: x and y overlap");
   Operand ox = operand_x(x, T, K, x_rs), W = operand_W(*L, substitute != 0), A = operand_A(*L), B = operand_B(*L);
   const size_t need = workspace(*L, substitute != 0, T, n_requests, ox, W, A, B, nullptr, nullptr, nullptr);
+  const bool few = few_rows(*L, substitute != 0, T), rows = rows_alone(T, n_requests);
+  CF_REQUIRE(!adapters || !(few || rows) || L->rank <= kMaxRowRank, CF_ERR_SHAPE,
+             "adapter_matmul: rank %d for requests of few rows", (int)L->rank);
   CF_REQUIRE(ws_bytes >= need && (need == 0 || ws), CF_ERR_WORKSPACE, "adapter_matmul: workspace of %zu bytes, needs %zu",
              ws_bytes, need);
   CF_REQUIRE((uintptr_t)ws % 256 == 0, CF_ERR_WORKSPACE, "adapter_matmul: the workspace must be 256-byte aligned");
@@ -186,8 +189,7 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   p.p_vec = substitute ? b_vec : a_vec;
   p.q_vec = substitute ? a_vec : b_vec;
   p.y_vec = vec(y, T > 1 ? y_rs : 0, 0);
-  if (few_rows(*L, substitute != 0, T)) return launch_gemv(p, L->dtype, substitute != 0, as_stream(stream));
-  const bool rows = rows_alone(T, n_requests);
+  if (few) return launch_gemv(p, L->dtype, substitute != 0, as_stream(stream));
   if (L->dtype == CF_F32) return launch_f32(p, substitute != 0, rows, as_stream(stream));
   CF_TRY(launch_pack(pack, as_stream(stream)));
   if (K == 0) p.K = 8;

@@ -11,6 +11,7 @@ namespace adapter {
 // Widths of a layer: the kernels step an int through the contraction and the columns, at most kMaxStep
 // past their end.
 constexpr int kMaxStep = 1 << 16, kMaxWidth = 0x7fffffff - kMaxStep;
+constexpr int kMaxRowRank = 65535 * 8;  // v row by row: eight columns a CTA, dealt out over gridDim.y
 constexpr int kBM = 128;  // rows of a tile
 // tile_e: what a tile's rows carry
 constexpr int kNone = -1;   // no adapter

@@ -11,6 +11,7 @@ namespace {
 constexpr int kRowThreads = 256;
 template <bool kSub>
 constexpr int kRowCols = kSub ? 16 : kRowThreads / 32;
+static_assert(kMaxRowRank <= 65535 * kRowCols<false> && kMaxRowRank <= 65535 * kRowCols<true>, "a grid's rows");
 
 template <typename T, bool kSub>
 __global__ void __launch_bounds__(kRowThreads) k_adapter_shrink_rows(const Problem p, int64_t m_tiles, int whole) {

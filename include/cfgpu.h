@@ -402,7 +402,8 @@ cf_status cf_conv_transpose(const cf_conv_geom* g, int64_t nb, int64_t per_b, co
  * W, A_e and B_e are contiguous, at w_rs / a_rs / b_rs elements; adapter e starts at e*a_es /
  * e*b_es.  ranks_dev (or NULL) gives each adapter's own rank <= rank: what A_e and B_e hold
  * beyond it is not used, whatever it is.  Data is of one dtype (CF_F32, CF_BF16, CF_F16),
- * scales are float32.  n_out and n_in are below 2^31 - 2^16. */
+ * scales are float32.  n_out and n_in are below 2^31 - 2^16; ranks above
+ * 524280 are refused where requests have few rows. */
 typedef struct cf_adapter_layer {
   int32_t dtype;
   int32_t n_adapters;

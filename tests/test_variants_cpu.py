@@ -206,3 +206,11 @@ def test_unaligned_lists_are_refused():
     R = ctypes.byref(c_rules())
     for labels, margin, rival in ((260, 256, 256), (256, 258, 256), (256, 256, 257)):
         assert _lib.lib.cf_answer_margin(R, 256, 10, 256, 10, labels, margin, rival, None) == S
+
+
+@pytest.mark.parametrize("substitute", [0, 1])
+def test_ranks_beyond_a_grid_are_refused(substitute):
+    rank = 65535 * 8 + 1
+    L = c_layer(rank=rank, a_es=16 * rank, b_es=32 * rank, b_rs=rank)
+    assert call(L, substitute, x_rs=32, ws=1 << 40, wsb=1 << 50, y=1 << 50) == _lib.CF_ERR_SHAPE
+    assert b"rank" in _lib.lib.cf_last_error()
