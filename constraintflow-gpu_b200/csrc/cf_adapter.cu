@@ -5,6 +5,7 @@
 //   y = x M + b + v Q_e         M: W^T or W;  Q_e: B_e^T or A_e
 // a shrink kernel writes v to the workspace and a product kernel adds v Q_e to its tiles.
 #include "cf_adapter.cuh"
+#include "cf_tc.cuh"
 
 namespace cf {
 namespace {
@@ -170,6 +171,8 @@ extern "C" cf_status cf_adapter_matmul(const cf_adapter_layer* L, int32_t substi
   p.R = adapters ? L->rank : 0, p.E = adapters ? L->n_adapters : 0, p.Q = n_requests;
   p.x = ox.p, p.x_rs = ox.rs, p.M = W.p, p.y = y, p.y_rs = y_rs;
   p.scale = L->scale_dev, p.ranks = L->ranks_dev, p.offsets = offsets, p.ids = ids;
+  // CF_FAULT=adapter_withhold_stage withholds one arrival so that a wait runs out
+  p.max_polls = tc::wait_polls(), p.withhold = fault_injected("adapter_withhold_stage") ? 1 : 0;
   if (substitute) {
     p.m_ks = W.rs, p.m_ns = 1;
     p.P = B.p, p.p_es = B.es, p.p_ks = B.rs, p.p_rs = 1;

@@ -41,6 +41,8 @@ struct Problem {
   __nv_bfloat16 *v_hi, *v_lo;
   int64_t v_rs;
   int32_t *tile_e, *tile_q;
+  uint32_t max_polls;  // of every bounded wait
+  uint32_t withhold;   // 1: the first stage of operands is never released (the failure-path tests)
 };
 
 // The request of row t: -1 for a row of no request.

@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars.full[i], kLoad);
-      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.empty[i], i == 0 ? 1 + p.withhold : 1);
     }
     for (int i = 0; i < kBufs; ++i) {
       mbar_init(&bars.acc_full[i], 1);
@@ -232,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     };
     auto store = [&](const Chunks<kBN>& d) -> bool {
       const int s = it % kStages, round = it / kStages;
-      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 51)) return false;
+      if (!warp_wait(&bars.empty[s], (round & 1) ^ 1, err, 51, p.max_polls)) return false;
       const uint32_t a = sbase + s * kStageBytes, b = a + 2 * kABytes;
 #pragma unroll
       for (int j = 0; j < kBM * 8 / kLoad; ++j) put<float>(a, kABytes, prow + j * (kLoad / 8), chunk, d.x[j]);
@@ -324,8 +324,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     // one step into chunk ch; first / last of its chunk
     auto step = [&](int mmas, bool first, bool last, uint32_t id) -> bool {
       const int s = it % kStages, buf = ch % kBufs;
-      if (first && !mbar_wait(&bars.acc_empty[buf], ((ch / kBufs) & 1) ^ 1, err, 61)) return false;
-      if (!mbar_wait(&bars.full[s], (it / kStages) & 1, err, 62)) return false;
+      if (first && !warp_wait(&bars.acc_empty[buf], ((ch / kBufs) & 1) ^ 1, err, 61, p.max_polls)) return false;
+      if (!warp_wait(&bars.full[s], (it / kStages) & 1, err, 62, p.max_polls)) return false;
       tc_fence_after();
       if (lane == 0) {
         const uint32_t a = sbase + s * kStageBytes, d = tmem + buf * kBN;
@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       for (int i = 0; i < kBN / 2; ++i) acc[i] = 0.0f;
       auto drain = [&](bool mine) -> bool {
         const int buf = ch % kBufs;
-        if (!mbar_wait(&bars.acc_full[buf], (ch / kBufs) & 1, err, 71)) return false;
+        if (!warp_wait(&bars.acc_full[buf], (ch / kBufs) & 1, err, 71, p.max_polls)) return false;
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < kBN / 2; c += 16) {

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.empty[i], i == 0 ? 1 + p.withhold : 1);
     }
     mbar_init(&bars.done, 1);
     fence_mbar_init();
@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
     int it = 0, te, tr;
     auto stage_for = [&](uint32_t bytes) -> int {
       const int s = it % kStages, round = it / kStages;
-      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 11)) return -1;
+      if (!mbar_wait(&bars.empty[s], (round & 1) ^ 1, err, 11, p.max_polls)) return -1;
       mbar_arrive_expect_tx(&bars.full[s], bytes);
       ++it;
       return s;
@@ -182,15 +182,15 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
         load_b(b, &maps.q, (int)n0, r, te, kBN, &bars.full[s]);
       }
     }
-    if (!ok)  // copies in flight land before shared memory is given up
-      for (int i = max(0, it - kStages); i < it; ++i)
-        mbar_wait_drain(&bars.full[i % kStages], (i / kStages) & 1, err, 12);
+    // Copies in flight land before shared memory is given up: the others may have given up on them.
+    for (int i = max(0, it - kStages); i < it; ++i)
+      mbar_wait_drain(&bars.full[i % kStages], (i / kStages) & 1, err, 12);
   } else if (warp == kMmaWarp && lane == 0) {
     int it = 0, te = kNone, tr = 0;
     const uint32_t id = idesc(Kind<T>::kAb, cols, kMn);
     auto step = [&](int k16) -> bool {  // k16: MMAs of this step
       const int s = it % kStages, round = it / kStages;
-      if (!mbar_wait(&bars.full[s], round & 1, err, 21)) return false;
+      if (!mbar_wait(&bars.full[s], round & 1, err, 21, p.max_polls)) return false;
       tc_fence_after();
       const uint32_t a = sbase + s * kStageBytes, b = a + kABytes;
       const uint64_t ad = sw128_desc(a), bd = kMn ? mn_desc(b) : sw128_desc(b);
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
       }
     }
     mma_commit(&bars.done);
-    if (!ok) mbar_wait_drain(&bars.done, 0, err, 22);
+    mbar_wait_drain(&bars.done, 0, err, 22);  // every MMA has run before tensor memory is given up
   }
 
   // ---- the accumulators, staged in shared memory
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
   constexpr int kLd = kBN + 4;
   int te = kNone;
   if (warp < kProducerWarp) {
-    ok = mbar_wait(&bars.done, 0, err, 41);
+    ok = warp_wait(&bars.done, 0, err, 41, p.max_polls);
     tc_fence_after();
     const int row = (warp & 3) * 32 + lane;
     const bool any = kb < ke;  // else the accumulators were never written (or by low-rank steps only)

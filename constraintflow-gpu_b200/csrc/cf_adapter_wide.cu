@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&bars.full[i], 1);
-      mbar_init(&bars.empty[i], 1);
+      mbar_init(&bars.empty[i], i == 0 ? 1 + p.withhold : 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars.acc_full[i], 1);
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // x map entry at (xk, t0) and 256 columns from n0 on of b at contraction bk
     auto load = [&](const CUtensorMap* x, int xk, int64_t t0, const CUtensorMap* b, int bk, int64_t n0, int z) {
       const int s = it % kStages;
-      if (!mbar_wait(&bars.empty[s], ((it / kStages) & 1) ^ 1, err, 81)) return false;
+      if (!warp_wait(&bars.empty[s], ((it / kStages) & 1) ^ 1, err, 81, p.max_polls)) return false;
       if (lane == 0) {
         mbar_arrive_expect_tx(&bars.full[s], x_bytes + kBBytes);
         const uint32_t dst = sbase + s * kStageBytes;
@@ -129,14 +129,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && te >= 0) ok = lowrank(te, tr, 0, 0);
       if (ok && te == kFew) ok = for_requests(p, m, p.tile_q[m], reach(p, m, p.tile_q[m]), lowrank);
     }
-    if (!ok)  // copies in flight land before shared memory is given up
-      for (int i = max(0, it - kStages); i < it; ++i)
-        mbar_wait_drain(&bars.full[i % kStages], (i / kStages) & 1, err, 82);
+    // Copies in flight land before shared memory is given up: the others may have given up on them.
+    for (int i = max(0, it - kStages); i < it; ++i)
+      mbar_wait_drain(&bars.full[i % kStages], (i / kStages) & 1, err, 82);
   } else if (warp == kMmaWarp) {
     int it = 0, n_tile = 0, uses[2] = {0, 0};  // uses of each accumulator
     const uint32_t id = idesc(Kind<T>::kAb, kBN, kSub);
     auto claim = [&](int buf) {
-      if (!mbar_wait(&bars.acc_empty[buf], (uses[buf] & 1) ^ 1, err, 83)) return false;
+      if (!warp_wait(&bars.acc_empty[buf], (uses[buf] & 1) ^ 1, err, 83, p.max_polls)) return false;
       tc_fence_after();
       ++uses[buf];
       return true;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // k16 MMAs of the next stage into accumulator buf; first: it starts there
     auto step = [&](int buf, int k16, bool first) {
       const int s = it % kStages;
-      if (!mbar_wait(&bars.full[s], (it / kStages) & 1, err, 84)) return false;
+      if (!warp_wait(&bars.full[s], (it / kStages) & 1, err, 84, p.max_polls)) return false;
       tc_fence_after();
       if (lane == 0) {
         const uint32_t a = sbase + s * kStageBytes;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint8_t* stage = smem + kStages * kStageBytes + warp * 4096;  // 32 rows x 128 B, swizzled
     int n_tile = 0, uses[2] = {0, 0};
     auto full = [&](int buf) {
-      if (!mbar_wait(&bars.acc_full[buf], uses[buf] & 1, err, 86)) return false;
+      if (!warp_wait(&bars.acc_full[buf], uses[buf] & 1, err, 86, p.max_polls)) return false;
       tc_fence_after();
       ++uses[buf];
       return true;

@@ -159,14 +159,6 @@ __device__ __forceinline__ void load16g(const float* __restrict__ p, int k0, int
   }
 }
 
-// Bounded wait by every lane of a warp with a warp-uniform result, so that warp-collective
-// code after it (__syncwarp, tcgen05.ld) is reached by all lanes or by none.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int site,
-                                          uint32_t max_polls = kMaxPolls) {
-  const bool ok = mbar_wait(bar, parity, err, site, max_polls);
-  return __all_sync(0xffffffffu, ok);
-}
-
 // 16 consecutive floats at shared-memory byte address `saddr` (16-byte aligned): four
 // ld.shared.v4.  Ordered after the mbarrier waits that publish them (asm volatile).
 __device__ __forceinline__ void lds16(uint32_t saddr, float (&o)[16]) {
@@ -726,13 +718,8 @@ static cf_status chain_prepare(const ChainParams& P, ChainParams& Q, size_t& sme
   CF_REQUIRE(P.st[P.S - 1].N == P.n0, CF_ERR_SHAPE, "chain: last step does not reach the input");
   Q = P;
   if (Q.ld_box == 0) Q.ld_box = Q.n0;
-  // bounded-wait limit: kMaxPolls, or CF_WAIT_POLLS (>= 256) for the failure-path test;
   // CF_FAULT=chain_withhold_acc withholds one arrival so that a wait runs out
-  Q.max_polls = kMaxPolls;
-  if (const char* e = getenv("CF_WAIT_POLLS")) {
-    const long v = strtol(e, nullptr, 10);
-    if (v >= 256 && v < (long)kMaxPolls) Q.max_polls = (uint32_t)v;
-  }
+  Q.max_polls = wait_polls();
   Q.withhold_acc = fault_injected("chain_withhold_acc") ? 1 : 0;
   CF_REQUIRE(Q.ld_box >= Q.n0, CF_ERR_SHAPE, "chain: box row stride %lld < %lld", (long long)Q.ld_box,
              (long long)Q.n0);

@@ -62,6 +62,23 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int* e
   return false;
 }
 
+// Bounded wait by every lane of a warp with a warp-uniform result, so that warp-collective
+// code after it (__syncwarp, tcgen05.ld) is reached by all lanes or by none.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int site,
+                                          uint32_t max_polls = kMaxPolls) {
+  const bool ok = mbar_wait(bar, parity, err, site, max_polls);
+  return __all_sync(0xffffffffu, ok);
+}
+
+// The poll limit of a launch: kMaxPolls, or CF_WAIT_POLLS (>= 256) for the failure-path tests.
+inline uint32_t wait_polls() {
+  if (const char* e = getenv("CF_WAIT_POLLS")) {
+    const long v = strtol(e, nullptr, 10);
+    if (v >= 256 && v < (long)kMaxPolls) return (uint32_t)v;
+  }
+  return kMaxPolls;
+}
+
 // Bounded wait for work already in flight (bulk copies, MMAs) before the CTA releases what
 // that work writes: unlike mbar_wait it does not give up when another role has recorded
 // an error, only after kMaxPolls polls (then it records `site` if nothing was recorded).

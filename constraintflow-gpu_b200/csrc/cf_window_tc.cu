@@ -83,11 +83,6 @@ __device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~(uintptr_t)1023);
 }
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int site) {
-  const bool ok = mbar_wait(bar, parity, err, site);
-  return __all_sync(0xffffffffu, ok);
-}
-
 // B^T image: element (n, k) -> plane c = k / 32 of the hi / lo image at the SW128 position
 // of (n, k % 32); zero outside [0, N) x [0, K) and past the kernel.  TY, TX: k taps per
 // dimension; f: the output blocking factor (S = s*f phases per dimension).

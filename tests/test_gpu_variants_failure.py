@@ -1,0 +1,64 @@
+"""Failure detection of the adapter product without a GPU fault: bounded device waits that run out.
+
+With a short poll limit (CF_WAIT_POLLS) and one arrival withheld (CF_FAULT=adapter_withhold_stage:
+the barrier of each CTA's first stage of operands expects an arrival that nothing makes), the loads
+of a later step wait for that stage and give up, the MMAs wait for the loads, the epilogue for the
+MMAs.  Copies and MMAs in flight are awaited before shared memory and tensor memory are released,
+adapter_check reports the site, and the next call, without the fault, gives the usual bits.
+"""
+import re
+
+import pytest
+import torch
+
+from test_gpu_variants import BF16, F16, F32, layer, make, ops
+
+pytestmark = pytest.mark.gpu
+
+# the bounded waits of k_adapter_tile, k_adapter_wide and k_adapter_f32
+TILE, WIDE, F32_SITES = {11, 21, 41}, {81, 83, 84, 86}, {51, 61, 62, 71}
+
+# more steps of the contraction than stages in every CTA
+CASES = [
+    # dtype, T, K, N, sites of v's kernel and of the product's
+    (BF16, 200, 1024, 256, TILE), (F16, 200, 1024, 256, TILE),
+    (BF16, 1024, 512, 1280, TILE | WIDE), (F16, 1024, 512, 2304, TILE | WIDE),
+    (F32, 1100, 128, 520, F32_SITES),
+]
+
+
+def withhold(monkeypatch):
+    monkeypatch.setenv("CF_WAIT_POLLS", "65536")
+    monkeypatch.setenv("CF_FAULT", "adapter_withhold_stage")
+
+
+def restore(monkeypatch):
+    monkeypatch.delenv("CF_FAULT")
+    monkeypatch.delenv("CF_WAIT_POLLS")
+
+
+def gave_up(call):
+    """The site at which a bounded wait gave up, as `call` reports it."""
+    from cfgpu import _lib
+    with pytest.raises(_lib.CfError) as e:
+        call()
+    m = re.search(r"gave up \(site (\d+)\)", str(e.value))
+    assert m and e.value.status == _lib.CF_ERR_TIMEOUT, e.value
+    return int(m.group(1))
+
+
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "x".join(map(str, c[1:4])) + str(c[0])[5:])
+def test_a_stage_that_is_never_released(monkeypatch, case, sub):
+    dtype, T, K, N, sites = case
+    t = make(T, K, N, 16, 3, 3, dtype, sub, seed=8)
+    args = t["x"].cuda(), layer(t), t["offsets"].cuda(), t["ids"].cuda(), sub
+    good = ops().adapter_matmul(*args)
+    ops().adapter_check()
+    withhold(monkeypatch)
+    ops().adapter_matmul(*args)
+    assert gave_up(ops().adapter_check) in sites
+    restore(monkeypatch)
+    ops().adapter_check()                      # reported once
+    assert torch.equal(ops().adapter_matmul(*args), good)
+    ops().adapter_check()
