@@ -210,6 +210,11 @@ __device__ __forceinline__ void add_lowrank16(const Problem& p, int64_t t, int e
   }
 }
 
+// A CTA's error word, by one warp at its end, into its kernel file's.
+__device__ __forceinline__ void report(int err, int* site) {
+  if (err != 0 && (threadIdx.x & 31) == 0) atomicCAS(site, 0, err);
+}
+
 // Read and clear a kernel file's error word.
 inline cf_status take_site(int* symbol, int* site, cudaStream_t st) {
   void* at = nullptr;

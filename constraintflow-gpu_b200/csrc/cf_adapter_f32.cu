@@ -53,7 +53,7 @@ constexpr int kStep = 32;   // contraction of a stage: 128 bytes
 constexpr int kChunk = 2;   // steps of one accumulation
 constexpr int kStages = 2, kBufs = 2;
 
-// A bounded wait that gave up leaves its site here (cf_adapter_check).
+// The site at which a bounded wait gave up (cf_adapter_check); kernels only write it.
 __device__ int g_err;
 
 template <int kRegs>
@@ -112,6 +112,7 @@ __device__ __forceinline__ bool tile_of(const Problem& p, const Tiling& g, int64
 struct Bars {
   uint64_t full[kStages], empty[kStages], acc_full[kBufs], acc_empty[kBufs], done;
   uint32_t tmem;
+  int err;  // the site at which a wait of this CTA gave up: the others follow
 };
 
 template <int kBN>
@@ -153,13 +154,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       mbar_init(&bars.acc_empty[i], kDrain / 32);
     }
     mbar_init(&bars.done, 1);
+    bars.err = 0;
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  int* err = &g_err;
+  int* err = &bars.err;
   const int n_k = (int)((p.K + kStep - 1) / kStep);
   const int kb = (int)((int64_t)n_k * rank / split), ke = (int)((int64_t)n_k * (rank + 1) / split);
   // the requests' low-rank parts as chunks
@@ -467,6 +469,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     tc_fence_after();
     tmem_relinquish();
     tmem_dealloc(tmem, kBufs * kBN);
+    report(bars.err, &g_err);
   }
   if (split == 1) return;
 

@@ -32,7 +32,7 @@ constexpr int kWorkers = 256;  // warps 0-7: epilogue
 constexpr int kProducerWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 320;
 
-// A bounded wait that gave up leaves its site here (cf_adapter_check).
+// The site at which a bounded wait gave up (cf_adapter_check); kernels only write it.
 __device__ int g_err;
 
 struct Tiling {
@@ -48,6 +48,7 @@ template <int kStages>
 struct Bars {
   uint64_t full[kStages], empty[kStages], done;
   uint32_t tmem;
+  int err;  // the site at which a wait of this CTA gave up: the others follow
 };
 
 template <typename T, bool kSub, bool kShrink, int kBN, int kStages>
@@ -118,13 +119,14 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
       mbar_init(&bars.empty[i], i == 0 ? 1 + p.withhold : 1);
     }
     mbar_init(&bars.done, 1);
+    bars.err = 0;
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  int* err = &g_err;
+  int* err = &bars.err;
 
   // The low-rank steps behind the contraction: only known once the shrink kernel is done.
   auto lowrank_steps = [&](int& te, int& tr) {
@@ -257,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) k_adapter_tile(const Problem p, c
     tc_fence_after();
     tmem_relinquish();
     tmem_dealloc(tmem, kBN < 32 ? 32 : kBN);
+    report(bars.err, &g_err);
   }
   if (split > 1) cl.sync();
   if (warp < kProducerWarp) {

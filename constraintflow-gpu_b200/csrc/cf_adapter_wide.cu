@@ -28,7 +28,7 @@ constexpr int kEpilogue = 256, kProducerWarp = 8, kMmaWarp = 9, kThreads = 320;
 constexpr uint32_t kABytes = kBM * 128, kBBytes = kBN * 128, kStageBytes = kABytes + kBBytes;
 constexpr int kSmem = kStages * kStageBytes + 8 * 4096 + 1024;
 
-// A bounded wait that gave up leaves its site here (cf_adapter_check).
+// The site at which a bounded wait gave up (cf_adapter_check); kernels only write it.
 __device__ int g_err;
 
 // Tiles go through the row tiles of a group of kGroup first, then through the columns: what 148 CTAs read
@@ -39,6 +39,7 @@ constexpr int kGroup = 16;
 struct Bars {
   uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2], done;
   uint32_t tmem;
+  int err;  // the site at which a wait of this CTA gave up: the others follow
 };
 
 template <typename T, bool kSub>
@@ -65,13 +66,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bars.acc_empty[i], kEpilogue / 32);
     }
     mbar_init(&bars.done, 1);
+    bars.err = 0;
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars.tmem;
-  int* err = &g_err;
+  int* err = &bars.err;
   const int n_k = (int)((p.K + kStep - 1) / kStep);
   bool ok = true, waited = false;
   const int64_t n_tiles = units / m_tiles;
@@ -304,6 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_relinquish();
     tmem_dealloc(tmem, 512);
+    report(bars.err, &g_err);
   }
 }
 

@@ -62,3 +62,24 @@ def test_a_stage_that_is_never_released(monkeypatch, case, sub):
     ops().adapter_check()                      # reported once
     assert torch.equal(ops().adapter_matmul(*args), good)
     ops().adapter_check()
+
+
+def test_later_waits_do_not_give_up_on_an_earlier_one(monkeypatch):
+    """Until it is reported, a wait that gave up is a record only: a later call whose epilogue waits
+    through a contraction of 2^20 gives the usual bits."""
+    K = 1 << 20
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    x, W = (torch.randn(128, K, generator=g, device="cuda").bfloat16() for _ in range(2))
+    L = ops().AdapterLayer(W, W.new_empty(1, 0, K), W.new_empty(1, 128, 0), torch.ones(1, device="cuda"))
+    rest = torch.tensor([0, 128]).cuda(), torch.zeros(1, dtype=torch.int32).cuda()
+    good = ops().adapter_matmul(x, L, *rest)
+    t = make(200, 1024, 256, 16, 3, 3, BF16, False, seed=8)
+    withhold(monkeypatch)
+    ops().adapter_matmul(t["x"].cuda(), layer(t), t["offsets"].cuda(), t["ids"].cuda())
+    torch.cuda.synchronize()
+    restore(monkeypatch)
+    for _ in range(3):
+        assert torch.equal(ops().adapter_matmul(x, L, *rest), good)
+    assert gave_up(ops().adapter_check) in TILE
+    ops().adapter_check()
