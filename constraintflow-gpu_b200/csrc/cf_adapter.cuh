@@ -24,7 +24,9 @@ constexpr int kFewRequests = 8;
 struct Problem {
   int64_t T, K, N;
   int32_t R, E;
-  int64_t Q;  // requests
+  uint32_t max_polls;  // of every bounded wait
+  uint32_t withhold;   // 1: the first stage of operands is never released (the failure-path tests)
+  int64_t Q;           // requests
   const void *x, *M, *bias, *P, *Qm;
   int64_t x_rs, m_ks, m_ns, p_es, p_ks, p_rs, q_es, q_rs, q_ns;
   const float* scale;
@@ -41,8 +43,6 @@ struct Problem {
   __nv_bfloat16 *v_hi, *v_lo;
   int64_t v_rs;
   int32_t *tile_e, *tile_q;
-  uint32_t max_polls;  // of every bounded wait
-  uint32_t withhold;   // 1: the first stage of operands is never released (the failure-path tests)
 };
 
 // The request of row t: -1 for a row of no request.

@@ -326,10 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
     // one step into chunk ch; first / last of its chunk
     auto step = [&](int mmas, bool first, bool last, uint32_t id) -> bool {
       const int s = it % kStages, buf = ch % kBufs;
-      if (first && !warp_wait(&bars.acc_empty[buf], ((ch / kBufs) & 1) ^ 1, err, 61, p.max_polls)) return false;
-      if (!warp_wait(&bars.full[s], (it / kStages) & 1, err, 62, p.max_polls)) return false;
+      const bool ok = (!first || mbar_wait(&bars.acc_empty[buf], ((ch / kBufs) & 1) ^ 1, err, 61, p.max_polls)) &&
+                      mbar_wait(&bars.full[s], (it / kStages) & 1, err, 62, p.max_polls);
       tc_fence_after();
-      if (lane == 0) {
+      if (ok && lane == 0) {
         const uint32_t a = sbase + s * kStageBytes, d = tmem + buf * kBN;
         const uint64_t ad = sw128_desc(a), bd = sw128_desc(a + 2 * kABytes);
         constexpr uint64_t kALo = kABytes >> 4, kBLo = kBBytes >> 4;
@@ -341,10 +341,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
         mma_commit(&bars.empty[s]);
         if (last) mma_commit(&bars.acc_full[buf]);
       }
-      __syncwarp();
       ++it;
       ch += last;
-      return true;
+      return __all_sync(0xffffffffu, ok);  // all lanes go on, or none; behind the MMAs, which it would delay
     };
     for (int64_t unit = cluster; unit < g.units && ok; unit += g.clusters) {
       if (!tile_of<kShrink, kBN>(p, g, unit, w)) continue;
@@ -385,7 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       for (int i = 0; i < kBN / 2; ++i) acc[i] = 0.0f;
       auto drain = [&](bool mine) -> bool {
         const int buf = ch % kBufs;
-        if (!warp_wait(&bars.acc_full[buf], (ch / kBufs) & 1, err, 71, p.max_polls)) return false;
+        const bool ok = mbar_wait(&bars.acc_full[buf], (ch / kBufs) & 1, err, 71, p.max_polls);
+        // (a chunk that a lane gave up on is read all the same, and is worth nothing: the lanes agree behind it)
         tc_fence_after();
 #pragma unroll
         for (int c = 0; c < kBN / 2; c += 16) {
@@ -397,10 +397,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
           for (int i = 0; i < 16; ++i) acc[c + i] = mine ? acc[c + i] + v[i] : acc[c + i];
         }
         tc_fence_before();
-        __syncwarp();
+        const bool all = __all_sync(0xffffffffu, ok);
         if (lane == 0) mbar_arrive(&bars.acc_empty[buf]);
         ++ch;
-        return true;
+        return all;
       };
       for (int k = kb; k < ke && ok; k += kChunk) ok = drain(true);
       if (!kShrink && p.R > 0 && !waited) {

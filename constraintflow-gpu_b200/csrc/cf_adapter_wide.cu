@@ -91,12 +91,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
 
   if (warp == kProducerWarp) {
-    int it = 0;
+    int it = 0, loads = 0;  // steps; those that lane 0 has loaded
     // x map entry at (xk, t0) and 256 columns from n0 on of b at contraction bk
     auto load = [&](const CUtensorMap* x, int xk, int64_t t0, const CUtensorMap* b, int bk, int64_t n0, int z) {
       const int s = it % kStages;
-      if (!warp_wait(&bars.empty[s], ((it / kStages) & 1) ^ 1, err, 81, p.max_polls)) return false;
-      if (lane == 0) {
+      const bool ok = mbar_wait(&bars.empty[s], ((it / kStages) & 1) ^ 1, err, 81, p.max_polls);
+      if (ok && lane == 0) {
         mbar_arrive_expect_tx(&bars.full[s], x_bytes + kBBytes);
         const uint32_t dst = sbase + s * kStageBytes;
         tma_3d(dst, x, xk, (int)t0, 0, &bars.full[s]);
@@ -106,10 +106,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           tma_3d(dst + kABytes, b, bk, (int)n0, z, &bars.full[s]);
         }
+        ++loads;
       }
-      __syncwarp();
       ++it;
-      return true;
+      return (bool)__all_sync(0xffffffffu, ok);  // all lanes go on, or none; behind the loads, which it would delay
     };
     for (int64_t unit = blockIdx.x; unit < units && ok; unit += gridDim.x) {
       int64_t m, n0;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ok && te == kFew) ok = for_requests(p, m, p.tile_q[m], reach(p, m, p.tile_q[m]), lowrank);
     }
     // Copies in flight land before shared memory is given up: the others may have given up on them.
-    for (int i = max(0, it - kStages); i < it; ++i)
+    for (int i = max(0, loads - kStages); i < loads; ++i)
       mbar_wait_drain(&bars.full[i % kStages], (i / kStages) & 1, err, 82);
   } else if (warp == kMmaWarp) {
     int it = 0, n_tile = 0, uses[2] = {0, 0};  // uses of each accumulator
@@ -146,9 +146,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // k16 MMAs of the next stage into accumulator buf; first: it starts there
     auto step = [&](int buf, int k16, bool first) {
       const int s = it % kStages;
-      if (!warp_wait(&bars.full[s], (it / kStages) & 1, err, 84, p.max_polls)) return false;
+      const bool ok = mbar_wait(&bars.full[s], (it / kStages) & 1, err, 84, p.max_polls);
       tc_fence_after();
-      if (lane == 0) {
+      if (ok && lane == 0) {
         const uint32_t a = sbase + s * kStageBytes;
         const uint64_t ad = sw128_desc(a), bd = kSub ? mn_desc(a + kABytes) : sw128_desc(a + kABytes);
         constexpr uint64_t kAStep = 32 >> 4, kBStep = kSub ? (16 * 128) >> 4 : 32 >> 4;
@@ -156,9 +156,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           mma_f16(tmem + buf * kBN, ad + j * kAStep, bd + j * kBStep, id, !first || j > 0);
         mma_commit(&bars.empty[s]);
       }
-      __syncwarp();
       ++it;
-      return true;
+      return (bool)__all_sync(0xffffffffu, ok);
     };
     auto lowrank = [&](int buf, int rank, bool first) {
       for (int r = 0; r < rank; r += kStep) {
