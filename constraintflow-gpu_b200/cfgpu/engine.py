@@ -183,7 +183,8 @@ class DeepPolyEngine:
         spec_W: [B, n_spec, n_last] float32 device tensor (property matrix).
         Returns (lb, ub) float64 [B, n_spec] and, if want_state, (state_l, state_u)
         float32 [B, N] with every neuron's bounds in the reference's neuron order.
-        check_device=True synchronises and raises if a bounded device wait gave up.
+        check_device=True synchronises and raises if a bounded device wait gave up (with adapter_ids: in
+        any adapter_matmul on this device since the last check).
         replay=(dec_l, dec_u): [B, N] float32 device tensors (state layout) from which every
         ReLU branch decision is taken (cf_deeppoly_run_replay; DeepPoly chains only).
         """
@@ -215,6 +216,10 @@ class DeepPolyEngine:
             if want_state:
                 sl.copy_(sl_g)
                 su.copy_(su_g)
+            if check_device and adapter_ids is not None:
+                from . import ops
+                ops.adapter_check(self.device)
+            if want_state:
                 return lb, ub, sl, su
             return lb, ub
         ws = self._workspace(B, self.workspace_budget if workspace_budget is None else workspace_budget)
@@ -336,7 +341,7 @@ class DeepPolyEngine:
         lb, ub = self.run(l0, u0, W, out=out)
         return lb, ub
 
-    def answer(self, l0, u0, labels, rules, adapter_ids=None):
+    def answer(self, l0, u0, labels, rules, adapter_ids=None, check_device=False):
         """Whether each region's answer under `rules` (ops.AnswerRules over the network's last
         layer) is its label: (margin [B] float32, rival [B] int32), margin > 0 certifies it
         (ops.answer_margin): ops.edit_logits of any float32 logits within the bounds then leaves
@@ -344,7 +349,8 @@ class DeepPolyEngine:
         to a logit, and the margin is taken from the property rows' bounds of y[label] - y[j], less
         what the additions to logits of that size may round by; with one, from the bounds of the
         logits themselves.  labels [B] int64 device tensor of answers in 0 .. n_last-1.  The property
-        rows take B (n_last - 1) n_last floats."""
+        rows take B (n_last - 1) n_last floats.  check_device as in run: without it a margin may come
+        from bounds that a device wait gave up on."""
         from . import ops
         B, n = int(l0.shape[0]), self.n_last
         if (rules.rows, rules.n) != (B, n) or self.n_spec != n - 1:
@@ -358,9 +364,10 @@ class DeepPolyEngine:
         check(lib.cf_spec_matrix(B, n, labels.data_ptr(), W.data_ptr(), stream), "cf_spec_matrix")
         edits = rules.launches > 1
         if not edits:
-            lb, _ = self.run(l0, u0, W, adapter_ids=adapter_ids)
+            lb, _ = self.run(l0, u0, W, adapter_ids=adapter_ids, check_device=check_device)
         else:
-            lb, _, sl, su = self.run(l0, u0, W, want_state=True, adapter_ids=adapter_ids)
+            lb, _, sl, su = self.run(l0, u0, W, want_state=True, adapter_ids=adapter_ids,
+                                     check_device=check_device)
             at = self.N - self.n_spec - n
             l, u = sl[:, at:at + n], su[:, at:at + n]
             if rules.c.repetition_dev:

@@ -83,3 +83,26 @@ def test_later_waits_do_not_give_up_on_an_earlier_one(monkeypatch):
         assert torch.equal(ops().adapter_matmul(x, L, *rest), good)
     assert gave_up(ops().adapter_check) in TILE
     ops().adapter_check()
+
+
+def test_the_engine_reports_a_wait_that_gave_up(monkeypatch):
+    """run and answer with check_device raise, and succeed on the next call.  64 regions: 3200 rows
+    through 50 x 784 weights are more tiles than CTAs, so some need a stage twice."""
+    from cfgpu import nets
+    from test_gpu_variants_engine import dev, engine, make as network
+    wl, y, l0, u0, adapters, ids = network(B=64)
+    eng = engine(wl, adapters)
+    eng.graphs = False                                  # a captured pass keeps the launches it was made of
+    box, spec = (l0.to(dev()), u0.to(dev())), nets.spec_weight(y).to(dev())
+    kw = dict(adapter_ids=ids.to(dev()), check_device=True)
+    rules = ops().AnswerRules(64, 10)
+    lb, ub = eng.run(*box, spec, **kw)
+    margin, _ = eng.answer(*box, y.to(dev()), rules, **kw)
+    withhold(monkeypatch)
+    assert gave_up(lambda: eng.run(*box, spec, **kw)) in F32_SITES
+    assert gave_up(lambda: eng.run(*box, spec, want_state=True, **kw)) in F32_SITES
+    assert gave_up(lambda: eng.answer(*box, y.to(dev()), rules, **kw)) in F32_SITES
+    restore(monkeypatch)
+    again = eng.run(*box, spec, **kw)
+    assert torch.equal(again[0], lb) and torch.equal(again[1], ub)
+    assert torch.equal(eng.answer(*box, y.to(dev()), rules, **kw)[0], margin)
