@@ -50,6 +50,8 @@ class DeepPolyEngine:
         self.device = torch.device(device)
         if self.device.type != "cuda":
             raise ValueError("DeepPolyEngine runs on a CUDA device only (no CPU fallback)")
+        if self.device.index is None:          # tensors are on a device with an index
+            self.device = torch.device("cuda", torch.cuda.current_device())
         self.input_size = int(input_size)
         self.n_spec = int(n_spec)
         relax = {"deeppoly": _lib.CF_RELAX_DEEPPOLY, "crown": _lib.CF_RELAX_CROWN, "zono": _lib.CF_RELAX_ZONO,

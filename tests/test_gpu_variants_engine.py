@@ -276,3 +276,16 @@ def test_bans_by_infinite_biases_and_by_sets():
     assert margin.tolist() == [2.0, -2.0, -math.inf]
     margin, _ = certified(logits, labels, allowed=V.pack(torch.tensor([[True, False, False, True]] * 3)))
     assert margin.tolist() == [2.0] * 3
+
+
+def test_a_device_without_an_index_is_the_current_one():
+    from cfgpu import nets, ops
+    from cfgpu.engine import DeepPolyEngine
+    wl, y, l0, u0, adapters, ids = make()
+    eng = DeepPolyEngine(wl.layers, wl.input_size, "cuda", adapters=adapters)
+    assert eng.device == torch.device("cuda", torch.cuda.current_device())
+    box = l0.cuda(), u0.cuda()
+    got = eng.run(*box, nets.spec_weight(y).cuda(), adapter_ids=ids.cuda())
+    want = engine(wl, adapters).run(*box, nets.spec_weight(y).cuda(), adapter_ids=ids.cuda())
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    eng.answer(*box, y.cuda(), ops.AnswerRules(l0.shape[0], 10), adapter_ids=ids.cuda())
