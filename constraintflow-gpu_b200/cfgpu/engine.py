@@ -214,10 +214,7 @@ class DeepPolyEngine:
                     adapter_ids.device != self.device or not adapter_ids.is_contiguous():
                 raise Exception(f"SHAPE MISMATCH: adapter_ids must be contiguous int32 {(B,)} on {self.device}")
         if self.net is None or adapter_ids is not None:
-            lb, ub, sl_g, su_g = self._general_run(l0, u0, spec_W, lb, ub, adapter_ids)
-            if want_state:
-                sl.copy_(sl_g)
-                su.copy_(su_g)
+            self._general_run(l0, u0, spec_W, lb, ub, sl, su, adapter_ids)
             if check_device and adapter_ids is not None:
                 from . import ops
                 ops.adapter_check(self.device)
@@ -248,10 +245,7 @@ class DeepPolyEngine:
             st = lib.cf_deeppoly_check(ws.data_ptr(), stream)
             if st == _lib.CF_ERR_UNSUPPORTED:
                 # a ReLU layer took the all-crossing branch: its polyexps mix layers
-                lb, ub, sl_g, su_g = self._general_run(l0, u0, spec_W, lb, ub)
-                if want_state:
-                    sl.copy_(sl_g)
-                    su.copy_(su_g)
+                self._general_run(l0, u0, spec_W, lb, ub, sl, su)
             else:
                 check(st, "device status")
         elif check_device:
@@ -260,13 +254,14 @@ class DeepPolyEngine:
             return lb, ub, sl, su
         return lb, ub
 
-    def _general_run(self, l0, u0, spec_W, lb, ub, adapter_ids=None):
-        """Bounds through the general lowest-layer-first traversal (cfgpu.general).
+    def _general_run(self, l0, u0, spec_W, lb, ub, state_l, state_u, adapter_ids=None):
+        """Bounds through the general lowest-layer-first traversal (cfgpu.general) into lb, ub
+        and, where they are not None, state_l, state_u.
 
         DeepPoly's traversal takes no data-dependent decision on the host, so for a given
         batch size its launches are captured once in a CUDA graph and replayed (the inputs
-        are copied into the graph's buffers); CROWN decides its ReLU branches on the host and
-        runs eagerly."""
+        are copied into the graph's buffers, which a call on another stream waits for); CROWN
+        decides its ReLU branches on the host and runs eagerly."""
         from . import general
         if self.certifier == "deeppoly" and self.graphs:
             key = (int(l0.shape[0]), adapter_ids is not None)
@@ -274,6 +269,10 @@ class DeepPolyEngine:
             if g is None:
                 g = self._capture(l0, u0, spec_W, adapter_ids, key)
             if g is not None:
+                stream = torch.cuda.current_stream(self.device)
+                ordered = not torch.cuda.is_current_stream_capturing()
+                if ordered:
+                    stream.wait_event(g["done"])
                 g["l0"].copy_(l0)
                 g["u0"].copy_(u0)
                 g["W"].copy_(spec_W)
@@ -283,18 +282,25 @@ class DeepPolyEngine:
                 self.replayed_launches += g["launches"]
                 lb.copy_(g["sl"][:, -self.n_spec:])
                 ub.copy_(g["su"][:, -self.n_spec:])
-                return lb, ub, g["sl"], g["su"]
+                if state_l is not None:
+                    state_l.copy_(g["sl"])
+                    state_u.copy_(g["su"])
+                if ordered:
+                    g["done"].record(stream)
+                return
         adapters = self._adapters if adapter_ids is not None else None
         bounds, _ = general.run(self._general, l0, u0, spec_W, self.certifier, adapters, adapter_ids)
-        sl, su = general.state(l0, u0, bounds)
         lb.copy_(bounds[-1][0])
         ub.copy_(bounds[-1][1])
-        return lb, ub, sl, su
+        if state_l is not None:
+            sl, su = general.state(l0, u0, bounds)
+            state_l.copy_(sl)
+            state_u.copy_(su)
 
     def _capture(self, l0, u0, spec_W, adapter_ids, key):
         from . import general
         static = {"l0": l0.clone(), "u0": u0.clone(), "W": spec_W.clone(),
-                  "ids": None if adapter_ids is None else adapter_ids.clone()}
+                  "ids": None if adapter_ids is None else adapter_ids.clone(), "done": torch.cuda.Event()}
         variant = (self._adapters if adapter_ids is not None else None, static["ids"])
         try:
             side = torch.cuda.Stream(self.device)

@@ -289,3 +289,28 @@ def test_a_device_without_an_index_is_the_current_one():
     want = engine(wl, adapters).run(*box, nets.spec_weight(y).cuda(), adapter_ids=ids.cuda())
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     eng.answer(*box, y.cuda(), ops.AnswerRules(l0.shape[0], 10), adapter_ids=ids.cuda())
+
+
+@pytest.mark.parametrize("want_state", [False, True])
+def test_calls_on_two_streams(want_state):
+    """Calls of one engine on streams of their own, neither waited for: each has its own inputs' bounds."""
+    from cfgpu import nets
+    wl, y, l0, u0, adapters, ids = make(B=48)
+    eng = engine(wl, adapters)
+    spec, ids = nets.spec_weight(y).to(dev()), ids.to(dev())
+    inputs = []
+    for k in range(2):
+        inputs.append(((l0 - 0.1 * k).to(dev()), (u0 + 0.1 * k).to(dev()), spec, want_state))
+    want = [[t.clone() for t in eng.run(*a, adapter_ids=ids.roll(k))] for k, a in enumerate(inputs)]
+    assert not torch.equal(want[0][0], want[1][0])
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    rolled = [ids.roll(k) for k in range(2)]
+    torch.cuda.synchronize()
+    for turn in range(10):
+        got = []
+        for k in range(2):
+            with torch.cuda.stream(streams[k]):
+                got.append(eng.run(*inputs[k], adapter_ids=rolled[k]))
+        torch.cuda.synchronize()
+        for k in range(2):
+            assert all(torch.equal(g, w) for g, w in zip(got[k], want[k])), (turn, k)
