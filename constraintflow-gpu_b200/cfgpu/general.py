@@ -84,9 +84,25 @@ class _Adapted:
         return out.view(B, r, self.layer.n_in)
 
     def dense(self):
-        n = self.layer.n_out
-        eye = torch.eye(n, dtype=F32, device=self.ids.device)
-        return self.apply(eye.expand(self.shape[0], n, n))
+        """[B, n_out, n_in]: W as it is, and scale_e B_e A_e added in float32 where the region has
+        an adapter (through apply, a product with the identity, W would keep 3xTF32's 22 bits)."""
+        W, A, B, scale, ranks, _ = self.layer._keep
+        n_adapters, rank = self.layer.n_adapters, self.layer.rank
+        if n_adapters == 0 or rank == 0:
+            return W.expand(self.shape)
+        e = self.ids.clamp(0, n_adapters - 1).long()
+        own = torch.full_like(e, rank) if ranks is None else ranks.clamp(0, rank)[e].long()
+        own = own * (self.ids == e)
+        used = torch.arange(rank, device=e.device) < own[:, None]      # [B, rank]
+        # what is not used may be anything, NaN included
+        Ae = _kept(used[:, :, None], A[e])
+        Be = _kept(used[:, None, :], ops.binary(operator.mul, B[e], scale[e][:, None, None].expand_as(B[e]), F32))
+        return _add(W.expand(self.shape), ops.bmm(Be, Ae))
+
+
+def _kept(used, t):
+    """t where `used`, else 0."""
+    return ops.where(used.expand(t.shape), t, ops.scalar_view(0.0, tuple(t.shape), F32))
 
 
 def _full(B, t):
@@ -339,7 +355,8 @@ def run(layers, l0, u0, spec_W, relaxation="deeppoly", adapters=None, adapter_id
         else:
             raise NotImplementedError(f"a {kind} layer in the general traversal (it runs linear, conv, relu, add "
                                       "and concat layers)")
-        res = [_traverse(B, {ks[0]: A0}, c0, polys, lower) for lower in (True, False)]
+        first = A0.dense() if isinstance(A0, _Adapted) else A0      # once for both traversals
+        res = [_traverse(B, {ks[0]: first}, c0, polys, lower) for lower in (True, False)]
         bnd[k] = (res[0], res[1])
         poly = ({ks[0]: A0}, c0)
         polys[k] = (poly, poly)

@@ -314,3 +314,48 @@ def test_calls_on_two_streams(want_state):
         torch.cuda.synchronize()
         for k in range(2):
             assert all(torch.equal(g, w) for g, w in zip(got[k], want[k])), (turn, k)
+
+
+def test_dense_weights_of_the_variants():
+    """The weights that a traversal starts from: the shared ones bit for bit without an adapter (also
+    where unused adapters hold NaN), else within the float32 roundings of R products, their sums, the
+    scale and the last addition: (R + 3) 2^-24 of the magnitudes, doubled for second-order terms."""
+    from cfgpu import general, ops
+    g = torch.Generator()
+    g.manual_seed(5)
+    n_out, n_in, R = 37, 53, 6
+    W, A, B = (torch.randn(*s, generator=g) for s in ((n_out, n_in), (4, R, n_in), (4, n_out, R)))
+    scale, ranks = torch.rand(4, generator=g) + 0.5, torch.tensor([R, 2, 0, 99], dtype=torch.int32)
+    A[1, 2:], B[1, :, 2:], A[2], B[2] = math.nan, math.inf, math.nan, math.nan
+    ids = torch.tensor([0, -1, 1, 2, 3, 4, -7, 0], dtype=torch.int32)
+    layer = ops.AdapterLayer(*(t.to(dev()) for t in (W, A, B, scale, ranks)))
+    D = general._Adapted(layer, ids.to(dev())).dense().cpu()
+    assert tuple(D.shape) == (8, n_out, n_in)
+    for b, e in enumerate(ids.tolist()):
+        r = min(R, int(ranks[e])) if 0 <= e < 4 else 0
+        if r == 0:
+            assert torch.equal(D[b], W)
+            continue
+        low = float(scale[e]) * B[e, :, :r].double() @ A[e, :r].double()
+        size = float(scale[e]) * B[e, :, :r].double().abs() @ A[e, :r].double().abs() + W.double().abs()
+        assert ((D[b].double() - W.double() - low).abs() <= 2 * (R + 3) * 2.0**-24 * size).all()
+    bad = [t.clone() for t in (A, B, scale)]
+    bad[0][0], bad[1][0], bad[2][0] = math.nan, math.inf, math.nan      # the one that ids below 0 clamp to
+    layer = ops.AdapterLayer(W.to(dev()), *(t.to(dev()) for t in bad))
+    none = general._Adapted(layer, torch.tensor([-1, 9], dtype=torch.int32, device=dev())).dense().cpu()
+    assert torch.equal(none[0], W) and torch.equal(none[1], W)
+
+
+def test_without_an_adapter_the_first_bounds_are_the_networks():
+    """Regions of no adapter, beside others: the first layer's bounds are those of the same traversal
+    of the network itself, bit for bit."""
+    from cfgpu import general, nets
+    wl, y, l0, u0, adapters, ids = make(adapted=(0,))
+    eng = engine(wl, adapters)
+    box, spec = (l0.to(dev()), u0.to(dev())), nets.spec_weight(y).to(dev())
+    some, _ = general.run(eng._general, *box, spec, "deeppoly", eng._adapters, ids.to(dev()))
+    plain, _ = general.run(eng._general, *box, spec, "deeppoly")
+    rows = ids == -1
+    assert rows.any()
+    for got, want in zip(some[0], plain[0]):
+        assert torch.equal(got.cpu()[rows], want.cpu()[rows])
