@@ -749,3 +749,42 @@ def test_rules_on_two_streams_at_once():
             same(g[0], w[0])
             same(g[1], w[1])
             assert torch.equal(g[2].cpu(), w[2])
+
+
+@pytest.mark.parametrize("adapted", [False, True])
+@pytest.mark.parametrize("sub", [False, True])
+@pytest.mark.parametrize("K", [1027, 4096])
+def test_float32_precision_of_long_contractions(K, sub, adapted):
+    """The error of whole results, which the bounds of single values above do not hold to what
+    emptying the accumulator gives.  Relative to the root mean square of y, for independent terms:
+
+    * a chunk of 64 columns is 24 additions that truncate, each by half of 2^-23 of its partial sum on
+      average; partial sums grow as a root, so the 24 make at most 2/3 * 24 * 2^-24 of the chunk's, and the
+      chunks' together at most that of y's;
+    * hi + lo keeps 22 bits of each operand and lo * lo is left out: 2^-22 of a product;
+    * the chunks' sums are added with rounding: 2^-25 * sqrt(K / 64) at K = 4096, less than 2^-22.
+
+    16 * 2^-24 + 2 * 2^-22 in all (1.4e-6), twice for the chained low-rank part.  Without
+    chunks the first term would be K / 64 times that, one TF32 product would be off by 2^-11."""
+    T, N, R, Q = 1100, 384, 32, 3
+    t = make(T, K, N, R, 2, Q, F32, sub, seed=K)
+    if not adapted:
+        t["ids"] = torch.full((Q,), -1, dtype=torch.int32)
+    d = {k: t[k].cuda() for k in ("x", "W", "A", "B")}
+    got = ops().adapter_matmul(d["x"], layer(t), t["offsets"].cuda(), t["ids"].cuda(), substitute=sub)
+    d = {k: v.double() for k, v in d.items()}
+    base = d["x"] @ (d["W"] if sub else d["W"].t())
+    low = torch.zeros_like(base)
+    for q, e in enumerate(t["ids"].tolist()):
+        a, b = int(t["offsets"][q]), int(t["offsets"][q + 1])
+        if e >= 0:
+            P, O = (d["B"][e], d["A"][e]) if sub else (d["A"][e].t(), d["B"][e].t())
+            low[a:b] = float(t["scale"][e]) * (d["x"][a:b] @ P) @ O
+
+    def rms(z):
+        return float(z.square().mean().sqrt())
+    off = got.double() - base - low
+    allowed = (16 * 2.0**-24 + 2 * 2.0**-22) * (rms(base) + 2 * rms(low))
+    assert rms(off) <= allowed, (rms(off) / allowed, rms(off) / rms(base + low))
+    towards_zero = float((off * (base + low).sign()).mean())
+    assert abs(towards_zero) <= allowed, (towards_zero / allowed)
