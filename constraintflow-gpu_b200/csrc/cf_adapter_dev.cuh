@@ -15,18 +15,18 @@ __device__ __forceinline__ uint32_t idesc(uint32_t ab, uint32_t n, bool mn_major
 }
 
 template <typename T>
-struct Kind;  // of a type: elements in 128 bytes, planes of an operand, descriptor type
+struct Kind;  // of a type: elements in 128 bytes, descriptor type
 template <>
 struct Kind<float> {
-  static constexpr int kStep = 32, kPlanes = 2, kAb = 2;
+  static constexpr int kStep = 32, kAb = 2;
 };
 template <>
 struct Kind<__nv_bfloat16> {
-  static constexpr int kStep = 64, kPlanes = 1, kAb = 1;
+  static constexpr int kStep = 64, kAb = 1;
 };
 template <>
 struct Kind<__half> {
-  static constexpr int kStep = 64, kPlanes = 1, kAb = 0;
+  static constexpr int kStep = 64, kAb = 0;
 };
 
 // Loads that stay where they are written, zeros where not `ok`: a thread has two steps' loads in
@@ -65,25 +65,19 @@ __device__ __forceinline__ uint4 load16(const T* row, int64_t k, int64_t n_k, bo
   return *(const uint4*)t;
 }
 
-// a 16-byte chunk of one operand row into its plane(s)
-template <typename T>
+// a 16-byte chunk of one float32 operand row into its planes hi and lo
 __device__ __forceinline__ void put(uint32_t plane, uint32_t plane_bytes, uint32_t row, uint32_t chunk, uint4 d) {
   const uint32_t at = plane + row * 128u + ((chunk ^ (row & 7u)) << 4);
-  if constexpr (Kind<T>::kPlanes == 2) {
-    float hi[4], lo[4];
-    tc::split_tf32(__uint_as_float(d.x), hi[0], lo[0]);
-    tc::split_tf32(__uint_as_float(d.y), hi[1], lo[1]);
-    tc::split_tf32(__uint_as_float(d.z), hi[2], lo[2]);
-    tc::split_tf32(__uint_as_float(d.w), hi[3], lo[3]);
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(hi[0]), "f"(hi[1]), "f"(hi[2]), "f"(hi[3])
-                 : "memory");
-    asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + plane_bytes), "f"(lo[0]), "f"(lo[1]),
-                 "f"(lo[2]), "f"(lo[3])
-                 : "memory");
-  } else {
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(d.x), "r"(d.y), "r"(d.z), "r"(d.w)
-                 : "memory");
-  }
+  float hi[4], lo[4];
+  tc::split_tf32(__uint_as_float(d.x), hi[0], lo[0]);
+  tc::split_tf32(__uint_as_float(d.y), hi[1], lo[1]);
+  tc::split_tf32(__uint_as_float(d.z), hi[2], lo[2]);
+  tc::split_tf32(__uint_as_float(d.w), hi[3], lo[3]);
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(hi[0]), "f"(hi[1]), "f"(hi[2]), "f"(hi[3])
+               : "memory");
+  asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + plane_bytes), "f"(lo[0]), "f"(lo[1]), "f"(lo[2]),
+               "f"(lo[3])
+               : "memory");
 }
 
 // y columns n .. n+3 of row t

@@ -237,14 +237,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_adapter_f32(const Problem p, co
       if (!warp_wait(&bars.empty[s], (round & 1) ^ 1, err, 51, p.max_polls)) return false;
       const uint32_t a = sbase + s * kStageBytes, b = a + 2 * kABytes;
 #pragma unroll
-      for (int j = 0; j < kBM * 8 / kLoad; ++j) put<float>(a, kABytes, prow + j * (kLoad / 8), chunk, d.x[j]);
+      for (int j = 0; j < kBM * 8 / kLoad; ++j) put(a, kABytes, prow + j * (kLoad / 8), chunk, d.x[j]);
 #pragma unroll
       for (int j = 0; j < kBN * 8 / kLoad; ++j) {
         if constexpr (kSub) {
           const int task = j * kLoad + tid;
-          put<float>(b, kBBytes, task % kBN, task / kBN, d.b[j]);
+          put(b, kBBytes, task % kBN, task / kBN, d.b[j]);
         } else {
-          put<float>(b, kBBytes, prow + j * (kLoad / 8), chunk, d.b[j]);
+          put(b, kBBytes, prow + j * (kLoad / 8), chunk, d.b[j]);
         }
       }
       fence_proxy_async_smem();

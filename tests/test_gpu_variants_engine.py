@@ -359,3 +359,23 @@ def test_without_an_adapter_the_first_bounds_are_the_networks():
     assert rows.any()
     for got, want in zip(some[0], plain[0]):
         assert torch.equal(got.cpu()[rows], want.cpu()[rows])
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_adapters_are_exchanged_by_writing_into_them(graphs):
+    """Tensors on the engine's device are read at every call, also by a captured pass."""
+    from cfgpu import nets
+    wl, y, l0, u0, adapters, ids = make()
+    box, spec, ids = (l0.to(dev()), u0.to(dev())), nets.spec_weight(y).to(dev()), ids.to(dev())
+    held = {i: tuple(t.to(dev()) for t in a) for i, a in adapters.items()}
+    eng = engine(wl, held)
+    eng.graphs = graphs
+    before = eng.run(*box, spec, adapter_ids=ids)[0].clone()
+    other = make(seed=1)[4]
+    for i, a in held.items():
+        for t, n in zip(a, other[i]):
+            t.copy_(n)
+    fresh = engine(wl, other)
+    fresh.graphs = graphs
+    after = eng.run(*box, spec, adapter_ids=ids)[0]
+    assert torch.equal(after, fresh.run(*box, spec, adapter_ids=ids)[0]) and not torch.equal(after, before)
