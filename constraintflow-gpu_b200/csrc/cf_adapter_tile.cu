@@ -378,8 +378,11 @@ cf_status run(const Problem& p, int dtype, bool row_shrink, bool lowrank_tma, cu
     return launch_wide(p, dtype, kSub, maps, g.q_tma, g.x_rows, st);
   CF_TRY(encode_weights(p, dtype, kSub, bn, g.q_tma, &maps));
   g.split = split_for(g.units, steps);
-  // tiles for more than half of the SMs: three CTAs a tile, two an SM (86 tiles: 25.2 us, 28.6 with one)
-  if (g.units > 64 && g.units <= 88 && steps >= 12) g.split = 3;
+  // Tiles for more than half of the SMs: three CTAs a tile, two an SM, where the contraction repays the
+  // sums (66 / 88 tiles, us with three and with one: K = 4096 27.1 and 30.4 / 30.2 and 32.5, 2560 20.9 and 21.5 / 21.6
+  // and 21.9, 2048 18.8 and 18.5 / 20.0 and 18.6, 768 13.9 and 10.5 / 14.1 and 10.5).  From 89 tiles on two an SM do
+  // not hold all CTAs at once.
+  if (g.units > 64 && g.units <= 88 && steps >= 36) g.split = 3;
   return launch<T, kSub, false, bn, kStages>("k_adapter_tile", p, maps, g, g.units, st);
 }
 
