@@ -292,8 +292,10 @@ def adapter_matmul(x, layer, offsets, ids, substitute=False, out=None):
     offsets [n_requests + 1] int64: the rows of request q are offsets[q] .. offsets[q+1]-1;
     ids [n_requests] int32: its adapter, any value outside 0 .. n_adapters-1 none.  Both are
     read on the device, without a synchronisation.  Rows of no request are left as they were in
-    `out`, and are 0 in a new result.  `out` must not overlap x.  What meets an infinity comes out
-    as an infinity or NaN, in rows of that request only."""
+    `out`, and are 0 in a new result (filled first: a launch and a write more than with `out`).  `out`
+    must not overlap x.  What meets an infinity comes out as an infinity or NaN, in rows of that
+    request only.  No gradient is recorded: substitute gives the input's, those of the weights and
+    adapters are the caller's products."""
     dev, gpu, dt = layer.device, layer.gpu, layer.dtype
     K, N = (layer.n_out, layer.n_in) if substitute else (layer.n_in, layer.n_out)
     if x.dim() == 2 and x.stride(1) != 1:
@@ -418,7 +420,7 @@ def _rules_rows(name, t, rules, dtype, gpu):
 
 def edit_logits(logits, rules, out=None):
     """The rules applied to logits [rows, n] (float32, bfloat16, float16), in float32, rounded
-    once to the logits' dtype; `out` may be the logits themselves."""
+    once to the logits' dtype; `out` may be the logits themselves.  No gradient is recorded."""
     dt = logits.dtype
     if dt not in _DTYPES:
         raise NotImplementedError(f"logits of {dt} (float32, bfloat16 and float16 are supported)")

@@ -65,7 +65,9 @@ bool few_rows(const cf_adapter_layer& L, bool substitute, int64_t T) {
 }
 
 // With few rows a request, a tile of the tensor cores would be multiplied once for each of its
-// requests: v row by row on the CUDA cores instead.
+// requests: v row by row on the CUDA cores instead.  The mean decides for all rows, empty requests
+// included: 4000 rows of one request take 127 us (4096 x 4096 bfloat16, rank 16), 241 beside 300 requests
+// of one row, 202 beside 300 of none.
 bool rows_alone(int64_t T, int64_t n_requests) { return T < 16 * n_requests; }
 
 // The workspace's parts, from `base` on (NULL: only their sizes are asked for); returns its bytes.

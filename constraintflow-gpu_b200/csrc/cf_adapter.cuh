@@ -171,6 +171,8 @@ __device__ __forceinline__ void plan_tile(const Problem& p, int64_t m, int whole
   }
 }
 
+// For the tensor cores v is a bfloat16 pair: 16 bits of it, off by 2^-16 at most where the result is
+// rounded to 2^-8, for two passes of Q_e (float32 itself would take three).
 __device__ __forceinline__ void store_v(const Problem& p, int64_t t, int r, float v) {
   p.v[t * p.v_rs + r] = v;
   if (p.v_hi) {

@@ -7,8 +7,9 @@
 // core adds into its accumulator with truncation, an error that grows with every addition and
 // always points towards zero, so a sum stays in the accumulator for kChunk steps of 32 only; the
 // epilogue's warps add the chunks in registers, rounded to nearest.  The error of a sum is then
-// that of 24 truncated additions of a chunk, not of 3 K / 8: against 64 bits about that of a
-// float32 FMA loop.
+// that of 24 truncated additions of a chunk, not of 3 K / 8.  It is above that of float32 FMAs all the
+// same, as an operand keeps 22 bits and lo*lo is left out: 4.6e-7 of y against 64 bits where FMAs are
+// 2.6e-7 off (51200 x 200 x 784).
 //
 // The chunks also keep requests apart: the low-rank part of each request that reaches into the
 // tile is a chunk of its own, added to that request's rows only (a masked operand would not do:
@@ -21,10 +22,12 @@
 // with few tiles the contraction is dealt out to the CTAs of a cluster instead, which sum their
 // parts in rank order.
 //
-// 4096 x 4096 x 4096, rank 64: 925 us, 149 TFLOP/s, 0.54 of the rate of 3xTF32 alone (276): a step's images
+// 4096 x 4096 x 4096, rank 64: 971 us, 146 TFLOP/s, 0.53 of the rate of 3xTF32 alone (276): a step's images
 // are written, read for three products and loaded through the same 128 bytes a cycle of the SM, about
-// as long as its MMAs take to issue.  A third stage takes the L1 cache that the loads go through (1104 us).
-// 51200 x 200 x 784 with 256 requests of rank 8: 244 us, substituted 302, without adapters 162 and 178.
+// as long as its MMAs take to issue.  A third stage takes the L1 cache that the loads go through (1104 us, 975
+// with two at that time).
+// 51200 x 200 x 784 with 256 requests of rank 8: 257 us, substituted 283, without adapters 166 and 176.
+// About 3% of these times is the lanes' agreement on the outcome of each wait.
 #include <cooperative_groups.h>
 
 #include <type_traits>

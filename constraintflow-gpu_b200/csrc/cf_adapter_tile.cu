@@ -12,10 +12,12 @@
 //
 // Operands in shared memory are 128-byte-swizzled images, 128 bytes of the contraction a row:
 // loaded by tensor maps; M and Q_e with n contiguous (substitution) stay as they lie, as MN-major
-// images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.
+// images.  v is a bfloat16 pair (hi, lo), two passes of the same Q_e.  The accumulator truncates and is kept
+// for all of a CTA's steps, as in the wide tiles.
 //
-// 64 rows of 4096 x 4096, each with its own adapter of rank 16: 18.5 us, 47 MB at 2.5 TB/s: a chain of
-// launch, v, weights, sums and the rows' own adapters, each part waiting for the one before.
+// 64 rows of 4096 x 4096, each with its own adapter of rank 16: 19.0 us, 47 MB at 2.5 TB/s: a chain of
+// launch, v, weights, sums and the rows' own adapters.  Of these only v Q_e needs v: the adapters' rows
+// are still read behind the contraction, not under it.
 #include <cooperative_groups.h>
 
 #include "cf_adapter_tma.cuh"

@@ -15,8 +15,9 @@
 // What the history and the biases touch is little and is put right from their side, in the result
 // that the stream has left in the cache.  For 256 x 131072 bfloat16 and 1024 tokens a row: a lookup
 // for every answer on the way 228 us (some lane of nearly every warp edits), edits of each slice in
-// shared memory on its way 50, the stream 22 (134 MB: 0.94 of a copy's rate) and behind it the edits
-// 12: random reads and writes of single answers, each waiting on the last for its address.
+// shared memory on its way 50, the stream 21 (134 MB: 0.98 of a copy's rate, partly from the cache; 26
+// with a cold one) and behind it the edits 12: random reads and writes of single answers, each waiting on the
+// last for its address.
 //
 // Short histories go into a hash table of the answers they touch, one CTA a row, whatever the row's
 // length.  Long ones are counted slice by slice in tables of all answers: 16 bits an answer, seen
@@ -822,9 +823,12 @@ cf_status edit_logits(const cf_answer_rules& R, const void* in, int64_t in_rs, v
                   R, (const T*)in, in_rs, (T*)out, out_rs, chunks, units));
   }
   if (!has_edits(R)) return CF_OK;
-  // Rows of up to 2048 tokens on average: one small CTA a row, which counts while the stream runs.
-  // Longer ones: 32768 answers a slice (64 KB of tables, three CTAs an SM), fewer where that leaves
-  // SMs idle.
+  // Rows of up to 2048 tokens on average: one small CTA a row, which counts while the stream's last CTAs
+  // run (four of them leave an SM a quarter of its registers, half of what the smaller CTA takes).
+  // Longer ones: 32768 answers a slice (64 KB of tables; 1024 threads of 64 registers are an SM's), fewer
+  // where that leaves SMs idle.  The mean decides for all rows: 256 rows of 131072 bfloat16 take 29 us
+  // with 1000 tokens each and 204 if one of them has 32768, whose slices then go through one CTA (191
+  // if all have).
   const bool brief = R.n_tokens <= R.rows * 2048;
   int log_s = brief ? 14 : 15;
   if (!brief)

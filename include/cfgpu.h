@@ -442,7 +442,8 @@ cf_status cf_adapter_matmul(const cf_adapter_layer* layer, int32_t substitute, i
                             int64_t x_rs, int64_t n_requests, const int64_t* offsets_dev, const int32_t* ids_dev,
                             void* y_dev, int64_t y_rs, void* workspace_dev, size_t workspace_bytes, void* stream);
 /* Synchronise `stream` and report whether a bounded device-side wait of a cf_adapter_matmul on
- * the current device gave up (CF_ERR_TIMEOUT) since the last check; its rows are not valid. */
+ * the current device gave up (CF_ERR_TIMEOUT) since the last check; its rows are not valid.  Until
+ * then it is a record only: other calls run as usual. */
 cf_status cf_adapter_check(void* stream);
 
 /* The rule by which each of `rows` rows' answer is taken from its n logits:
