@@ -357,7 +357,8 @@ class DeepPolyEngine:
         to a logit, and the margin is taken from the property rows' bounds of y[label] - y[j], less
         what the additions to logits of that size may round by; with one, from the bounds of the
         logits themselves.  labels [B] int64 device tensor of answers in 0 .. n_last-1.  The property
-        rows take B (n_last - 1) n_last floats.  check_device as in run: without it a margin may come
+        rows take B (n_last - 1) n_last floats.  A margin proves as much as the certifier's bounds do:
+        CROWN's and DeepZ's programs are not sound in every case.  check_device as in run: without it a margin may come
         from bounds that a device wait gave up on."""
         from . import ops
         B, n = int(l0.shape[0]), self.n_last

@@ -379,3 +379,46 @@ def test_adapters_are_exchanged_by_writing_into_them(graphs):
     fresh.graphs = graphs
     after = eng.run(*box, spec, adapter_ids=ids)[0]
     assert torch.equal(after, fresh.run(*box, spec, adapter_ids=ids)[0]) and not torch.equal(after, before)
+
+
+@pytest.mark.parametrize("certifier", ["deeppoly", "crown", "zono", "ibp", "crownibp"])
+def test_answers_of_every_certifier(certifier):
+    """Biases and sets on the bounds of each certifier: the margin is the property's plus the edits
+    (whole numbers), less the allowance of 2^-21 of the magnitudes and their rounding, here 2^-17 of
+    them; and the values at points of a region keep it, up to the float32 error of the bounds.  Not
+    so CROWN's: its program takes one branch for a whole layer, and its property's bounds do not
+    hold at points either."""
+    from cfgpu import nets, ops
+    from cfgpu.engine import DeepPolyEngine
+    wl, y, l0, u0, _, _ = make()
+    B, n = l0.shape[0], 10
+    u0 = l0 + (u0 - l0) * 0.05
+    eng = DeepPolyEngine(wl.layers, wl.input_size, dev(), certifier=certifier)
+    box = l0.to(dev()), u0.to(dev())
+    kw, _ = rules_for(B, n, 3, False)
+    kw = {k: kw[k] for k in ("bias_ids", "bias_values", "bias_offsets", "allowed", "allowed_row")}
+    kw["bias_values"] = kw["bias_values"].round()
+    margin = eng.answer(*box, y.to(dev()), ops.AnswerRules(B, n, **{k: v.to(dev()) for k, v in kw.items()}))[0].cpu()
+    lb = eng.run(*box, nets.spec_weight(y).to(dev()))[0].cpu()
+    g = torch.Generator()
+    g.manual_seed(3)
+    edits = V.rules(torch.zeros(B, n), n, **kw)
+    for b in range(B):
+        z = l0[b].double() + (u0[b] - l0[b]).double() * torch.rand(40, l0.shape[1], generator=g).double()
+        logits = points(wl.layers, z)[-1]
+        label = int(y[b])
+        v = logits + edits[b]
+        others = v.clone()
+        others[:, label] = -math.inf
+        gap = v[:, label] - others.max(dim=1).values
+        gap[gap.isnan()] = -math.inf
+        size = logits.abs().max() + lb[b].abs().max() + edits[b][edits[b] > -math.inf].abs().sum()
+        if certifier != "crown":
+            assert (gap >= margin[b].double() - 1e-4 * size).all(), b
+        others = [j for j in range(n) if j != label]
+        want = min(float(lb[b, i] + edits[b, label] - edits[b, j]) if edits[b, label] > -math.inf else -math.inf
+                   for i, j in enumerate(others) if edits[b, j] > -math.inf)
+        if want == -math.inf:
+            assert margin[b] == -math.inf
+        else:
+            assert abs(float(margin[b]) - want) <= 2.0**-17 * float(size + 1), (b, float(margin[b]), want)
