@@ -260,19 +260,18 @@ class DeepPolyEngine:
 
         DeepPoly's traversal takes no data-dependent decision on the host, so for a given
         batch size its launches are captured once in a CUDA graph and replayed (the inputs
-        are copied into the graph's buffers, which a call on another stream waits for); CROWN
-        decides its ReLU branches on the host and runs eagerly."""
+        are copied into the graph's buffers, which a call on another stream waits for); a call
+        that is itself captured issues the launches into that graph.  CROWN decides its ReLU
+        branches on the host and runs eagerly."""
         from . import general
-        if self.certifier == "deeppoly" and self.graphs:
+        if self.certifier == "deeppoly" and self.graphs and not torch.cuda.is_current_stream_capturing():
             key = (int(l0.shape[0]), adapter_ids is not None)
             g = self._graph_cache.get(key)
             if g is None:
                 g = self._capture(l0, u0, spec_W, adapter_ids, key)
             if g is not None:
                 stream = torch.cuda.current_stream(self.device)
-                ordered = not torch.cuda.is_current_stream_capturing()
-                if ordered:
-                    stream.wait_event(g["done"])
+                stream.wait_event(g["done"])
                 g["l0"].copy_(l0)
                 g["u0"].copy_(u0)
                 g["W"].copy_(spec_W)
@@ -285,8 +284,7 @@ class DeepPolyEngine:
                 if state_l is not None:
                     state_l.copy_(g["sl"])
                     state_u.copy_(g["su"])
-                if ordered:
-                    g["done"].record(stream)
+                g["done"].record(stream)
                 return
         adapters = self._adapters if adapter_ids is not None else None
         bounds, _ = general.run(self._general, l0, u0, spec_W, self.certifier, adapters, adapter_ids)

@@ -422,3 +422,35 @@ def test_answers_of_every_certifier(certifier):
             assert margin[b] == -math.inf
         else:
             assert abs(float(margin[b]) - want) <= 2.0**-17 * float(size + 1), (b, float(margin[b]), want)
+
+
+@pytest.mark.parametrize("before", [True, False])
+def test_run_and_answer_in_a_callers_graph(before):
+    """Captured by the caller, with and without an eager call before it, and replayed on other inputs."""
+    from cfgpu import nets, ops
+    wl, y, l0, u0, adapters, ids = make()
+    eng, other = engine(wl, adapters), engine(wl, adapters)
+    box, spec, ids, y = (l0.to(dev()), u0.to(dev())), nets.spec_weight(y).to(dev()), ids.to(dev()), y.to(dev())
+    kw, rules = rules_for(l0.shape[0], 10, 3, False)
+    warm = engine(wl, adapters)                    # kernels' first uses
+    warm.run(*box, spec, adapter_ids=ids)
+    warm.answer(*box, y, rules, adapter_ids=ids)
+    if before:
+        eng.run(*box, spec, adapter_ids=ids)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lb, ub = eng.run(*box, spec, adapter_ids=ids)
+        margin, rival = eng.answer(*box, y, rules, adapter_ids=ids)
+    for turn in range(2):
+        if turn:
+            box[0].sub_(0.01)
+            ids.copy_(ids.roll(1))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = other.run(*box, spec, adapter_ids=ids)
+        assert torch.equal(lb, want[0]) and torch.equal(ub, want[1])
+        m, j = other.answer(*box, y, rules, adapter_ids=ids)
+        assert torch.equal(margin, m) and torch.equal(rival, j)
+    again = eng.run(*box, spec, adapter_ids=ids)   # the engine's own pass still is one
+    assert torch.equal(again[0], lb) and eng.graphs
