@@ -356,8 +356,8 @@ class DeepPolyEngine:
         what the additions to logits of that size may round by; with one, from the bounds of the
         logits themselves.  labels [B] int64 device tensor of answers in 0 .. n_last-1.  The property
         rows take B (n_last - 1) n_last floats.  A margin proves as much as the certifier's bounds do:
-        CROWN's and DeepZ's programs are not sound in every case.  check_device as in run: without it a margin may come
-        from bounds that a device wait gave up on."""
+        CROWN's and DeepZ's programs are not sound in every case.  check_device as in run: without
+        it a margin may come from bounds that a device wait gave up on."""
         from . import ops
         B, n = int(l0.shape[0]), self.n_last
         if (rules.rows, rules.n) != (B, n) or self.n_spec != n - 1:
